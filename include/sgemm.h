@@ -349,6 +349,37 @@ int sg_fp8_decode_rows(const uint8_t* Q, const float* scales, void* Y_bf16, int 
 int sg_fp8_reduce_rows(const uint8_t* Q, const float* scales, void* Y_bf16,
                        int nbuf, size_t q_buf_stride, int rows, int cols, void* stream);
 
+/* MXFP4: 4-bit weights and activations - no counterpart in the reference.  32 neighbouring columns of a row share a scale
+ * 2^(S - 127), one byte S (255 = NaN); every value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two
+ * codes a byte, the even column in the low nibble.  Codes are [rows][cols / 2], scales [rows][cols / 32], both contiguous;
+ * cols must be a multiple of 32.
+ *   encode: S = clamp(floor(log2(absmax of the block)) + 125, 0, 254), 127 for a block of zeros;
+ *           code = e2m1_rne_sat(X / 2^(S - 127)), a zero keeping the value's sign; a block that holds a NaN or an infinity
+ *           has S = 255 and codes 0                                       (bit exact)
+ *   decode: Y = bf16(e2m1(code) * 2^(S - 127)), NaN where S = 255.  Exact but for the two ends of the range: beyond bf16's
+ *           largest value an infinity.
+ * X, Q, Y must be 16-byte aligned; scales are bytes at any address. */
+int sg_mxfp4_encode_rows(const void* X_bf16, uint8_t* Q, uint8_t* scales, int rows, int cols, void* stream);
+int sg_mxfp4_decode_rows(const uint8_t* Q, const uint8_t* scales, void* Y_bf16, int rows, int cols, void* stream);
+
+/* Weights B [n][k] in MXFP4 (codes [n][k / 2] with row stride b_stride bytes, scales [n][k / 32]) laid out as the matrix
+ * instruction takes them: once, when a program loads them.  P: sg_mxfp4_packed_bytes(n, k) bytes of device memory (0 for an
+ * n or k that sg_mxfp4_pack refuses), 16-byte aligned; all of them are written.  B 16-byte aligned, b_stride a multiple of 16 and at least k / 2. */
+size_t sg_mxfp4_packed_bytes(int n, int k);
+int    sg_mxfp4_pack(const uint8_t* B, const uint8_t* B_scales, uint8_t* P, int n, int k, int b_stride, void* stream);
+
+/* Products with packed MXFP4 weights, overwriting D [m][n] in bf16:
+ *     sg_mxfp4_gemm         D = bf16( (sum_k A[i][k]*B[j][k]) * scale ),  A [m][k] in MXFP4 (sg_mxfp4_encode_rows)
+ *     sg_mxfp4_gemm_fp8act  D = bf16( ((sum_k A[i][k]*B[j][k]) * scale) * row_scales[i] ),  A [m][k] in E4M3
+ *                           (sg_fp8_encode_rows, whose scales are row_scales)
+ * with fp32 sums in a fixed order and separately rounded fp32 products.  scale_tensor (one float) and row_scales ([m] floats) may be
+ * NULL (factor 1).  Any m and n, k a multiple of 32; A and P 16-byte, D 8-byte aligned, A_scales at any address.  A NaN in an operand
+ * (a block scale of 255, an E4M3 NaN) makes the outputs of its row or column NaN.  P must come from sg_mxfp4_pack with the same n and k. */
+int sg_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D_bf16, const float* scale_tensor,
+                  int m, int n, int k, void* stream);
+int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const float* scale_tensor, const float* row_scales,
+                         int m, int n, int k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,6 +72,12 @@ SIGNATURES = {
     "sg_fp8_encode_rows": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
     "sg_fp8_decode_rows": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
     "sg_fp8_reduce_rows": (_i, [_vp, _vp, _vp, _i, _sz, _i, _i, _vp]),
+    "sg_mxfp4_encode_rows": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
+    "sg_mxfp4_decode_rows": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
+    "sg_mxfp4_packed_bytes": (_sz, [_i, _i]),
+    "sg_mxfp4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "sg_mxfp4_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "sg_mxfp4_gemm_fp8act": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():

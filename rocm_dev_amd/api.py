@@ -526,3 +526,123 @@ def fp8_reduce_rows(Q, scales, Y, check=False):
         rc = lib.sg_fp8_reduce_rows(_dev(Q, *_FP8), _dev(scales, torch.float32), _dev(Y, torch.bfloat16),
                                     nbuf, Q.stride(0), rows, cols, _stream())
     return _done(rc, check)
+
+
+# MXFP4 (include/sgemm.h): codes two a byte, one scale byte per 32 columns.
+def _mx_operands(X, Q, scales):
+    if X.dim() != 2 or X.shape[1] % 32:
+        raise ValueError("the bf16 matrix must be [rows, cols] with cols a multiple of 32, got %s" % (tuple(X.shape),))
+    rows, cols = X.shape
+    _mx_codes(Q, scales, rows, cols, ("Q", "scales"))
+    _row_major(X, "the bf16 matrix")
+    _same_device(X, Q, scales)
+    return rows, cols
+
+
+def _mx_codes(Q, scales, rows, cols, names):
+    if tuple(Q.shape) != (rows, cols // 2) or tuple(scales.shape) != (rows, cols // 32):
+        raise ValueError("%s must be [%d, %d] and %s [%d, %d], got %s and %s"
+                         % (names[0], rows, cols // 2, names[1], rows, cols // 32, tuple(Q.shape), tuple(scales.shape)))
+    _row_major(Q, names[0])
+    _row_major(scales, names[1])
+
+
+def mxfp4_encode_rows(X, Q, scales, check=False):
+    """X [rows, cols] bfloat16 -> Q [rows, cols/2] codes and scales [rows, cols/32], both uint8."""
+    rc = host.mxfp4_encode_rows(X, Q, scales)
+    if rc is not None:
+        return _done(rc, check)
+    rows, cols = _mx_operands(X, Q, scales)
+    with torch.cuda.device(X.device):
+        rc = lib.sg_mxfp4_encode_rows(_dev(X, torch.bfloat16), _dev(Q, torch.uint8), _dev(scales, torch.uint8), rows, cols, _stream())
+    return _done(rc, check)
+
+
+def mxfp4_decode_rows(Q, scales, Y, check=False):
+    """Q [rows, cols/2] codes and scales [rows, cols/32] -> Y [rows, cols] bfloat16."""
+    rc = host.mxfp4_decode_rows(Q, scales, Y)
+    if rc is not None:
+        return _done(rc, check)
+    rows, cols = _mx_operands(Y, Q, scales)
+    with torch.cuda.device(Q.device):
+        rc = lib.sg_mxfp4_decode_rows(_dev(Q, torch.uint8), _dev(scales, torch.uint8), _dev(Y, torch.bfloat16), rows, cols, _stream())
+    return _done(rc, check)
+
+
+def mxfp4_packed_bytes(n, k):
+    """Bytes of the packed form of an n x k weight matrix (k a multiple of 32)."""
+    need = lib.sg_mxfp4_packed_bytes(n, k)
+    if need == 0:
+        raise ValueError("packed weights need n > 0 and k a positive multiple of 32, got n = %d, k = %d" % (n, k))
+    return need
+
+
+def mxfp4_pack(B, B_scales, P, check=False):
+    """Weights B [n, k/2] codes (rows at any stride that 16 divides) with scales [n, k/32] -> P, a contiguous uint8 vector of
+    mxfp4_packed_bytes(n, k) that the GEMMs read.  Once per weight matrix."""
+    if B.dim() != 2 or B.shape[1] % 16:
+        raise ValueError("B must be [n, k/2] with k a multiple of 32, got %s" % (tuple(B.shape),))
+    n, k = B.shape[0], 2 * B.shape[1]
+    b_stride = _weights(B, k // 2)
+    if tuple(B_scales.shape) != (n, k // 32):
+        raise ValueError("B_scales must be [%d, %d], got %s" % (n, k // 32, tuple(B_scales.shape)))
+    _row_major(B_scales, "B_scales")
+    _packed(P, n, k)
+    _same_device(B, B_scales, P)
+    with torch.cuda.device(B.device):
+        rc = lib.sg_mxfp4_pack(_dev(B, torch.uint8), _dev(B_scales, torch.uint8), _dev(P, torch.uint8), n, k, b_stride, _stream())
+    return _done(rc, check)
+
+
+def _packed(P, n, k):
+    need = mxfp4_packed_bytes(n, k)
+    if P.dim() != 1 or P.numel() != need or not P.is_contiguous():
+        raise ValueError("P must be a contiguous vector of %d bytes (%d x %d weights packed), got shape %s strides %s"
+                         % (need, n, k, tuple(P.shape), tuple(P.stride())))
+
+
+def _mx_gemm(A, k, P, D, scale_tensor, extra):
+    if A.dim() != 2 or D.dim() != 2 or D.shape[0] != A.shape[0]:
+        raise ValueError("A and D must be matrices of as many rows, got %s and %s" % (tuple(A.shape), tuple(D.shape)))
+    m, n = D.shape
+    _packed(P, n, k)
+    _row_major(A, "A")
+    _row_major(D, "D")
+    if scale_tensor is not None and (scale_tensor.numel() < 1 or not scale_tensor.is_contiguous()):
+        raise ValueError("scale_tensor must hold at least one float")
+    _same_device(A, P, D, scale_tensor, *extra)
+    return m, n
+
+
+def mxfp4_gemm(A, A_scales, P, D, scale_tensor=None, check=False):
+    """D[m,n] = bf16(scale * A @ B^T), A [m, k/2] codes with A_scales [m, k/32] (mxfp4_encode_rows), B packed into P
+    (mxfp4_pack)."""
+    rc = host.mxfp4_gemm(A, A_scales, P, D, scale_tensor)
+    if rc is not None:
+        return _done(rc, check)
+    if A.dim() != 2 or A.shape[1] % 16:
+        raise ValueError("A must be [m, k/2] with k a multiple of 32, got %s" % (tuple(A.shape),))
+    k = 2 * A.shape[1]
+    _mx_codes(A, A_scales, A.shape[0], k, ("A", "A_scales"))
+    m, n = _mx_gemm(A, k, P, D, scale_tensor, (A_scales,))
+    with torch.cuda.device(A.device):
+        rc = lib.sg_mxfp4_gemm(_dev(A, torch.uint8), _dev(A_scales, torch.uint8), _dev(P, torch.uint8), _dev(D, torch.bfloat16),
+                               None if scale_tensor is None else _dev(scale_tensor, torch.float32), m, n, k, _stream())
+    return _done(rc, check)
+
+
+def mxfp4_gemm_fp8act(A, P, D, scale_tensor=None, row_scales=None, check=False):
+    """D[m,n] = bf16((scale * A @ B^T) * row_scales[:, None]), A [m, k] E4M3 (fp8_encode_rows), B packed into P (mxfp4_pack)."""
+    rc = host.mxfp4_gemm_fp8act(A, P, D, scale_tensor, row_scales)
+    if rc is not None:
+        return _done(rc, check)
+    if A.dim() != 2 or A.shape[1] % 32:
+        raise ValueError("A must be [m, k] with k a multiple of 32, got %s" % (tuple(A.shape),))
+    k = A.shape[1]
+    m, n = _mx_gemm(A, k, P, D, scale_tensor, (row_scales,))
+    _vector(row_scales, m, "row_scales")
+    with torch.cuda.device(A.device):
+        rc = lib.sg_mxfp4_gemm_fp8act(_dev(A, *_FP8), _dev(P, torch.uint8), _dev(D, torch.bfloat16),
+                                      None if scale_tensor is None else _dev(scale_tensor, torch.float32),
+                                      None if row_scales is None else _dev(row_scales, torch.float32), m, n, k, _stream())
+    return _done(rc, check)

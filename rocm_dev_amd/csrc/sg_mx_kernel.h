@@ -1,0 +1,190 @@
+// Products with MXFP4 weights for up to 64 activation rows:  D[m,n] = bf16(scale * row[m] * sum_k A[m,k] * B[n,k]).
+//
+// What bounds it is the stream of weights, 17/32 byte a value.  A wave takes NF 16-row weight tiles and MF 16-row activation
+// tiles and walks a part of K in steps of 128 columns: operands go from memory to the registers of
+// v_mfma_scale_f32_16x16x128_f8f6f4 as they lie - the weights by contiguous KBs of the packed buffer (sg_mx.h), the
+// activations row by row out of the L2.  A step's registers are loaded again for the step four steps on as soon as its
+// products are issued, so a wave keeps four steps in flight.  The waves of a workgroup share K by groups of four steps and
+// meet in LDS, partial sums added in wave order: the result does not depend on which wave is first.
+//
+// The instruction multiplies every block of 32 products by both operands' scales exactly and adds in 32 bits; E4M3
+// activations take the scale 1.  Inside a run of 8 E4M3 products it cuts products off about 14 binades below the largest
+// (as it does for E4M3 weights).
+#pragma once
+
+#include "sg_mx.h"
+
+namespace sg {
+
+// D += W x X with the scale bytes T of ws and XT of xs.  FP4: codes in the low 16 bytes of x.
+template <bool FP4, int T, int XT>
+__device__ __forceinline__ f32x4 mfma_mx(const i32x4 w, const i32x8 x, const f32x4 c, int ws, int xs) {
+    const i32x8 w8 = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x, c, 4, FP4 ? 4 : 0, T, ws, XT, xs);
+}
+
+// four consecutive n of row m_idx, at n_idx = a multiple of 4
+__device__ __forceinline__ void mx_store4(const MxArgs& a, int m_idx, int n_idx, f32x4 v) {
+    uint16_t* const d = a.D + (size_t)m_idx * a.n + n_idx;
+    const uint32_t lo = pack_bf16x2(v[0], v[1]), hi = pack_bf16x2(v[2], v[3]);
+    if ((a.n & 3) == 0) {
+        *reinterpret_cast<u32x2*>(d) = u32x2{lo, hi};
+    } else if ((a.n & 1) == 0) {
+        *reinterpret_cast<uint32_t*>(d) = lo;
+        if (n_idx + 2 < a.n) *reinterpret_cast<uint32_t*>(d + 2) = hi;
+    } else {
+        d[0] = (uint16_t)lo;
+        if (n_idx + 1 < a.n) d[1] = (uint16_t)(lo >> 16);
+        if (n_idx + 2 < a.n) d[2] = (uint16_t)hi;
+        if (n_idx + 3 < a.n) d[3] = (uint16_t)(hi >> 16);
+    }
+}
+
+template <bool FP4, int NF, int MF>
+__global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [waves][NF * MF][64 lanes] f32x4
+    const int lane = lane_id(), r = lane & 15, g = lane >> 4;
+    const int wave = wave_id(), waves = (int)(blockDim.x >> 6);
+    const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int tn = at / a.m_groups, tm = at - tn * a.m_groups;
+    const int k_blocks = a.k / kMxBlock;
+
+    // ---- operands: lane (r, g) ----
+    const uint8_t* wp[NF];
+    const uint8_t* wsp[NF];
+#pragma unroll
+    for (int i = 0; i < NF; i++) {
+        const int tile = tn * NF + i < a.tiles ? tn * NF + i : a.tiles - 1;      // beyond the last tile: it again, not stored
+        wp[i] = a.P + (size_t)tile * a.steps * kMxStepBytes + lane * 16;
+        wsp[i] = a.PS + (size_t)tile * a.quads * kMxQuadBytes + lane * 4;
+    }
+    const uint8_t* xp[MF];
+    const uint8_t* xsp[MF];
+#pragma unroll
+    for (int j = 0; j < MF; j++) {
+        const int row = (tm * MF + j) * 16 + r < a.m ? (tm * MF + j) * 16 + r : a.m - 1;
+        xp[j] = a.A + (size_t)row * (FP4 ? a.k / 2 : a.k);
+        xsp[j] = FP4 ? a.SA + (size_t)row * k_blocks : nullptr;
+    }
+
+    i32x4 w[4][NF], x[4][MF][FP4 ? 1 : 2];
+    int ws[NF], xs[MF][4], ws_next[NF], xs_next[MF][4];
+    f32x4 acc[NF][MF];
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // Step t of group q.  A step beyond the matrix takes the last one again (never multiplied), a piece of a row beyond its
+    // end the last piece (its weights are zero).
+    auto load_step = [&](int q, int t) __attribute__((always_inline)) {
+        const int step = 4 * q + t < a.steps ? 4 * q + t : a.steps - 1;
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+            w[t][i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp[i] + (size_t)step * kMxStepBytes));
+#pragma unroll
+        for (int j = 0; j < MF; j++) {
+            if (FP4) {
+                const int p = 4 * step + g < k_blocks ? 4 * step + g : k_blocks - 1;
+                x[t][j][0] = *reinterpret_cast<const i32x4*>(xp[j] + (size_t)p * 16);
+            } else {
+                // E4M3 columns of a lane: 16 from 16 * g on and 16 from 64 + 16 * g on
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int c = 8 * step + 4 * h + g, p = c < 2 * k_blocks ? c : 2 * k_blocks - 1;
+                    x[t][j][h] = *reinterpret_cast<const i32x4*>(xp[j] + (size_t)p * 16);
+                }
+            }
+        }
+    };
+    auto load_scales = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NF; i++) ws_next[i] = *reinterpret_cast<const int*>(wsp[i] + (size_t)q * kMxQuadBytes);
+        if (FP4) {
+#pragma unroll
+            for (int j = 0; j < MF; j++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int b = 16 * q + 4 * t + g;
+                    xs_next[j][t] = xsp[j][b < k_blocks ? b : k_blocks - 1];
+                }
+        }
+    };
+    auto multiply = [&](auto tc) __attribute__((always_inline)) {
+        constexpr int t = decltype(tc)::value;
+#pragma unroll
+        for (int j = 0; j < MF; j++) {
+            const i32x8 x8 = FP4 ? __builtin_shufflevector(x[t][j][0], x[t][j][0], 0, 1, 2, 3, -1, -1, -1, -1)
+                                 : __builtin_shufflevector(x[t][j][0], x[t][j][FP4 ? 0 : 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int i = 0; i < NF; i++) acc[i][j] = mfma_mx<FP4, t, 0>(w[t][i], x8, acc[i][j], ws[i], FP4 ? xs[j][t] : 127);
+        }
+    };
+    auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NF; i++) ws[i] = ws_next[i];
+#pragma unroll
+        for (int j = 0; j < MF; j++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) xs[j][t] = xs_next[j][t];
+    };
+    using T0 = std::integral_constant<int, 0>;
+    using T1 = std::integral_constant<int, 1>;
+    using T2 = std::integral_constant<int, 2>;
+    using T3 = std::integral_constant<int, 3>;
+
+    int q = wave;
+    if (q < a.quads) {
+        load_scales(q);
+#pragma unroll
+        for (int t = 0; t < 4; t++) load_step(q, t);
+        for (; q + waves < a.quads; q += waves) {
+            take_scales();
+            load_scales(q + waves);
+            multiply(T0{});
+            load_step(q + waves, 0);
+            multiply(T1{});
+            load_step(q + waves, 1);
+            multiply(T2{});
+            load_step(q + waves, 2);
+            multiply(T3{});
+            load_step(q + waves, 3);
+        }
+        take_scales();
+        const int left = a.steps - 4 * q;        // steps of the wave's last group
+        multiply(T0{});
+        if (left > 1) multiply(T1{});
+        if (left > 2) multiply(T2{});
+        if (left > 3) multiply(T3{});
+    }
+
+    // ---- the waves' sums, in wave order ----
+    const float scale = a.scale ? a.scale[0] : 1.0f;
+    auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) {
+        const int m_idx = (tm * MF + j) * 16 + r, n_idx = (tn * NF + i) * 16 + 4 * g;
+        if (m_idx >= a.m || n_idx >= a.n) return;
+        v *= scale;
+        if (a.row_scale) v *= a.row_scale[m_idx];
+        mx_store4(a, m_idx, n_idx, v);
+    };
+    if (waves == 1) {
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int j = 0; j < MF; j++) finish(acc[i][j], i, j);
+        return;
+    }
+    f32x4* const part = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) part[(wave * NF * MF + i * MF + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int f = wave; f < NF * MF; f += waves) {
+        f32x4 v = part[f * 64 + lane];
+        for (int u = 1; u < waves; u++) v += part[(u * NF * MF + f) * 64 + lane];
+        finish(v, f / MF, f % MF);
+    }
+}
+
+}  // namespace sg

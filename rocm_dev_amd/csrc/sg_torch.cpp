@@ -25,7 +25,8 @@ namespace {
 // entry points of the libsgemm.so that the package has loaded (bind)
 #define SG_ENTRIES(X)                                                                                               \
     X(sg_skinny_gemm_auto) X(sg_skinny_gemm_rowcol) X(sg_skinny_gemm_bf16act) X(sg_sparse24_gemm)                   \
-    X(sg_sparse24_compress) X(sg_fp8_encode_rows) X(sg_fp8_decode_rows) X(sg_fp8_reduce_rows) X(sg_tiled_sum_reduce)
+    X(sg_sparse24_compress) X(sg_fp8_encode_rows) X(sg_fp8_decode_rows) X(sg_fp8_reduce_rows) X(sg_tiled_sum_reduce)    \
+    X(sg_mxfp4_packed_bytes) X(sg_mxfp4_encode_rows) X(sg_mxfp4_decode_rows) X(sg_mxfp4_gemm) X(sg_mxfp4_gemm_fp8act)
 #define SG_POINTER(name) decltype(&::name) p_##name = nullptr;
 SG_ENTRIES(SG_POINTER)
 #undef SG_POINTER
@@ -308,6 +309,105 @@ PyObject* tiled_sum_reduce(PyObject*, Args v, Py_ssize_t nargs) {
     });
 }
 
+// MXFP4 codes [rows, cols / 2] and scales [rows, cols / 32]
+struct MxCodes {
+    const at::Tensor *Q = nullptr, *S = nullptr;
+    int rows = 0, cols = 0;
+    MxCodes(Operands& o, PyObject* q, PyObject* s) {
+        Q = o.row_major(q, 2);
+        S = o.row_major(s, 2);
+        if (!o.plain) return;
+        o.need(Q->scalar_type() == at::kByte && S->scalar_type() == at::kByte && Q->size(1) % 16 == 0);
+        o.need(S->size(0) == Q->size(0) && S->size(1) * 16 == Q->size(1));
+        rows = o.size(Q->size(0));
+        cols = o.size(Q->size(1) * 2);
+    }
+};
+
+// X, Q, scales
+PyObject* mxfp4_encode_rows(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 3, [&]() -> PyObject* {
+        Operands o;
+        const at::Tensor* X = o.row_major(v[0], 2);
+        const MxCodes c(o, v[1], v[2]);
+        if (!o.plain) return nullptr;
+        o.need(X->scalar_type() == at::kBFloat16 && X->size(0) == c.rows && X->size(1) == c.cols);
+        if (!o.ready()) return nullptr;
+        const void* x = X->const_data_ptr();
+        uint8_t *q = static_cast<uint8_t*>(c.Q->mutable_data_ptr()), *s = static_cast<uint8_t*>(c.S->mutable_data_ptr());
+        void* st = o.stream();
+        return enqueue([&] { return p_sg_mxfp4_encode_rows(x, q, s, c.rows, c.cols, st); });
+    });
+}
+
+// Q, scales, Y
+PyObject* mxfp4_decode_rows(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 3, [&]() -> PyObject* {
+        Operands o;
+        const MxCodes c(o, v[0], v[1]);
+        const at::Tensor* Y = o.row_major(v[2], 2);
+        if (!o.plain) return nullptr;
+        o.need(Y->scalar_type() == at::kBFloat16 && Y->size(0) == c.rows && Y->size(1) == c.cols);
+        if (!o.ready()) return nullptr;
+        const uint8_t *q = bytes(*c.Q), *s = bytes(*c.S);
+        void *y = Y->mutable_data_ptr(), *st = o.stream();
+        return enqueue([&] { return p_sg_mxfp4_decode_rows(q, s, y, c.rows, c.cols, st); });
+    });
+}
+
+// P and D [m, n] of a product with packed n x k weights
+struct MxProduct {
+    const at::Tensor *P = nullptr, *D = nullptr;
+    int m = 0, n = 0;
+    MxProduct(Operands& o, PyObject* p, PyObject* d) {
+        P = o.row_major(p, 1);
+        D = o.row_major(d, 2);
+        if (!o.plain) return;
+        o.need(P->scalar_type() == at::kByte && D->scalar_type() == at::kBFloat16);
+        m = o.size(D->size(0));
+        n = o.size(D->size(1));
+    }
+    void fits(Operands& o, int64_t rows, int k) {
+        if (!o.plain) return;
+        const size_t need = p_sg_mxfp4_packed_bytes(n, k);
+        o.need(rows == m && need > 0 && (size_t)P->numel() == need);
+    }
+};
+
+// A, A_scales, P, D, scale or None
+PyObject* mxfp4_gemm(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 5, [&]() -> PyObject* {
+        Operands o;
+        const MxCodes c(o, v[0], v[1]);
+        MxProduct g(o, v[2], v[3]);
+        const float* s = o.scale(v[4], kOptional);
+        g.fits(o, c.rows, c.cols);
+        if (!o.ready()) return nullptr;
+        const uint8_t *a = bytes(*c.Q), *as = bytes(*c.S), *p = bytes(*g.P);
+        void *d = g.D->mutable_data_ptr(), *st = o.stream();
+        return enqueue([&] { return p_sg_mxfp4_gemm(a, as, p, d, s, g.m, g.n, c.cols, st); });
+    });
+}
+
+// A, P, D, scale or None, row_scales or None
+PyObject* mxfp4_gemm_fp8act(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 5, [&]() -> PyObject* {
+        Operands o;
+        const at::Tensor* A = o.row_major(v[0], 2);
+        MxProduct g(o, v[1], v[2]);
+        const float* s = o.scale(v[3], kOptional);
+        const float* rs = o.factors(v[4], g.m);
+        if (!o.plain) return nullptr;
+        o.need(fp8(A->scalar_type()));
+        const int k = o.size(A->size(1));
+        g.fits(o, A->size(0), k);
+        if (!o.ready()) return nullptr;
+        const uint8_t *a = bytes(*A), *p = bytes(*g.P);
+        void *d = g.D->mutable_data_ptr(), *st = o.stream();
+        return enqueue([&] { return p_sg_mxfp4_gemm_fp8act(a, p, d, s, rs, g.m, g.n, k, st); });
+    });
+}
+
 // bind(handle of libsgemm.so)
 PyObject* bind(PyObject*, PyObject* arg) {
     void* handle = PyLong_AsVoidPtr(arg);
@@ -334,6 +434,10 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          SG_METHOD(fp8_decode_rows),
                          SG_METHOD(fp8_reduce_rows),
                          SG_METHOD(tiled_sum_reduce),
+                         SG_METHOD(mxfp4_encode_rows),
+                         SG_METHOD(mxfp4_decode_rows),
+                         SG_METHOD(mxfp4_gemm),
+                         SG_METHOD(mxfp4_gemm_fp8act),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods};
 

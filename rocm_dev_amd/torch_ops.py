@@ -12,6 +12,11 @@ their output shapes through fake (meta) implementations, and launch on torch's c
     Q, s = torch.ops.sgemm.fp8_encode_rows(X_bf16)
     Y = torch.ops.sgemm.fp8_decode_rows(Q, s)
     D = torch.ops.sgemm.sparse24_gemm(A_fp8, vals, meta, scale)
+    Q, S = torch.ops.sgemm.mxfp4_encode_rows(X_bf16)                        # MXFP4 codes and block scales
+    Y = torch.ops.sgemm.mxfp4_decode_rows(Q, S)
+    P = torch.ops.sgemm.mxfp4_pack(W_codes, W_scales)                       # once per weight matrix
+    D = torch.ops.sgemm.mxfp4_gemm(Q, S, P, n, scale)                       # [m, n] bf16
+    D = torch.ops.sgemm.mxfp4_gemm_fp8act(A_fp8, P, n, scale, row_scales)
 
 FP8 operands are uint8 or float8_e4m3fn tensors holding OCP E4M3 codes; weights are [n, k] with k contiguous.
 """
@@ -111,3 +116,68 @@ def sparse24_gemm(A: torch.Tensor, vals: torch.Tensor, meta: torch.Tensor, scale
 @sparse24_gemm.register_fake
 def _(A, vals, meta, scale):
     return A.new_empty((A.shape[0], vals.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("sgemm::mxfp4_encode_rows", mutates_args=())
+def mxfp4_encode_rows(X: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    Q = torch.empty((X.shape[0], X.shape[1] // 2), dtype=torch.uint8, device=X.device)
+    S = torch.empty((X.shape[0], X.shape[1] // 32), dtype=torch.uint8, device=X.device)
+    api.mxfp4_encode_rows(_rows(X), Q, S, check=True)
+    return Q, S
+
+
+@mxfp4_encode_rows.register_fake
+def _(X):
+    return (X.new_empty((X.shape[0], X.shape[1] // 2), dtype=torch.uint8),
+            X.new_empty((X.shape[0], X.shape[1] // 32), dtype=torch.uint8))
+
+
+@torch.library.custom_op("sgemm::mxfp4_decode_rows", mutates_args=())
+def mxfp4_decode_rows(Q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    Y = torch.empty((Q.shape[0], Q.shape[1] * 2), dtype=torch.bfloat16, device=Q.device)
+    api.mxfp4_decode_rows(_rows(Q), _rows(scales), Y, check=True)
+    return Y
+
+
+@mxfp4_decode_rows.register_fake
+def _(Q, scales):
+    return Q.new_empty((Q.shape[0], Q.shape[1] * 2), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("sgemm::mxfp4_pack", mutates_args=())
+def mxfp4_pack(B: torch.Tensor, B_scales: torch.Tensor) -> torch.Tensor:
+    P = torch.empty((api.mxfp4_packed_bytes(B.shape[0], B.shape[1] * 2),), dtype=torch.uint8, device=B.device)
+    api.mxfp4_pack(_weights(B), _rows(B_scales), P, check=True)
+    return P
+
+
+@mxfp4_pack.register_fake
+def _(B, B_scales):
+    tiles, steps = (B.shape[0] + 15) // 16, (B.shape[1] + 63) // 64
+    return B.new_empty((tiles * (steps * 1024 + (steps + 3) // 4 * 256),), dtype=torch.uint8)
+
+
+@torch.library.custom_op("sgemm::mxfp4_gemm", mutates_args=())
+def mxfp4_gemm(A: torch.Tensor, A_scales: torch.Tensor, P: torch.Tensor, n: int,
+               scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    D = torch.empty((A.shape[0], n), dtype=torch.bfloat16, device=A.device)
+    api.mxfp4_gemm(_rows(A), _rows(A_scales), P, D, _rows(scale), check=True)
+    return D
+
+
+@mxfp4_gemm.register_fake
+def _(A, A_scales, P, n, scale=None):
+    return A.new_empty((A.shape[0], n), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("sgemm::mxfp4_gemm_fp8act", mutates_args=())
+def mxfp4_gemm_fp8act(A: torch.Tensor, P: torch.Tensor, n: int, scale: Optional[torch.Tensor] = None,
+                      row_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    D = torch.empty((A.shape[0], n), dtype=torch.bfloat16, device=A.device)
+    api.mxfp4_gemm_fp8act(_rows(A), P, D, _rows(scale), _rows(row_scales), check=True)
+    return D
+
+
+@mxfp4_gemm_fp8act.register_fake
+def _(A, P, n, scale=None, row_scales=None):
+    return A.new_empty((A.shape[0], n), dtype=torch.bfloat16)

@@ -1,0 +1,403 @@
+"""MXFP4 on the GPU: codec and packing bit for bit, products against 64 bits (tests/mx_reference.py)."""
+import numpy as np
+import pytest
+import torch
+
+import mx_reference as ref
+import rocm_dev_amd as sg
+import rocm_dev_amd.torch_ops  # noqa: F401
+from rocm_dev_amd._lib import host, lib
+
+pytestmark = pytest.mark.gpu
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def dev_bf16(bits):
+    return dev(bits.view(np.int16)).view(torch.bfloat16)
+
+
+def bits(t):
+    return t.cpu().view(torch.int16).numpy().view(np.uint16)
+
+
+def some_bf16(rng, rows, cols):
+    """Normals of all sizes, block by block, with zeros, whole blocks of zeros and ties."""
+    x = rng.standard_normal((rows, cols // 32, 32)) * np.exp2(rng.integers(-20, 20, (rows, cols // 32, 1)))
+    x[rng.random(x.shape) < 0.05] = 0
+    x[rng.random(x.shape[:2]) < 0.05] = 0
+    ties = rng.random(x.shape[:2]) < 0.2
+    x[ties] = rng.choice([0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 7, -0.25, -2.5, -5, 6], (int(ties.sum()), 32))
+    return torch.from_numpy(x.reshape(rows, cols)).bfloat16().view(torch.int16).numpy().view(np.uint16)
+
+
+def some_mx(rng, rows, k):
+    """Codes and scales as an encoder makes them, spread over 2^+-6."""
+    codes = rng.integers(0, 256, (rows, k // 2), dtype=np.uint8)
+    return codes, (127 + rng.integers(-6, 7, (rows, k // 32))).astype(np.uint8)
+
+
+def some_e4m3(rng, rows, k):
+    c = rng.integers(0, 256, (rows, k), dtype=np.uint8)
+    return np.where((c & 127) == 127, 0x38, c).astype(np.uint8)
+
+
+def packed(codes, scales):
+    n, k = codes.shape[0], codes.shape[1] * 2
+    P = torch.full((sg.mxfp4_packed_bytes(n, k),), 0xAA, dtype=torch.uint8, device="cuda")
+    sg.mxfp4_pack(dev(codes), dev(scales), P, check=True)
+    return P
+
+
+# ---- codec --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 64), (3, 96), (7, 2048), (1, 8192), (1, 8224), (64, 1024), (33, 5440), (1021, 352)])
+def test_encode_and_decode_bit_exact(rows, cols):
+    x = some_bf16(np.random.default_rng(rows * cols), rows, cols)
+    Q = torch.full((rows + 1, cols // 2), 0xAA, dtype=torch.uint8, device="cuda")
+    S = torch.full((rows + 1, cols // 32), 0xAA, dtype=torch.uint8, device="cuda")
+    Y = torch.full((rows + 1, cols), -7.0, dtype=torch.bfloat16, device="cuda")
+    sg.mxfp4_encode_rows(dev_bf16(x), Q[:rows], S[:rows], check=True)
+    sg.mxfp4_decode_rows(Q[:rows], S[:rows], Y[:rows], check=True)
+    q, s = ref.encode(x)
+    assert np.array_equal(S[:rows].cpu().numpy(), s) and np.array_equal(Q[:rows].cpu().numpy(), q)
+    assert np.array_equal(Y[:rows].double().cpu().numpy(), ref.values(q, s))       # exact in bf16
+    assert (Q[rows] == 0xAA).all() and (S[rows] == 0xAA).all() and (Y[rows] == -7).all()
+
+
+@pytest.mark.parametrize("beside", [0x0000, 0x0001, 0x0080, 0x3f80, 0x4700, 0x7f7f])
+def test_encode_every_bf16_value(beside):
+    """Every bit pattern, NaNs and infinities among them, in blocks whose other values are `beside`."""
+    x = np.full((65536, 32), beside, np.uint16)
+    x[:, 5] = np.arange(65536)
+    Q, S = torch.ops.sgemm.mxfp4_encode_rows(dev_bf16(x))
+    q, s = ref.encode(x)
+    assert np.array_equal(S.cpu().numpy(), s) and np.array_equal(Q.cpu().numpy(), q)
+
+
+def test_decode_every_code_and_scale():
+    q = np.tile(np.arange(256, dtype=np.uint8).reshape(1, 16, 16), (256, 1, 1))       # [scale][block][byte]
+    s = np.tile(np.arange(256, dtype=np.uint8)[:, None], (1, 16))
+    Y = torch.ops.sgemm.mxfp4_decode_rows(dev(q.reshape(256, 256)), dev(s))
+    want = ref.values(q.reshape(256, 256), s)
+    got = Y.double().cpu().numpy()
+    with np.errstate(over="ignore"):
+        rounded = torch.from_numpy(want).float().bfloat16().double().numpy()          # 6 * 2^127 and the like: infinities
+    assert np.array_equal(got, rounded, equal_nan=True)
+    assert np.array_equal(np.signbit(got[:255]), np.signbit(want[:255]))
+
+
+def test_codec_beyond_32_bits():
+    """More than 2^32 values: the last rows land where they belong."""
+    rows, cols = 65540, 65568
+    X = torch.zeros((rows, cols), dtype=torch.bfloat16, device="cuda")
+    tail = some_bf16(np.random.default_rng(1), 3, cols)
+    X[-3:] = dev_bf16(tail)
+    Q, S = torch.ops.sgemm.mxfp4_encode_rows(X)
+    X.fill_(-7)
+    sg.mxfp4_decode_rows(Q, S, X, check=True)
+    q, s = ref.encode(tail)
+    assert np.array_equal(Q[-3:].cpu().numpy(), q) and np.array_equal(S[-3:].cpu().numpy(), s)
+    assert np.array_equal(X[-3:].double().cpu().numpy(), ref.values(q, s))
+    assert not X[:-3].any() and not Q[:-3].any() and (S[:-3] == 127).all()
+
+
+# ---- packing ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,k,pad", [(1, 32, 0), (16, 128, 0), (15, 96, 16), (17, 512, 0), (33, 544, 48), (129, 1376, 0), (70, 5440, 16)])
+def test_pack(n, k, pad):
+    rng = np.random.default_rng(n + k)
+    codes, scales = rng.integers(0, 256, (n, k // 2), dtype=np.uint8), rng.integers(0, 256, (n, k // 32), dtype=np.uint8)
+    wide = torch.full((n, k // 2 + pad), 0x55, dtype=torch.uint8, device="cuda")
+    wide[:, :k // 2] = dev(codes)
+    P = torch.full((sg.mxfp4_packed_bytes(n, k) + 64,), 0xAA, dtype=torch.uint8, device="cuda")
+    sg.mxfp4_pack(wide[:, :k // 2], dev(scales), P[:-64], check=True)
+    assert np.array_equal(P[:-64].cpu().numpy(), ref.pack(codes, scales)) and (P[-64:] == 0xAA).all()
+
+
+# ---- products -----------------------------------------------------------------------------------------------
+
+MS = (1, 2, 15, 16, 17, 31, 32, 33, 48, 64, 65, 100, 128, 129, 200, 257)
+SHAPES = [(1, 32), (16, 64), (15, 96), (17, 128), (30, 160), (31, 512), (33, 544), (129, 608), (64, 2048), (257, 2080), (100, 4096), (18, 5440),
+          (200, 8192 + 96)]
+
+
+def product(kind, rng, m, n, k, scale=None, row=None, edit=None):
+    """Runs one product; checks it.  edit(A, SA or None, B, SB) may change the operands."""
+    B, SB = some_mx(rng, n, k)
+    A, SA = some_mx(rng, m, k) if kind == "mx" else (some_e4m3(rng, m, k), None)
+    if edit:
+        edit(A, SA, B, SB)
+    P = packed(B, SB)
+    D = torch.full((m + 1, n), -7.0, dtype=torch.bfloat16, device="cuda")      # the row behind stays as it is
+    st = None if scale is None else torch.tensor([scale], dtype=torch.float32, device="cuda")
+    if kind == "mx":
+        sg.mxfp4_gemm(dev(A), dev(SA), P, D[:m], st, check=True)
+    else:
+        sg.mxfp4_gemm_fp8act(dev(A), P, D[:m], st, None if row is None else dev(row), check=True)
+    a = ref.values(A, SA) if kind == "mx" else ref.e4m3(A)
+    want, slack = ref.gemm(a, ref.values(B, SB), kind == "fp8act")
+    factor = np.full((m, 1), 1.0 if scale is None else np.float64(np.float32(scale)))
+    if row is not None:
+        factor = factor * row.astype(np.float64)[:, None]
+    ref.check(bits(D[:m]), want * factor, slack * np.abs(factor))
+    assert (D[m] == -7).all()
+    return D[:m]
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("n,k", SHAPES)
+@pytest.mark.parametrize("m", MS)
+def test_product(kind, m, n, k):
+    product(kind, np.random.default_rng(m * 7 + n * 3 + k), m, n, k)
+
+
+@pytest.mark.parametrize("m", [1, 20, 100, 300])
+def test_factors(m):
+    rng = np.random.default_rng(m)
+    row = rng.uniform(0.5, 1.5, m).astype(np.float32)
+    product("fp8act", rng, m, 70, 1056, 0.37, row)
+    product("fp8act", rng, m, 70, 1056, None, row)
+    product("mx", rng, m, 70, 1056, 0.37)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (8, 6144, 4096), (40, 4100, 1408), (300, 1030, 2880), (1000, 515, 1376), (513, 2048, 4128)])
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+def test_larger_products(kind, m, n, k):
+    product(kind, np.random.default_rng(m + n), m, n, k)
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("m", [1, 16, 33, 130, 300])
+def test_nan_stays_in_its_row_and_column(kind, m):
+    def edit(A, SA, B, SB):
+        SB[5, 2] = 255                       # a block of weight row 5
+        B[5, 32:48] = 0                      # ... of zeros: still NaN
+        if SA is None:
+            A[m // 2, 70] = 0x7f
+        else:
+            SA[m // 2, 1] = 255
+
+    D = product(kind, np.random.default_rng(m), m, 40, 1120, edit=edit)
+    nan = torch.isnan(D)
+    assert nan[m // 2].all() and nan[:, 5].all() and int(nan.sum()) == 40 + m - 1
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("m", [3, 130])
+def test_nan_in_the_last_block_of_a_ragged_row(kind, m):
+    """The columns beyond k repeat a row's last block with weights of zero: they may not spread a NaN further."""
+    def edit(A, SA, B, SB):
+        if SA is None:
+            A[1, -1] = 0xff
+        else:
+            SA[1, -1] = 255
+
+    D = product(kind, np.random.default_rng(m), m, 20, 96 + 512, edit=edit)
+    assert torch.isnan(D[1]).all() and int(torch.isnan(D).sum()) == 20
+
+
+@pytest.mark.parametrize("m", [2, 200])
+def test_ends_of_the_scales(m):
+    """Blocks of the smallest and largest scales: products that underflow, cancel each other's exponent, or overflow."""
+    def edit(A, SA, B, SB):
+        B[:] = 0x22                          # ones
+        A[:] = 0x22
+        SA[:], SB[:] = 127, 127
+        SA[0], SB[0] = 254, 0                # 2^127 * 2^-127
+        SB[1] = 254                          # row 0 x column 1: beyond fp32
+        SB[2], SA[1] = 0, 0                  # 2^-254: zero
+
+    rng = np.random.default_rng(0)
+    B, SB = some_mx(rng, 20, 256)
+    A, SA = some_mx(rng, m, 256)
+    edit(A, SA, B, SB)
+    D = torch.ops.sgemm.mxfp4_gemm(dev(A), dev(SA), packed(B, SB), 20).float().cpu().numpy()
+    assert D[0, 0] == 256 and np.isposinf(D[0, 1]) and D[1, 2] == 0
+    assert np.isposinf(D[0, 3])
+    assert D[1, 4] == np.float32(256 * 2.0 ** -127)
+
+
+def test_zero_weights_and_zero_activations():
+    for kind in ("mx", "fp8act"):
+        D = product(kind, np.random.default_rng(0), 9, 33, 224, edit=lambda A, SA, B, SB: B.__setitem__(slice(None), 0))
+        assert not D.any()
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 512), (8, 4096, 4096), (100, 2373, 5440), (700, 1000, 2880)])
+def test_same_bits_every_time_and_on_another_stream(kind, m, n, k):
+    rng = np.random.default_rng(5)
+    B, SB = some_mx(rng, n, k)
+    P = packed(B, SB)
+    if kind == "mx":
+        A, SA = (dev(t) for t in some_mx(rng, m, k))
+        run = lambda D: sg.mxfp4_gemm(A, SA, P, D, check=True)  # noqa: E731
+    else:
+        A = dev(some_e4m3(rng, m, k))
+        run = lambda D: sg.mxfp4_gemm_fp8act(A, P, D, check=True)  # noqa: E731
+    first = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    run(first)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    outs = [torch.empty_like(first) for _ in range(4)]
+    with torch.cuda.stream(side):
+        run(outs[0])
+        run(outs[1])
+    run(outs[2])
+    run(outs[3])
+    torch.cuda.synchronize()
+    for D in outs:
+        assert torch.equal(D.view(torch.int16), first.view(torch.int16))
+
+
+@pytest.mark.parametrize("m", [4, 150])
+def test_recorded_layer_replays(m):
+    """Quantise, project, quantise, project: recorded once, replayed on changing inputs, every replay as eager."""
+    rng = np.random.default_rng(m)
+    k, hidden = 512, 544
+    P1, P2 = packed(*some_mx(rng, hidden, k)), packed(*some_mx(rng, k, hidden))
+
+    def buffers():
+        return [torch.empty(s, dtype=t, device="cuda") for s, t in (((m, k // 2), torch.uint8), ((m, k // 32), torch.uint8),
+                ((m, hidden), torch.bfloat16), ((m, hidden), torch.uint8), ((m,), torch.float32), ((m, k), torch.bfloat16))]
+
+    def layer(X, b):
+        sg.mxfp4_encode_rows(X, b[0], b[1], check=True)
+        sg.mxfp4_gemm(b[0], b[1], P1, b[2], check=True)
+        sg.fp8_encode_rows(b[2], b[3], b[4], check=True)
+        sg.mxfp4_gemm_fp8act(b[3], P2, b[5], None, b[4], check=True)
+
+    X, b, e = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda"), buffers(), buffers()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        layer(X, b)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(X, b)
+    for seed in range(4):
+        X.copy_(dev_bf16(some_bf16(np.random.default_rng(seed), m, k)))
+        b[5].fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        layer(X, e)
+        torch.cuda.synchronize()
+        assert torch.equal(b[5].view(torch.int16), e[5].view(torch.int16)) and e[5].any()
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+def test_activations_and_outputs_beyond_32_bits(kind):
+    """m * k and m * n beyond 2^32: the last rows against the definition."""
+    m, n, k = 140000, 33000, 65536 if kind == "mx" else 32768
+    rng = np.random.default_rng(2)
+    B, SB = some_mx(rng, n, k)
+    P = packed(B, SB)
+    rows = 5
+    if kind == "mx":
+        A = torch.zeros((m, k // 2), dtype=torch.uint8, device="cuda")
+        SA = torch.full((m, k // 32), 127, dtype=torch.uint8, device="cuda")
+        a, sa = some_mx(rng, rows, k)
+        A[-rows:], SA[-rows:] = dev(a), dev(sa)
+        D = torch.ops.sgemm.mxfp4_gemm(A, SA, P, n)
+        v = ref.values(a, sa)
+    else:
+        A = torch.zeros((m, k), dtype=torch.uint8, device="cuda")
+        a = some_e4m3(rng, rows, k)
+        A[-rows:] = dev(a)
+        D = torch.ops.sgemm.mxfp4_gemm_fp8act(A, P, n)
+        v = ref.e4m3(a)
+    cols = np.r_[0:40, n - 40:n]
+    want, slack = ref.gemm(v, ref.values(B[cols], SB[cols]), kind == "fp8act")
+    ref.check(bits(D[-rows:][:, torch.from_numpy(cols).cuda()].contiguous()), want, slack)
+    assert not D[:-rows].any()
+
+
+def test_weights_beyond_32_bits():
+    n, k, m = 300016, 32768, 3
+    B = torch.zeros((n, k // 2), dtype=torch.uint8, device="cuda")
+    SB = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(3)
+    b, sb = some_mx(rng, 37, k)
+    B[-37:], SB[-37:] = dev(b), dev(sb)
+    P = torch.ops.sgemm.mxfp4_pack(B, SB)
+    assert P.numel() > 1 << 32
+    a = some_e4m3(rng, m, k)
+    D = torch.ops.sgemm.mxfp4_gemm_fp8act(dev(a), P, n)
+    want, slack = ref.gemm(ref.e4m3(a), ref.values(b, sb), True)
+    ref.check(bits(D[:, -37:].contiguous()), want, slack)
+    assert not D[:, :-37].any()
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3, 5, 8])
+def test_activation_scales_at_any_address(offset):
+    rng = np.random.default_rng(offset)
+    m, n, k = 37, 48, 1024 + 512 * (offset % 2)
+    B, SB = some_mx(rng, n, k)
+    A, SA = some_mx(rng, m, k)
+    room = torch.empty((m * (k // 32) + 16,), dtype=torch.uint8, device="cuda")
+    view = room[offset:offset + m * (k // 32)].view(m, k // 32)
+    view.copy_(dev(SA))
+    D = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    sg.mxfp4_gemm(dev(A), view, packed(B, SB), D, check=True)
+    want, slack = ref.gemm(ref.values(A, SA), ref.values(B, SB), False)
+    ref.check(bits(D), want, slack)
+
+
+# ---- entry points -------------------------------------------------------------------------------------------
+
+def _operands():
+    rng = np.random.default_rng(9)
+    m, n, k = 5, 48, 512
+    B, SB = some_mx(rng, n, k)
+    A, SA = some_mx(rng, m, k)
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    one = torch.full((1,), 0.5, dtype=torch.float32, device="cuda")
+    row = torch.rand(m, device="cuda")
+    return {"mxfp4_encode_rows": ([dev_bf16(some_bf16(rng, m, k)), dev(A).zero_(), dev(SA).zero_()], [1, 2]),
+            "mxfp4_decode_rows": ([dev(A), dev(SA), bf(m, k)], [2]),
+            "mxfp4_gemm": ([dev(A), dev(SA), packed(B, SB), bf(m, n), one], [3]),
+            "mxfp4_gemm_fp8act": ([dev(some_e4m3(rng, m, k)).view(torch.float8_e4m3fn), packed(B, SB), bf(m, n), one, row], [2])}
+
+
+def _c_abi(name, ops):
+    ptr, st = [t.data_ptr() for t in ops], torch.cuda.current_stream().cuda_stream
+    return getattr(lib, "sg_" + name)(*ptr, *((5, 512) if len(ops) == 3 else (5, 48, 512)), st)
+
+
+@pytest.mark.parametrize("name", ["mxfp4_encode_rows", "mxfp4_decode_rows", "mxfp4_gemm", "mxfp4_gemm_fp8act"])
+def test_entry_points_agree(name):
+    ops, outs = _operands()[name]
+    assert _c_abi(name, ops) == 0
+    torch.cuda.synchronize()
+    want = [ops[i].clone() for i in outs]
+    assert all(t.count_nonzero() > 0 for t in want)
+    for entry in (getattr(host, name), getattr(sg, name)):
+        for i in outs:
+            ops[i].zero_()
+        assert entry(*ops) == 0
+        torch.cuda.synchronize()
+        assert all(torch.equal(ops[i], w) for i, w in zip(outs, want))
+    # the extension leaves what is not plain to Python, one operand at a time
+    for i, t in enumerate(ops):
+        bad = [t.cpu(), t.to(torch.float64), t[:-1] if t.shape[0] > 1 else t[:0]]
+        if t.dim() == 2:
+            bad += [t.t(), torch.cat([t, t], -1)[:, ::2]]
+        for b in bad:
+            assert getattr(host, name)(*ops[:i], b, *ops[i + 1:]) is None, (name, i)
+            with pytest.raises(ValueError):
+                getattr(sg, name)(*ops[:i], b, *ops[i + 1:])
+
+
+def test_operators_take_views_of_activations():
+    rng = np.random.default_rng(11)
+    X = dev_bf16(some_bf16(rng, 64, 96))
+    Q, S = torch.ops.sgemm.mxfp4_encode_rows(X.t().contiguous().t())
+    q, s = torch.ops.sgemm.mxfp4_encode_rows(X)
+    assert torch.equal(Q, q) and torch.equal(S, s)
+    torch.library.opcheck(torch.ops.sgemm.mxfp4_encode_rows, (X,))
+    B, SB = some_mx(rng, 40, 96)
+    P = torch.ops.sgemm.mxfp4_pack(dev(B), dev(SB))
+    torch.library.opcheck(torch.ops.sgemm.mxfp4_gemm, (Q, S, P, 40))

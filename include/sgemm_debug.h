@@ -80,6 +80,12 @@ int sg_debug_read_stream(const uint8_t* B, int n, int k, int b_stride, int segme
 int sg_debug_cu_ingest(const uint8_t* cold, size_t cold_bytes, const uint8_t* hot, size_t hot_bytes, int workgroups, int waves,
                        int cold_waves, int hot_per_cold, int depth, int ticks, unsigned long long* counts, void* stream);
 
+/* The products with packed MXFP4 weights through a given build of their kernels (0: the library's choice), for timing and for
+ * tests that have to reach every build at every size.  A_scales NULL: E4M3 activations, otherwise MXFP4.  SG_INVALID_CONFIG: no such
+ * build.  Builds are numbered in rocm_dev_amd/csrc/sg_mx_gemm.hip. */
+int sg_debug_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D_bf16, const float* scale_tensor,
+                        const float* row_scales, int m, int n, int k, int build, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -132,7 +132,7 @@ static int fill_zero_now(unsigned* p, size_t n) {
     return rc;
 }
 
-static bool stream_is_capturing(hipStream_t stream) {
+bool stream_is_capturing(hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
         (void)hipGetLastError();
@@ -191,15 +191,17 @@ int get_workspace(hipStream_t stream, size_t partial_bytes, size_t n_counters, W
 // costs such a call about 20 ns of host time; a call without a K split takes none.)
 constexpr int kTurns = 64;
 static std::recursive_mutex g_turn[kTurns];    // (recursive: the encoder's call holds it around the GEMM's)
+std::recursive_mutex& stream_turn(hipStream_t stream) {
+    int dev = 0;
+    (void)current_device(&dev);
+    const unsigned long long key = (unsigned long long)reinterpret_cast<uintptr_t>(stream) + (unsigned long long)dev;
+    return g_turn[(key * 0x9E3779B97F4A7C15ull) >> 58];
+}
 class StreamTurn {
     std::unique_lock<std::recursive_mutex> lock_;
 public:
     StreamTurn(bool needed, hipStream_t stream) {
-        if (!needed) return;
-        int dev = 0;
-        (void)current_device(&dev);
-        const unsigned long long key = (unsigned long long)reinterpret_cast<uintptr_t>(stream) + (unsigned long long)dev;
-        lock_ = std::unique_lock<std::recursive_mutex>(g_turn[(key * 0x9E3779B97F4A7C15ull) >> 58]);
+        if (needed) lock_ = std::unique_lock<std::recursive_mutex>(stream_turn(stream));
     }
 };
 static_assert(kTurns == 64, "the top six bits of the product");

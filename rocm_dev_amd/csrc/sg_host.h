@@ -97,6 +97,10 @@ struct Workspace {
 // The workspace of `stream` on the current device, created or grown on demand; *out is a copy.
 int get_workspace(hipStream_t stream, size_t partial_bytes, size_t n_counters, Workspace* out);
 
+// A call of more than one launch that hands memory of its stream's from one to the next holds this from its first launch to its last.
+std::recursive_mutex& stream_turn(hipStream_t stream);
+bool stream_is_capturing(hipStream_t stream);
+
 // Device facts queried once per device.
 struct DeviceInfo {
     int cu_count = 0;

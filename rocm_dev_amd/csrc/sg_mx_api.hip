@@ -1,4 +1,5 @@
 // C entry points of the MXFP4 operators (include/sgemm.h): every argument is checked here, before anything is launched.
+#include "../../include/sgemm_debug.h"
 #include "sg_mx.h"
 
 using namespace sg;
@@ -6,7 +7,7 @@ using namespace sg;
 namespace {
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-int gemm(bool fp4, const uint8_t* A, const uint8_t* SA, const uint8_t* P, void* D, const float* scale, const float* row_scales, int m, int n,
+int gemm(bool fp4, int build, const uint8_t* A, const uint8_t* SA, const uint8_t* P, void* D, const float* scale, const float* row_scales, int m, int n,
          int k, void* stream) {
     if (!A || (fp4 && !SA) || !P || !D || m <= 0 || n <= 0 || k <= 0) return SG_BAD_ARGUMENT;
     if (k % kMxBlock) return SG_K_NOT_DIVISIBLE_BY_WARPTILE_K;
@@ -28,7 +29,8 @@ int gemm(bool fp4, const uint8_t* A, const uint8_t* SA, const uint8_t* P, void* 
     a.tiles = l.tiles;
     a.steps = l.steps;
     a.quads = l.quads;
-    return launch_mx_gemm(fp4, a, dev->cu_count, static_cast<hipStream_t>(stream));
+    a.pitch = l.pitch;
+    return launch_mx_gemm(fp4, build, a, dev->cu_count, static_cast<hipStream_t>(stream));
 }
 }  // namespace
 
@@ -63,12 +65,17 @@ int sg_mxfp4_pack(const uint8_t* B, const uint8_t* B_scales, uint8_t* P, int n, 
 
 int sg_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D, const float* scale_tensor, int m, int n, int k,
                   void* stream) {
-    return gemm(true, A, A_scales, P, D, scale_tensor, nullptr, m, n, k, stream);
+    return gemm(true, 0, A, A_scales, P, D, scale_tensor, nullptr, m, n, k, stream);
 }
 
 int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D, const float* scale_tensor, const float* row_scales, int m, int n, int k,
                          void* stream) {
-    return gemm(false, A, nullptr, P, D, scale_tensor, row_scales, m, n, k, stream);
+    return gemm(false, 0, A, nullptr, P, D, scale_tensor, row_scales, m, n, k, stream);
+}
+
+int sg_debug_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D, const float* scale_tensor,
+                        const float* row_scales, int m, int n, int k, int build, void* stream) {
+    return gemm(A_scales != nullptr, build, A, A_scales, P, D, scale_tensor, row_scales, m, n, k, stream);
 }
 
 }  // extern "C"

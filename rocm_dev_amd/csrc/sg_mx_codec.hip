@@ -93,16 +93,16 @@ __global__ void __launch_bounds__(256) mx_decode_kernel(const uint32_t* __restri
 // One wave a step of a tile (1 KB of codes), and the scales of the four steps of a group with the first of them.
 __global__ void __launch_bounds__(256) mx_pack_kernel(const uint8_t* __restrict__ B, const uint8_t* __restrict__ SB,
                                                       uint8_t* __restrict__ P, uint8_t* __restrict__ PS, int n, int k_blocks,
-                                                      int steps, int quads, int b_stride) {
+                                                      int pitch, int quads, int b_stride) {
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const size_t tile = blockIdx.x;
     const size_t row = tile * 16 + r;
     const bool live = row < (size_t)n;
-    for (int step = blockIdx.y * 4 + (int)(threadIdx.x >> 6); step < steps; step += gridDim.y * 4) {
+    for (int step = blockIdx.y * 4 + (int)(threadIdx.x >> 6); step < pitch; step += gridDim.y * 4) {
         const int block = step * 4 + g;
         u32x4 codes = {0, 0, 0, 0};
         if (live && block < k_blocks) codes = *reinterpret_cast<const u32x4*>(B + row * (size_t)b_stride + (size_t)block * 16);
-        *reinterpret_cast<u32x4*>(P + (tile * steps + step) * kMxStepBytes + lane * 16) = codes;
+        *reinterpret_cast<u32x4*>(P + (tile * pitch + step) * kMxStepBytes + lane * 16) = codes;
         if (step % 4 == 0) {
             uint32_t s = 0;
 #pragma unroll
@@ -113,6 +113,35 @@ __global__ void __launch_bounds__(256) mx_pack_kernel(const uint8_t* __restrict_
             *reinterpret_cast<uint32_t*>(PS + (tile * quads + step / 4) * kMxQuadBytes + lane * 4) = s;
         }
     }
+}
+
+// Block scales of activations on rows of whole groups of four steps, 16 bytes each, for the wide kernel's direct loads: 16 bytes a lane.
+__global__ void __launch_bounds__(256) mx_scale_rows_kernel(const uint8_t* __restrict__ SA, u32x4* __restrict__ out, unsigned m, unsigned quads,
+                                                            unsigned inv_quads, int k_blocks) {
+    const unsigned at = blockIdx.x * 256 + threadIdx.x;
+    const unsigned row = fast_div(at, quads, inv_quads), q = at - row * quads;
+    if (row >= m) return;
+    const uint8_t* s = SA + (size_t)row * k_blocks + 16 * (size_t)q;
+    u32x4 v;
+    if (16 * (int)q + 16 <= k_blocks) {
+        __builtin_memcpy(&v, s, 16);
+    } else {
+        const int have = k_blocks - 16 * (int)q;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b++) v[e] |= (uint32_t)(4 * e + b < have ? s[4 * e + b] : 127) << (8 * b);
+        }
+    }
+    out[at] = v;
+}
+
+int launch_mx_scale_rows(const uint8_t* SA, uint8_t* out, int m, int k, int quads, hipStream_t stream) {
+    const unsigned pieces = (unsigned)m * (unsigned)quads;               // (the caller keeps it below 2^31)
+    mx_scale_rows_kernel<<<(pieces + 255) / 256, 256, 0, stream>>>(SA, reinterpret_cast<u32x4*>(out), (unsigned)m, (unsigned)quads,
+                                                                   div_reciprocal((unsigned)quads), k / kMxBlock);
+    return report_hip("mx_scale_rows launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
 static unsigned mx_codec_grid(size_t blocks) { return (unsigned)((blocks + 64 * kMxChunks - 1) / (64 * kMxChunks)); }
@@ -132,7 +161,7 @@ int launch_mx_decode(const uint8_t* Q, const uint8_t* S, void* Y, int rows, int 
 int launch_mx_pack(const uint8_t* B, const uint8_t* SB, uint8_t* P, int n, int k, int b_stride, hipStream_t stream) {
     const MxLayout l = mx_layout(n, k);
     const unsigned gy = l.quads < 65535 ? (unsigned)l.quads : 65535u;
-    mx_pack_kernel<<<dim3((unsigned)l.tiles, gy), 256, 0, stream>>>(B, SB, P, P + l.scales_at, n, k / kMxBlock, l.steps, l.quads, b_stride);
+    mx_pack_kernel<<<dim3((unsigned)l.tiles, gy), 256, 0, stream>>>(B, SB, P, P + l.scales_at, n, k / kMxBlock, l.pitch, l.quads, b_stride);
     return report_hip("mx_pack launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 

@@ -3,32 +3,126 @@
 
 #include <type_traits>
 
-#include "sg_mx_kernel.h"
+#include "sg_mx_wide_kernel.h"
 
 namespace sg {
 
+// Workgroup tiles of bn x bm rows, times the K splits; 0 where the grid would be too large.
+static unsigned mx_grid(MxArgs& a, int bn, int bm) {
+    a.n_groups = (a.tiles - 1) / (bn / 16) + 1;
+    a.m_groups = (a.m - 1) / bm + 1;
+    const long long grid = (long long)a.n_groups * a.m_groups * a.splits;
+    return grid > INT_MAX ? 0 : (unsigned)grid;
+}
+
 template <bool FP4, int NF, int MF>
 static int launch_small(MxArgs& a, int waves, hipStream_t stream) {
-    a.n_groups = (a.tiles + NF - 1) / NF;
-    a.m_groups = (int)(((unsigned)a.m + 16 * MF - 1) / (16 * MF));
-    const long long grid = (long long)a.n_groups * a.m_groups;
-    if (grid > INT_MAX) return SG_BAD_ARGUMENT;
+    const unsigned grid = mx_grid(a, 16 * NF, 16 * MF);
+    if (!grid) return SG_BAD_ARGUMENT;
     const size_t lds = waves > 1 ? (size_t)waves * NF * MF * 1024 : 0;
     static LdsGranted granted;
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(mx_gemm_kernel<FP4, NF, MF>), lds, granted)) return rc;
-    mx_gemm_kernel<FP4, NF, MF><<<(unsigned)grid, 64 * waves, lds, stream>>>(a);
+    mx_gemm_kernel<FP4, NF, MF><<<grid, 64 * waves, lds, stream>>>(a);
     return report_hip("mx_gemm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
-template <bool FP4>
-static int launch_any(MxArgs& a, int cu_count, hipStream_t stream) {
-    const int most = a.quads < 8 ? a.quads : 8;      // waves that have a share of K
-    if (a.m <= 16) return launch_small<FP4, 1, 1>(a, most, stream);
-    return launch_small<FP4, 2, 2>(a, most, stream);
+template <bool FP4, int NF, int MF, int WN, int WM>
+static int launch_tile(MxArgs& a, hipStream_t stream) {
+    const unsigned grid = mx_grid(a, 16 * NF * WN, 16 * MF * WM);
+    if (!grid) return SG_BAD_ARGUMENT;
+    mx_tile_kernel<FP4, NF, MF, WN, WM><<<grid, 64 * WN * WM, 0, stream>>>(a);
+    return report_hip("mx_tile launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
-int launch_mx_gemm(bool fp4, MxArgs& a, int cu_count, hipStream_t stream) {
-    return fp4 ? launch_any<true>(a, cu_count, stream) : launch_any<false>(a, cu_count, stream);
+// The wide kernel addresses rows of its tile with 32 bits.
+static bool wide_takes(const MxArgs& a) { return a.k <= 1 << 22; }
+// ... and reads the scales of MXFP4 activations from rows of whole groups of four steps.
+static bool scales_lie_right(const MxArgs& a) { return a.k % 512 == 0 && (reinterpret_cast<uintptr_t>(a.SA) & 15u) == 0; }
+
+template <bool FP4, int RGW, int MH, int DW, int DX>
+static int launch_mx_wide(MxArgs& a, hipStream_t stream) {
+    if (!wide_takes(a)) return SG_INVALID_CONFIG;
+    const unsigned grid = mx_grid(a, 32 * RGW, 32 * MH);
+    if (!grid) return SG_BAD_ARGUMENT;
+    constexpr size_t lds = mx_wide_lds(FP4, RGW, MH, DW, DX);
+    static_assert(lds <= 160 * 1024, "LDS");
+    static LdsGranted granted;
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(mx_wide_kernel<FP4, RGW, MH, DW, DX>), lds, granted)) return rc;
+    mx_wide_kernel<FP4, RGW, MH, DW, DX><<<grid, 256, lds, stream>>>(a);
+    return report_hip("mx_wide launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
+}
+
+// Every build, by number (include/sgemm_debug.h).
+template <bool FP4>
+static int launch_build(int build, MxArgs& a, hipStream_t stream) {
+    const int waves = build % 100;
+    if (build < 2000 && (waves < 1 || waves > 8)) return SG_INVALID_CONFIG;
+    switch (build < 2000 ? build / 100 : build) {
+        case 11: return launch_small<FP4, 1, 1>(a, waves, stream);
+        case 12: return launch_small<FP4, 2, 1>(a, waves, stream);
+        case 13: return launch_small<FP4, 2, 2>(a, waves, stream);
+        case 14: return launch_small<FP4, 1, 2>(a, waves, stream);
+        case 15: return launch_small<FP4, 1, 4>(a, waves, stream);
+        case 16: return launch_small<FP4, 2, 4>(a, waves, stream);
+        case 17: return launch_small<FP4, 4, 1>(a, waves, stream);
+        case 2001: return launch_tile<FP4, 2, 4, 4, 2>(a, stream);   // 128 weight rows x 128 activation rows
+        case 2002: return launch_tile<FP4, 2, 2, 4, 2>(a, stream);   // 128 x 64
+        case 2003: return launch_tile<FP4, 1, 4, 4, 2>(a, stream);   //  64 x 128
+        case 2004: return launch_tile<FP4, 1, 2, 4, 2>(a, stream);   //  64 x 64
+        case 2005: return launch_tile<FP4, 2, 8, 4, 1>(a, stream);   // 128 x 128
+        case 2006: return launch_tile<FP4, 1, 2, 4, 1>(a, stream);   //  64 x 32
+        case 2007: return launch_tile<FP4, 1, 4, 4, 1>(a, stream);   //  64 x 64
+        case 2008: return launch_tile<FP4, 1, 4, 2, 1>(a, stream);   //  32 x 64
+        case 2009: return launch_tile<FP4, 1, 2, 2, 1>(a, stream);   //  32 x 32
+        case 2010: return launch_tile<FP4, 2, 4, 4, 1>(a, stream);   // 128 x 64
+        case 3001: return launch_mx_wide<FP4, 8, 8, FP4 ? 2 : 3, FP4 ? 2 : 3>(a, stream);
+        case 3002: return launch_mx_wide<FP4, 6, 4, 3, 3>(a, stream);
+        case 3003: return launch_mx_wide<FP4, 8, 4, 3, 3>(a, stream);
+        case 3004: return launch_mx_wide<FP4, 6, 8, 3, 2>(a, stream);
+        case 3005: return launch_mx_wide<FP4, 4, 8, 3, FP4 ? 2 : 3>(a, stream);
+        case 3006: return launch_mx_wide<FP4, 4, 4, 3, 3>(a, stream);
+        default: return SG_INVALID_CONFIG;
+    }
+}
+
+static int pick_mx(const MxArgs& a, int cu_count) {
+    const int waves = a.quads < 8 ? a.quads : 8;      // waves that have a share of K
+    if (a.m <= 16) return 1100 + waves;
+    if (a.m <= 32) return 1300 + waves;
+    if (a.m <= 128) return 2002;
+    return 2001;
+}
+
+int launch_mx_gemm(bool fp4, int build, MxArgs& a, int cu_count, hipStream_t stream) {
+    a.splits = 1;
+    if (build == 0) build = pick_mx(a, cu_count);
+    const int splits = build / 10000 < 1 ? 1 : build / 10000;
+    build %= 10000;
+    if (splits > a.quads) return SG_INVALID_CONFIG;
+    a.SX = a.SA;
+    const bool copy_scales = fp4 && build >= 3000 && !scales_lie_right(a);
+    if (splits == 1 && !copy_scales) return fp4 ? launch_build<true>(build, a, stream) : launch_build<false>(build, a, stream);
+
+    // More than one launch: the copied scales, then the partial sums, in the stream's workspace.
+    std::lock_guard<std::recursive_mutex> turn(stream_turn(stream));
+    const size_t frags = (size_t)((a.m - 1) / 16 + 1) * a.tiles;
+    const size_t sum_grid = (frags + 3) / 4;
+    const size_t pieces = copy_scales ? (size_t)a.m * a.quads : 0;
+    if (sum_grid > INT_MAX || pieces > INT_MAX) return SG_BAD_ARGUMENT;
+    const size_t scale_bytes = (pieces * 16 + 255) / 256 * 256;
+    Workspace w;
+    if (int rc = get_workspace(stream, scale_bytes + (splits > 1 ? frags * splits * 1024 : 0), 0, &w)) return rc;
+    if (copy_scales) {
+        uint8_t* const copy = reinterpret_cast<uint8_t*>(w.partials);
+        if (int rc = launch_mx_scale_rows(a.SA, copy, a.m, a.k, a.quads, stream)) return rc;
+        a.SX = copy;
+    }
+    a.splits = splits;
+    a.ws = w.partials + scale_bytes / 4;
+    if (int rc = fp4 ? launch_build<true>(build, a, stream) : launch_build<false>(build, a, stream)) return rc;
+    if (splits == 1) return SG_SUCCESS;
+    mx_sum_kernel<<<(unsigned)sum_grid, 256, 0, stream>>>(a);
+    return report_hip("mx_sum launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
 }  // namespace sg

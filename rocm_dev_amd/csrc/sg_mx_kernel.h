@@ -27,17 +27,72 @@ __device__ __forceinline__ f32x4 mfma_mx(const i32x4 w, const i32x8 x, const f32
 __device__ __forceinline__ void mx_store4(const MxArgs& a, int m_idx, int n_idx, f32x4 v) {
     uint16_t* const d = a.D + (size_t)m_idx * a.n + n_idx;
     const uint32_t lo = pack_bf16x2(v[0], v[1]), hi = pack_bf16x2(v[2], v[3]);
-    if ((a.n & 3) == 0) {
-        *reinterpret_cast<u32x2*>(d) = u32x2{lo, hi};
-    } else if ((a.n & 1) == 0) {
-        *reinterpret_cast<uint32_t*>(d) = lo;
-        if (n_idx + 2 < a.n) *reinterpret_cast<uint32_t*>(d + 2) = hi;
+    if (n_idx + 4 <= a.n) {
+        // one store at whatever multiple of two bytes an odd n leaves it
+        using u32x2_at2 = u32x2 __attribute__((aligned(2)));
+        *reinterpret_cast<u32x2_at2*>(d) = u32x2{lo, hi};
     } else {
         d[0] = (uint16_t)lo;
         if (n_idx + 1 < a.n) d[1] = (uint16_t)(lo >> 16);
         if (n_idx + 2 < a.n) d[2] = (uint16_t)hi;
-        if (n_idx + 3 < a.n) d[3] = (uint16_t)(hi >> 16);
     }
+}
+
+// Which tile and which part of K a workgroup has.  Neighbours share the weights: the activation tiles of a weight tile first,
+// then its splits.
+struct MxPlace {
+    int tn, tm, split, q0, q1;      // groups of four steps [q0, q1)
+};
+__device__ __forceinline__ MxPlace mx_place(const MxArgs& a) {
+    const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int rest = at / a.m_groups, tn = a.splits > 1 ? rest / a.splits : rest;
+    MxPlace p;
+    p.tm = at - rest * a.m_groups;
+    p.tn = tn;
+    p.split = rest - tn * a.splits;
+    p.q0 = a.splits > 1 ? (int)((long long)a.quads * p.split / a.splits) : 0;
+    p.q1 = a.splits > 1 ? (int)((long long)a.quads * (p.split + 1) / a.splits) : a.quads;
+    return p;
+}
+
+// Fragment (fn, fm) of a workgroup's sums: into the output, or - K split - into the workspace.
+__device__ __forceinline__ void mx_put(const MxArgs& a, int split, int fn, int fm, int lane, f32x4 v, float scale) {
+    if (a.splits > 1) {
+        const int m_frags = (a.m - 1) / 16 + 1;
+        if (fn < a.tiles && fm < m_frags)
+            reinterpret_cast<f32x4*>(a.ws)[(((size_t)split * m_frags + fm) * a.tiles + fn) * 64 + lane] = v;
+        return;
+    }
+    const int m_idx = fm * 16 + (lane & 15), n_idx = fn * 16 + 4 * (lane >> 4);
+    if (m_idx >= a.m || n_idx >= a.n) return;
+    v *= scale;
+    if (a.row_scale) v *= a.row_scale[m_idx];
+    mx_store4(a, m_idx, n_idx, v);
+}
+
+// The second launch of a K split: a wave adds the splits of one fragment, in their order.
+__global__ void __launch_bounds__(256) mx_sum_kernel(const MxArgs a) {
+    const int lane = lane_id();
+    const int m_frags = (a.m - 1) / 16 + 1;
+    const size_t frags = (size_t)m_frags * a.tiles, f = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (f >= frags) return;
+    const f32x4* p = reinterpret_cast<const f32x4*>(a.ws) + f * 64 + lane;
+    const float scale = a.scale ? a.scale[0] : 1.0f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; s += 8) {            // eight loads in flight; behind the last split it again, not added
+        f32x4 t[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = p[(size_t)(s + i < a.splits ? s + i : a.splits - 1) * frags * 64];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (s + i < a.splits) v += t[i];
+    }
+    const int fm = (int)(f / a.tiles), fn = (int)(f - (size_t)fm * a.tiles);
+    const int m_idx = fm * 16 + (lane & 15), n_idx = fn * 16 + 4 * (lane >> 4);
+    if (m_idx >= a.m || n_idx >= a.n) return;
+    v *= scale;
+    if (a.row_scale) v *= a.row_scale[m_idx];
+    mx_store4(a, m_idx, n_idx, v);
 }
 
 template <bool FP4, int NF, int MF>
@@ -45,8 +100,8 @@ __global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [waves][NF * MF][64 lanes] f32x4
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int wave = wave_id(), waves = (int)(blockDim.x >> 6);
-    const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    const int tn = at / a.m_groups, tm = at - tn * a.m_groups;
+    const MxPlace place = mx_place(a);
+    const int tn = place.tn, tm = place.tm;
     const int k_blocks = a.k / kMxBlock;
 
     // ---- operands: lane (r, g) ----
@@ -55,7 +110,7 @@ __global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
 #pragma unroll
     for (int i = 0; i < NF; i++) {
         const int tile = tn * NF + i < a.tiles ? tn * NF + i : a.tiles - 1;      // beyond the last tile: it again, not stored
-        wp[i] = a.P + (size_t)tile * a.steps * kMxStepBytes + lane * 16;
+        wp[i] = a.P + (size_t)tile * a.pitch * kMxStepBytes + lane * 16;
         wsp[i] = a.PS + (size_t)tile * a.quads * kMxQuadBytes + lane * 4;
     }
     const uint8_t* xp[MF];
@@ -133,12 +188,12 @@ __global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
     using T2 = std::integral_constant<int, 2>;
     using T3 = std::integral_constant<int, 3>;
 
-    int q = wave;
-    if (q < a.quads) {
+    int q = place.q0 + wave;
+    if (q < place.q1) {
         load_scales(q);
 #pragma unroll
         for (int t = 0; t < 4; t++) load_step(q, t);
-        for (; q + waves < a.quads; q += waves) {
+        for (; q + waves < place.q1; q += waves) {
             take_scales();
             load_scales(q + waves);
             multiply(T0{});
@@ -160,13 +215,7 @@ __global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
 
     // ---- the waves' sums, in wave order ----
     const float scale = a.scale ? a.scale[0] : 1.0f;
-    auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) {
-        const int m_idx = (tm * MF + j) * 16 + r, n_idx = (tn * NF + i) * 16 + 4 * g;
-        if (m_idx >= a.m || n_idx >= a.n) return;
-        v *= scale;
-        if (a.row_scale) v *= a.row_scale[m_idx];
-        mx_store4(a, m_idx, n_idx, v);
-    };
+    auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) { mx_put(a, place.split, tn * NF + i, tm * MF + j, lane, v, scale); };
     if (waves == 1) {
 #pragma unroll
         for (int i = 0; i < NF; i++)

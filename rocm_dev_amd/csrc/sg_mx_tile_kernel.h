@@ -1,0 +1,198 @@
+// Products with MXFP4 weights on tiles of many activation rows:  D[m,n] = bf16(scale * row[m] * sum_k A[m,k] * B[n,k]).
+//
+// A workgroup of WN x WM waves owns 16 * NF * WN weight rows by 16 * MF * WM activation rows, a wave NF x MF fragments of
+// 16 x 16.  A stage is 128 bytes of every activation row: 128 columns of E4M3 (one step of the matrix instruction) or 256 of
+// MXFP4 (two).  The activations of a stage, which all waves along n read, go through LDS, two buffers, one barrier a stage; the
+// weights, which only the WM waves along m share, go straight to registers by contiguous KBs of the packed buffer (sg_mx.h):
+// through LDS they would be a quarter (E4M3) to a half (MXFP4) of its traffic.  Both are asked for a stage ahead.
+//
+// LDS: row x 128 bytes, the 16-byte piece p of row x at p ^ ((x / 2) % 8), so that the 16 rows of a fragment's read meet all
+// banks; lane (r, g) reads pieces g and g + 4 - of E4M3 the 32 columns the instruction wants of it, of MXFP4 block g of
+// each of the stage's two steps.  MXFP4's block scales lie beside, 8 bytes a row in the order a lane reads them: 2 bytes, one a step.
+#pragma once
+
+#include "sg_mx_kernel.h"
+
+namespace sg {
+
+// The matrix instruction as text, accumulators in the accumulation registers: the builtin, which has no form that adds in place
+// for mixed formats, gives every accumulator of the tile two to four homes.  Scale bytes T of ws and XT of xs.  The two idle states
+// are what a vector instruction that wrote an operand would need.  The compiler does not know how long the result takes:
+// mx_drain ends every stage with the idle states of the longest one, and inside a stage an accumulator is touched by these
+// instructions only (tests/test_mx_codegen.py).
+template <int T, int XT>
+__device__ __forceinline__ void mfma_mx_acc(f32x4& c, const i32x4& w, const i32x4& x, int ws, int xs) {
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                 : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(XT & 1), "n"(T >> 1), "n"(XT >> 1));
+}
+template <int T>
+__device__ __forceinline__ void mfma_mx_acc(f32x4& c, const i32x4& w, const i32x8& x, int ws, int xs) {
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,0,0] op_sel_hi:[%6,0,0] cbsz:4"
+                 : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(T >> 1));
+}
+template <int NF, int MF>
+__device__ __forceinline__ void mx_drain(f32x4 (&acc)[NF][MF]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    // what follows uses the values of these, so a copy that the compiler makes stands behind the idle states
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) asm volatile("" : "+a"(acc[i][j]));
+}
+
+template <bool FP4, int NF, int MF, int WN, int WM>
+__global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
+    constexpr int THREADS = 64 * WN * WM, BM = 16 * MF * WM;
+    constexpr int S = FP4 ? 2 : 1;                       // steps of a stage
+    constexpr int U = 4 / S;                             // stages of a group of four steps
+    constexpr int PIECES = BM * 8 / THREADS;             // 16-byte pieces of a stage that a thread brings
+    static_assert(BM * 8 % THREADS == 0 && (!FP4 || THREADS >= BM), "tile");
+    constexpr int BUF = BM * 128 + (FP4 ? BM * 8 : 0);
+    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * BUF];
+
+    const int tid = threadIdx.x, lane = lane_id(), r = lane & 15, g = lane >> 4;
+    const int wave = wave_id(), wn = wave % WN, wm = wave / WN;
+    const MxPlace place = mx_place(a);
+    const int tn = place.tn, tm = place.tm;
+    const int m0 = tm * BM, tile0 = (tn * WN + wn) * NF;
+    const int k_blocks = a.k / kMxBlock;
+    const int pieces = FP4 ? k_blocks : 2 * k_blocks;    // of an activation row
+    const int first = place.q0 * U, stages = (place.q1 * U < (a.steps + S - 1) / S ? place.q1 * U : (a.steps + S - 1) / S);   // [first, stages)
+
+    // ---- activations: memory -> registers -> LDS ----
+    const uint8_t* xp[PIECES];
+    int xlds[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        const int row = (i * THREADS + tid) >> 3, p = tid & 7;
+        xp[i] = a.A + (size_t)(m0 + row < a.m ? m0 + row : a.m - 1) * ((size_t)pieces * 16);
+        xlds[i] = row * 128 + ((p ^ ((row >> 1) & 7)) << 4);
+    }
+    const uint8_t* sp = FP4 && tid < BM ? a.SA + (size_t)(m0 + tid < a.m ? m0 + tid : a.m - 1) * k_blocks : nullptr;
+    i32x4 xr[PIECES];
+    u32x2 sr = {0, 0};
+    auto load_x = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            // a piece beyond the row's end is zero: whatever weights it meets, the row's own last block's scale
+            const int p = 8 * s + (tid & 7);
+            xr[i] = *reinterpret_cast<const i32x4*>(xp[i] + (size_t)(p < pieces ? p : pieces - 1) * 16);
+            if (p >= pieces) xr[i] = i32x4{0, 0, 0, 0};
+        }
+        if (FP4 && tid < BM) {
+            if (8 * s + 8 <= k_blocks) {
+                __builtin_memcpy(&sr, sp + 8 * s, 8);
+            } else {
+                sr = u32x2{0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int b = 8 * s + e < k_blocks ? 8 * s + e : k_blocks - 1;
+                    sr[e / 4] |= (uint32_t)sp[b] << (8 * (e % 4));
+                }
+            }
+        }
+    };
+    auto store_x = [&](uint8_t* buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) *reinterpret_cast<i32x4*>(buf + xlds[i]) = xr[i];
+        if (FP4 && tid < BM) {
+            const uint32_t lo = sr.x, hi = sr.y;           // blocks 0-3 and 4-7 -> 0 4 1 5, 2 6 3 7
+            *reinterpret_cast<u32x2*>(buf + BM * 128 + tid * 8) =
+                u32x2{__builtin_amdgcn_perm(hi, lo, 0x05010400u), __builtin_amdgcn_perm(hi, lo, 0x07030602u)};
+        }
+    };
+
+    // ---- weights ----
+    const uint8_t* wp[NF];
+    const uint8_t* wsp[NF];
+#pragma unroll
+    for (int i = 0; i < NF; i++) {
+        const int tile = tile0 + i < a.tiles ? tile0 + i : a.tiles - 1;
+        wp[i] = a.P + (size_t)tile * a.pitch * kMxStepBytes + lane * 16;
+        wsp[i] = a.PS + (size_t)tile * a.quads * kMxQuadBytes + lane * 4;
+    }
+    i32x4 w[2][S][NF];
+    int ws[NF], ws_next[NF];
+    auto load_w = [&](int s, auto bc) __attribute__((always_inline)) {
+        constexpr int b = decltype(bc)::value;
+#pragma unroll
+        for (int t = 0; t < S; t++) {
+            const int step = S * s + t < a.steps ? S * s + t : a.steps - 1;
+#pragma unroll
+            for (int i = 0; i < NF; i++) w[b][t][i] = *reinterpret_cast<const i32x4*>(wp[i] + (size_t)step * kMxStepBytes);
+        }
+    };
+    auto load_ws = [&](int q) __attribute__((always_inline)) {
+        const int qq = q < a.quads ? q : a.quads - 1;
+#pragma unroll
+        for (int i = 0; i < NF; i++) ws_next[i] = *reinterpret_cast<const int*>(wsp[i] + (size_t)qq * kMxQuadBytes);
+    };
+
+    f32x4 acc[NF][MF];
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int rd = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+    auto multiply = [&](const uint8_t* buf, auto bc) __attribute__((always_inline)) {
+        constexpr int b = decltype(bc)::value;
+#pragma unroll
+        for (int j = 0; j < MF; j++) {
+            const uint8_t* x = buf + (wm * MF + j) * 2048 + rd;
+            const i32x4 lo = *reinterpret_cast<const i32x4*>(x);
+            const i32x4 hi = *reinterpret_cast<const i32x4*>(buf + (wm * MF + j) * 2048 + (rd ^ 64));
+            if constexpr (FP4) {
+                const int xs = *reinterpret_cast<const uint16_t*>(buf + BM * 128 + ((wm * MF + j) * 16 + r) * 8 + g * 2);
+#pragma unroll
+                for (int i = 0; i < NF; i++) mfma_mx_acc<0, 0>(acc[i][j], w[b][0][i], lo, ws[i], xs);
+#pragma unroll
+                for (int i = 0; i < NF; i++) mfma_mx_acc<1, 1>(acc[i][j], w[b][S - 1][i], hi, ws[i], xs);
+            } else {
+                const i32x8 x8 = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int i = 0; i < NF; i++) mfma_mx_acc<0>(acc[i][j], w[b][0][i], x8, ws[i], 127);
+            }
+        }
+        mx_drain(acc);
+    };
+
+    load_x(first);
+    load_ws(place.q0);
+    load_w(first, std::integral_constant<int, 0>{});
+    store_x(lds);
+    load_x(first + 1 < stages ? first + 1 : first);
+    __syncthreads();
+
+    // Stage s, of parity b: the next stage's activations from registers to the other buffer, loads for the stage behind that
+    // and the next weights, then the products.  The other buffer was last read in front of the barrier.
+    auto stage = [&](int s, auto bc) __attribute__((always_inline)) {
+        constexpr int b = decltype(bc)::value;
+        store_x(lds + (b ^ 1) * BUF);
+        load_x(s + 2 < stages ? s + 2 : stages - 1);
+        load_w(s + 1, std::integral_constant<int, b ^ 1>{});
+        if (s % U == 0) {
+#pragma unroll
+            for (int i = 0; i < NF; i++) ws[i] = ws_next[i];
+            load_ws(s / U + 1);
+        }
+        multiply(lds + b * BUF, bc);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NF; i++) ws[i] = (int)((unsigned)ws[i] >> (8 * S));      // the next stage's scales to the low bytes
+    };
+    int s = first;                                       // a multiple of U: even
+    for (; s + 1 < stages; s += 2) {
+        stage(s, std::integral_constant<int, 0>{});
+        stage(s + 1, std::integral_constant<int, 1>{});
+    }
+    if (s < stages) stage(s, std::integral_constant<int, 0>{});
+
+    const float scale = a.scale ? a.scale[0] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < MF; j++)
+#pragma unroll
+        for (int i = 0; i < NF; i++) mx_put(a, place.split, tile0 + i, (tm * WM + wm) * MF + j, lane, acc[i][j], scale);
+}
+
+}  // namespace sg

@@ -154,7 +154,7 @@ def mxfp4_pack(B: torch.Tensor, B_scales: torch.Tensor) -> torch.Tensor:
 @mxfp4_pack.register_fake
 def _(B, B_scales):
     tiles, steps = (B.shape[0] + 15) // 16, (B.shape[1] + 63) // 64
-    return B.new_empty((tiles * (steps * 1024 + (steps + 3) // 4 * 256),), dtype=torch.uint8)
+    return B.new_empty((tiles * ((steps + 1) // 2 * 2048 + (steps + 3) // 4 * 256),), dtype=torch.uint8)
 
 
 @torch.library.custom_op("sgemm::mxfp4_gemm", mutates_args=())

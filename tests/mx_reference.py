@@ -48,7 +48,7 @@ def pack(codes, scales):
     """The packed buffer: [tile][step][lane][16] codes, then [tile][four steps][lane][4] scales (rocm_dev_amd/csrc/sg_mx.h)."""
     n, k = codes.shape[0], codes.shape[1] * 2
     tiles, steps = -(-n // 16), -(-k // 128)
-    quads = -(-steps // 4)
+    quads, steps = -(-steps // 4), steps + steps % 2
     c = np.zeros((tiles * 16, steps * 64), np.uint8)
     c[:n, :k // 2] = codes
     s = np.full((tiles * 16, quads * 16), 127, np.uint8)

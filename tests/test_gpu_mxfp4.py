@@ -401,3 +401,43 @@ def test_operators_take_views_of_activations():
     B, SB = some_mx(rng, 40, 96)
     P = torch.ops.sgemm.mxfp4_pack(dev(B), dev(SB))
     torch.library.opcheck(torch.ops.sgemm.mxfp4_gemm, (Q, S, P, 40))
+
+
+# ---- every build, with and without a K split ----------------------------------------------------------------
+
+SMALL = [1101, 1108, 1201, 1204, 1208, 1301, 1304, 1308, 1404, 1604, 1702]
+TILES = [2005, 2006, 2010]
+WIDE = [3001, 3002, 3003, 3004, 3006]
+
+
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (3, 33, 512), (20, 70, 1120), (70, 130, 2080), (300, 515, 2400), (129, 257, 3584), (260, 300, 8288)])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5])
+def test_every_build(kind, m, n, k, splits):
+    quads = -(-k // 512)
+    if splits > quads:
+        pytest.skip("fewer groups of four steps than splits")
+    rng = np.random.default_rng(m + n + k)
+    B, SB = some_mx(rng, n, k)
+    A, SA = some_mx(rng, m, k) if kind == "mx" else (some_e4m3(rng, m, k), None)
+    P, a, sa = packed(B, SB), dev(A), None if SA is None else dev(SA)
+    row = rng.uniform(0.5, 1.5, m).astype(np.float32)
+    rs, scale = dev(row), torch.tensor([0.25], device="cuda")
+    want, slack = ref.gemm(ref.values(A, SA) if kind == "mx" else ref.e4m3(A), ref.values(B, SB), kind == "fp8act")
+    factor = 0.25 * row.astype(np.float64)[:, None]
+    st = torch.cuda.current_stream().cuda_stream
+    for build in SMALL + TILES + WIDE:
+        D = torch.full((m + 1, n), -7.0, dtype=torch.bfloat16, device="cuda")
+        for _ in range(2):       # the second on a workspace that holds the first's sums
+            rc = lib.sg_debug_mxfp4_gemm(a.data_ptr(), 0 if sa is None else sa.data_ptr(), P.data_ptr(), D.data_ptr(), scale.data_ptr(),
+                                         rs.data_ptr(), m, n, k, build + (10000 * splits if splits > 1 else 0), st)
+            assert rc == 0, build
+            ref.check(bits(D[:m]), want * factor, slack * factor)
+            assert (D[m] == -7).all(), build
+
+
+def test_debug_entry_refuses_builds_that_do_not_exist():
+    x = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    p = x.data_ptr()
+    for build in (1, 99, 1100, 1109, 1801, 2099, 3000, 3999, 21101):        # the last: two splits of one group
+        assert lib.sg_debug_mxfp4_gemm(p, 0, p, p, 0, 0, 1, 16, 128, build, 0) == 6, build

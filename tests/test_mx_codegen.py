@@ -1,0 +1,70 @@
+"""The generated code of the MXFP4 products whose matrix instructions are inline text (csrc/sg_mx_tile_kernel.h): the compiler
+knows nothing of their latency, so that no other instruction touches an accumulator too early is checked in the assembly."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rocm_dev_amd", "csrc")
+# A vector or memory instruction may read the result of the longest matrix instruction 19 wait states after it.
+WAIT_STATES = 19
+
+
+@pytest.fixture(scope="module")
+def kernels():
+    """{name: (instructions, resource report)} of the tile and wide kernels."""
+    if not shutil.which("hipcc") and not os.path.exists("/opt/rocm/bin/hipcc"):
+        pytest.skip("no hipcc")
+    subprocess.run(["make", "-s", "-C", CSRC, "obj/sg_mx_gemm.s"], check=True, capture_output=True)
+    text = open(os.path.join(CSRC, "obj", "sg_mx_gemm.s")).read()
+    out = {}
+    for m in re.finditer(r"^(_ZN2sg14mx_(?:tile|wide)_kernel\w*):[^\n]*\n(.*?)^\s*\.section", text, re.S | re.M):
+        code = [line.split(";")[0].strip() for line in m.group(2).splitlines()]
+        report = re.search(r"\.name:\s*%s\n(.*?)\.wavefront_size" % m.group(1), text, re.S).group(1)
+        out[m.group(1)] = ([c for c in code if c and not c.startswith(".") or c.startswith(".LBB")], report)
+    return out
+
+
+def _registers(kind, text):
+    regs = set()
+    for lo, hi in re.findall(r"\b%s\[(\d+):(\d+)\]" % kind, text):
+        regs.update(range(int(lo), int(hi) + 1))
+    regs.update(int(r) for r in re.findall(r"\b%s(\d+)\b" % kind, text))
+    return regs
+
+
+def test_there_are_kernels_to_look_at(kernels):
+    assert len(kernels) >= 10
+
+
+def test_no_accumulator_is_touched_while_it_is_being_written(kernels):
+    for name, (code, report) in kernels.items():
+        busy = {}                                # accumulator register -> wait states since its matrix instruction
+        matrix = 0
+        for instruction in code:
+            if instruction.startswith(".LBB"):   # (a branch target: every path to it ends behind a stage's idle states)
+                continue
+            regs = _registers("a", instruction)
+            if instruction.startswith("v_mfma"):
+                matrix += 1
+                busy = {r: s + 1 for r, s in busy.items()}
+                busy.update({r: 0 for r in regs})
+                continue
+            early = [r for r in regs if busy.get(r, WAIT_STATES) < WAIT_STATES]
+            assert not early, "%s: %s: a%d is touched %d wait states behind its matrix instruction" % (name, instruction, early[0], busy[early[0]])
+            nop = re.match(r"s_nop (\d+)", instruction)
+            busy = {r: s + (int(nop.group(1)) + 1 if nop else 1) for r, s in busy.items()}
+        assert matrix > 0, name
+        for key in ("vgpr_spill_count",):
+            assert int(re.search(r"\.%s:\s*(\d+)" % key, report).group(1)) == 0, (name, key)
+
+
+def test_matrix_instructions_wait_for_vector_instructions_that_wrote_an_operand(kernels):
+    """Two idle states stand in front of every one of them."""
+    for name, (code, _) in kernels.items():
+        for before, instruction in zip(code, code[1:]):
+            if instruction.startswith("v_mfma"):
+                nop = re.match(r"s_nop (\d+)", before)
+                assert nop and int(nop.group(1)) >= 1, (name, instruction)

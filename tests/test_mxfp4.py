@@ -56,7 +56,7 @@ def test_reference_e4m3_is_torchs():
     assert np.array_equal(ref.e4m3(c), want, equal_nan=True)
 
 
-@pytest.mark.parametrize("n,k,want", [(1, 32, 1024 + 256), (16, 128, 1024 + 256), (17, 128, 2 * (1024 + 256)), (16, 640, 5 * 1024 + 512),
+@pytest.mark.parametrize("n,k,want", [(1, 32, 2048 + 256), (16, 256, 2048 + 256), (17, 128, 2 * (2048 + 256)), (16, 640, 6 * 1024 + 512),
                                       (4096, 4096, 4096 * 4096 // 32 * 17), (1 << 20, 32768, (1 << 30) * 17)])
 def test_packed_bytes(n, k, want):
     assert sg.mxfp4_packed_bytes(n, k) == want
@@ -103,19 +103,19 @@ def _u8(*shape):
     lambda: sg.mxfp4_encode_rows(torch.zeros(64, 4, dtype=torch.bfloat16).t(), _u8(4, 32), _u8(4, 2)),
     lambda: sg.mxfp4_encode_rows(torch.zeros(4, 64, dtype=torch.bfloat16), _u8(4, 32), _u8(4, 2)),           # not on a GPU
     lambda: sg.mxfp4_decode_rows(_u8(4, 32), _u8(2, 4).t(), torch.zeros(4, 64, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_pack(_u8(16, 40), _u8(16, 2), _u8(1280)),
-    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 3), _u8(1280)),
-    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 2), _u8(1279)),
-    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 2), _u8(2560)[::2]),
-    lambda: sg.mxfp4_pack(_u8(32, 16).t(), _u8(16, 2), _u8(1280)),
-    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 2), _u8(1280), torch.zeros(5, 16, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 2), _u8(1280), torch.zeros(4, 17, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 1), _u8(1280), torch.zeros(4, 16, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm(_u8(4, 24), _u8(4, 1), _u8(1280), torch.zeros(4, 16, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 48), _u8(1280), torch.zeros(4, 16, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm_fp8act(_u8(64, 4).t(), _u8(1280), torch.zeros(4, 16, dtype=torch.bfloat16)),
-    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 64), _u8(1280), torch.zeros(16, 4, dtype=torch.bfloat16).t()),
-    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 64), _u8(1280), torch.zeros(4, 16, dtype=torch.bfloat16)),           # not on a GPU
+    lambda: sg.mxfp4_pack(_u8(16, 40), _u8(16, 2), _u8(2304)),
+    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 3), _u8(2304)),
+    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 2), _u8(2303)),
+    lambda: sg.mxfp4_pack(_u8(16, 32), _u8(16, 2), _u8(4608)[::2]),
+    lambda: sg.mxfp4_pack(_u8(32, 16).t(), _u8(16, 2), _u8(2304)),
+    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 2), _u8(2304), torch.zeros(5, 16, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 2), _u8(2304), torch.zeros(4, 17, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm(_u8(4, 32), _u8(4, 1), _u8(2304), torch.zeros(4, 16, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm(_u8(4, 24), _u8(4, 1), _u8(2304), torch.zeros(4, 16, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 48), _u8(2304), torch.zeros(4, 16, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm_fp8act(_u8(64, 4).t(), _u8(2304), torch.zeros(4, 16, dtype=torch.bfloat16)),
+    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 64), _u8(2304), torch.zeros(16, 4, dtype=torch.bfloat16).t()),
+    lambda: sg.mxfp4_gemm_fp8act(_u8(4, 64), _u8(2304), torch.zeros(4, 16, dtype=torch.bfloat16)),           # not on a GPU
 ])
 def test_python_refuses(call):
     with pytest.raises(ValueError):

@@ -86,6 +86,10 @@ int sg_debug_cu_ingest(const uint8_t* cold, size_t cold_bytes, const uint8_t* ho
 int sg_debug_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D_bf16, const float* scale_tensor,
                         const float* row_scales, int m, int n, int k, int build, void* stream);
 
+/* ... and the build that sg_mxfp4_gemm (fp4_activations) or sg_mxfp4_gemm_fp8act launches for the shape on 256 CUs, plus 10000 times
+ * the K splits where there are any; workspace = 0: under capture.  0 for a shape that they refuse. */
+int sg_debug_mxfp4_choice(int fp4_activations, int m, int n, int k, int workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,4 +78,9 @@ int sg_debug_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t
     return gemm(A_scales != nullptr, build, A, A_scales, P, D, scale_tensor, row_scales, m, n, k, stream);
 }
 
+int sg_debug_mxfp4_choice(int fp4_activations, int m, int n, int k, int workspace) {
+    if (m <= 0 || n <= 0 || k <= 0 || k % kMxBlock) return 0;
+    return mx_choice(fp4_activations != 0, m, n, k, 256, workspace != 0);
+}
+
 }  // extern "C"

@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "sg_mx_choice.h"
 #include "sg_mx_wide_kernel.h"
 
 namespace sg {
@@ -81,21 +82,47 @@ static int launch_build(int build, MxArgs& a, hipStream_t stream) {
         case 3004: return launch_mx_wide<FP4, 6, 8, 3, 2>(a, stream);
         case 3005: return launch_mx_wide<FP4, 4, 8, 3, FP4 ? 2 : 3>(a, stream);
         case 3006: return launch_mx_wide<FP4, 4, 4, 3, 3>(a, stream);
+        case 3007: return launch_mx_wide<FP4, 4, 4, 2, 2>(a, stream);
+        case 3008: return launch_mx_wide<FP4, 6, 4, 2, 2>(a, stream);
         default: return SG_INVALID_CONFIG;
     }
 }
 
-static int pick_mx(const MxArgs& a, int cu_count) {
-    const int waves = a.quads < 8 ? a.quads : 8;      // waves that have a share of K
-    if (a.m <= 16) return 1100 + waves;
-    if (a.m <= 32) return 1300 + waves;
-    if (a.m <= 128) return 2002;
-    return 2001;
+// The build that a call without one runs.  The search takes about a microsecond of host time, so a thread keeps the last few
+// shapes' answers: a function of the shape, of nothing else.
+static int pick_mx(bool fp4, const MxArgs& a, int cu_count, bool workspace) {
+    struct Kept {
+        int m, n, k, flags, build;
+    };
+    static thread_local Kept kept[16];
+    const bool copy = fp4 && !scales_lie_right(a);
+    const int flags = 1 | (fp4 ? 2 : 0) | (copy ? 4 : 0) | (workspace ? 8 : 0) | cu_count << 4;
+    Kept& e = kept[((unsigned)a.m * 31u + (unsigned)a.n * 17u + (unsigned)a.k / 32u + (unsigned)flags) % 16];
+    if (e.m != a.m || e.n != a.n || e.k != a.k || e.flags != flags)
+        e = Kept{a.m, a.n, a.k, flags, mx_choose(fp4, a.m, a.n, a.k, cu_count, workspace, copy)};
+    return e.build;
 }
 
+int mx_choice(bool fp4, int m, int n, int k, int cu_count, bool workspace) {
+    return mx_choose(fp4, m, n, k, cu_count, workspace, fp4 && k % 512 != 0);
+}
+
+static int launch_mx(bool fp4, int build, MxArgs& a, hipStream_t stream);
+
 int launch_mx_gemm(bool fp4, int build, MxArgs& a, int cu_count, hipStream_t stream) {
+    if (build) return launch_mx(fp4, build, a, stream);
+    build = pick_mx(fp4, a, cu_count, true);
+    // A recorded launch uses no memory of the library's, so that graphs may replay side by side; a launch without device
+    // memory for it runs what needs none.
+    const bool shares = build >= 10000 || (fp4 && build >= 3000 && !scales_lie_right(a));
+    if (shares && stream_is_capturing(stream)) return launch_mx(fp4, pick_mx(fp4, a, cu_count, false), a, stream);
+    const int rc = launch_mx(fp4, build, a, stream);
+    if (shares && (rc == SG_NO_DEVICE || rc == SG_WORKSPACE_TOO_SMALL)) return launch_mx(fp4, pick_mx(fp4, a, cu_count, false), a, stream);
+    return rc;
+}
+
+static int launch_mx(bool fp4, int build, MxArgs& a, hipStream_t stream) {
     a.splits = 1;
-    if (build == 0) build = pick_mx(a, cu_count);
     const int splits = build / 10000 < 1 ? 1 : build / 10000;
     build %= 10000;
     if (splits > a.quads) return SG_INVALID_CONFIG;

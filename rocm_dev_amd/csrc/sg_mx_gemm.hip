@@ -27,11 +27,11 @@ static int launch_small(MxArgs& a, int waves, hipStream_t stream) {
     return report_hip("mx_gemm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
-template <bool FP4, int NF, int MF, int WN, int WM>
+template <bool FP4, int NF, int MF, int WN, int WM, int WR = 2, int XR = 1>
 static int launch_tile(MxArgs& a, hipStream_t stream) {
     const unsigned grid = mx_grid(a, 16 * NF * WN, 16 * MF * WM);
     if (!grid) return SG_BAD_ARGUMENT;
-    mx_tile_kernel<FP4, NF, MF, WN, WM><<<grid, 64 * WN * WM, 0, stream>>>(a);
+    mx_tile_kernel<FP4, NF, MF, WN, WM, WR, XR><<<grid, 64 * WN * WM, 0, stream>>>(a);
     return report_hip("mx_tile launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
@@ -76,6 +76,12 @@ static int launch_build(int build, MxArgs& a, hipStream_t stream) {
         case 2008: return launch_tile<FP4, 1, 4, 2, 1>(a, stream);   //  32 x 64
         case 2009: return launch_tile<FP4, 1, 2, 2, 1>(a, stream);   //  32 x 32
         case 2010: return launch_tile<FP4, 2, 4, 4, 1>(a, stream);   // 128 x 64
+        case 2011: return launch_tile<FP4, 2, 4, 4, 1, 4, 2>(a, stream);
+        case 2012: return launch_tile<FP4, 1, 2, 4, 1, 4, 2>(a, stream);
+        case 2013: return launch_tile<FP4, 1, 4, 4, 1, 4, 2>(a, stream);
+        case 2014: return launch_tile<FP4, 2, 8, 4, 1, 4, 2>(a, stream);
+        case 2015: return launch_tile<FP4, 2, 2, 4, 1, 4, 2>(a, stream);
+        case 2016: return launch_tile<FP4, 1, 4, 2, 1, 4, 2>(a, stream);
         case 3001: return launch_mx_wide<FP4, 8, 8, FP4 ? 2 : 3, FP4 ? 2 : 3>(a, stream);
         case 3002: return launch_mx_wide<FP4, 6, 4, 3, 3>(a, stream);
         case 3003: return launch_mx_wide<FP4, 8, 4, 3, 3>(a, stream);

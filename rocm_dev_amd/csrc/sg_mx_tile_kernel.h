@@ -2,9 +2,9 @@
 //
 // A workgroup of WN x WM waves owns 16 * NF * WN weight rows by 16 * MF * WM activation rows, a wave NF x MF fragments of
 // 16 x 16.  A stage is 128 bytes of every activation row: 128 columns of E4M3 (one step of the matrix instruction) or 256 of
-// MXFP4 (two).  The activations of a stage, which all waves along n read, go through LDS, two buffers, one barrier a stage; the
+// MXFP4 (two).  The activations of a stage, which all waves along n read, go through LDS, two buffers, one barrier a stage (and through registers, so that the compiler's own waits order everything); the
 // weights, which only the WM waves along m share, go straight to registers by contiguous KBs of the packed buffer (sg_mx.h):
-// through LDS they would be a quarter (E4M3) to a half (MXFP4) of its traffic.  Both are asked for a stage ahead.
+// through LDS they would be a quarter (E4M3) to a half (MXFP4) of its traffic.
 //
 // LDS: row x 128 bytes, the 16-byte piece p of row x at p ^ ((x / 2) % 8), so that the 16 rows of a fragment's read meet all
 // banks; lane (r, g) reads pieces g and g + 4 - of E4M3 the 32 columns the instruction wants of it, of MXFP4 block g of
@@ -40,8 +40,10 @@ __device__ __forceinline__ void mx_drain(f32x4 (&acc)[NF][MF]) {
         for (int j = 0; j < MF; j++) asm volatile("" : "+a"(acc[i][j]));
 }
 
-template <bool FP4, int NF, int MF, int WN, int WM>
+// WR: ring of weight stages in registers, asked for WR - 1 stages ahead; XR: of activation stages on their way to LDS, XR ahead.
+template <bool FP4, int NF, int MF, int WN, int WM, int WR, int XR>
 __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
+    static_assert((WR == 2 && XR == 1) || (WR == 4 && XR == 2), "the loops' unrolled stages leave both rings and the LDS buffers in phase");
     constexpr int THREADS = 64 * WN * WM, BM = 16 * MF * WM;
     constexpr int S = FP4 ? 2 : 1;                       // steps of a stage
     constexpr int U = 4 / S;                             // stages of a group of four steps
@@ -69,34 +71,36 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
         xlds[i] = row * 128 + ((p ^ ((row >> 1) & 7)) << 4);
     }
     const uint8_t* sp = FP4 && tid < BM ? a.SA + (size_t)(m0 + tid < a.m ? m0 + tid : a.m - 1) * k_blocks : nullptr;
-    i32x4 xr[PIECES];
-    u32x2 sr = {0, 0};
-    auto load_x = [&](int s) __attribute__((always_inline)) {
+    i32x4 xr[XR][PIECES];
+    u32x2 sr[XR];
+    auto load_x = [&](int s, auto qc) __attribute__((always_inline)) {
+        constexpr int q = decltype(qc)::value;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            // a piece beyond the row's end is zero: whatever weights it meets, the row's own last block's scale
             const int p = 8 * s + (tid & 7);
-            xr[i] = *reinterpret_cast<const i32x4*>(xp[i] + (size_t)(p < pieces ? p : pieces - 1) * 16);
-            if (p >= pieces) xr[i] = i32x4{0, 0, 0, 0};
+            xr[q][i] = *reinterpret_cast<const i32x4*>(xp[i] + (size_t)(p < pieces ? p : pieces - 1) * 16);
         }
         if (FP4 && tid < BM) {
             if (8 * s + 8 <= k_blocks) {
-                __builtin_memcpy(&sr, sp + 8 * s, 8);
+                __builtin_memcpy(&sr[q], sp + 8 * s, 8);
             } else {
-                sr = u32x2{0, 0};
+                sr[q] = u32x2{0, 0};
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int b = 8 * s + e < k_blocks ? 8 * s + e : k_blocks - 1;
-                    sr[e / 4] |= (uint32_t)sp[b] << (8 * (e % 4));
+                    sr[q][e / 4] |= (uint32_t)sp[b] << (8 * (e % 4));
                 }
             }
         }
     };
-    auto store_x = [&](uint8_t* buf) __attribute__((always_inline)) {
+    auto store_x = [&](int s, uint8_t* buf, auto qc) __attribute__((always_inline)) {
+        constexpr int q = decltype(qc)::value;
+        // a piece beyond the row's end is zero: whatever weights it meets, under the scale of the row's own last block
+        const bool beyond = 8 * s + (tid & 7) >= pieces;
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) *reinterpret_cast<i32x4*>(buf + xlds[i]) = xr[i];
+        for (int i = 0; i < PIECES; i++) *reinterpret_cast<i32x4*>(buf + xlds[i]) = beyond ? i32x4{0, 0, 0, 0} : xr[q][i];
         if (FP4 && tid < BM) {
-            const uint32_t lo = sr.x, hi = sr.y;           // blocks 0-3 and 4-7 -> 0 4 1 5, 2 6 3 7
+            const uint32_t lo = sr[q].x, hi = sr[q].y;           // blocks 0-3 and 4-7 -> 0 4 1 5, 2 6 3 7
             *reinterpret_cast<u32x2*>(buf + BM * 128 + tid * 8) =
                 u32x2{__builtin_amdgcn_perm(hi, lo, 0x05010400u), __builtin_amdgcn_perm(hi, lo, 0x07030602u)};
         }
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
         wp[i] = a.P + (size_t)tile * a.pitch * kMxStepBytes + lane * 16;
         wsp[i] = a.PS + (size_t)tile * a.quads * kMxQuadBytes + lane * 4;
     }
-    i32x4 w[2][S][NF];
+    i32x4 w[WR][S][NF];
     int ws[NF], ws_next[NF];
     auto load_w = [&](int s, auto bc) __attribute__((always_inline)) {
         constexpr int b = decltype(bc)::value;
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
 
     const int rd = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
     auto multiply = [&](const uint8_t* buf, auto bc) __attribute__((always_inline)) {
-        constexpr int b = decltype(bc)::value;
+        constexpr int b = decltype(bc)::value;             // of the weight ring
 #pragma unroll
         for (int j = 0; j < MF; j++) {
             const uint8_t* x = buf + (wm * MF + j) * 2048 + rd;
@@ -157,36 +161,54 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
         mx_drain(acc);
     };
 
-    load_x(first);
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    const auto in = [&](int s) __attribute__((always_inline)) { return s < stages ? s : stages - 1; };
+    load_x(first, I0{});
     load_ws(place.q0);
-    load_w(first, std::integral_constant<int, 0>{});
-    store_x(lds);
-    load_x(first + 1 < stages ? first + 1 : first);
+    load_w(first, I0{});
+    store_x(first, lds, I0{});
+    load_x(in(first + 1), std::integral_constant<int, 1 % XR>{});
+    if constexpr (XR == 2) load_x(in(first + 2), I0{});
+    if constexpr (WR == 4) {
+        load_w(in(first + 1), I1{});
+        load_w(in(first + 2), std::integral_constant<int, 2 % WR>{});
+    }
     __syncthreads();
 
-    // Stage s, of parity b: the next stage's activations from registers to the other buffer, loads for the stage behind that
-    // and the next weights, then the products.  The other buffer was last read in front of the barrier.
-    auto stage = [&](int s, auto bc) __attribute__((always_inline)) {
-        constexpr int b = decltype(bc)::value;
-        store_x(lds + (b ^ 1) * BUF);
-        load_x(s + 2 < stages ? s + 2 : stages - 1);
-        load_w(s + 1, std::integral_constant<int, b ^ 1>{});
+    // Stage s, the c-th of the unrolled ones: the next stage's activations from registers to the other buffer, loads (LAST: where
+    // there is such a stage) into what that frees, then the products.  The other buffer was last read in front of the barrier.
+    auto stage = [&](int s, auto cc, auto lc) __attribute__((always_inline)) {
+        constexpr int c = decltype(cc)::value, x = (c + 1) % XR;
+        constexpr bool LAST = decltype(lc)::value;
+        store_x(s + 1, lds + (c & 1 ? 0 : BUF), std::integral_constant<int, x>{});
+        if (!LAST || s + 1 + XR < stages) load_x(s + 1 + XR, std::integral_constant<int, x>{});
+        if (!LAST || s + WR - 1 < stages) load_w(s + WR - 1, std::integral_constant<int, (c + WR - 1) % WR>{});
         if (s % U == 0) {
 #pragma unroll
             for (int i = 0; i < NF; i++) ws[i] = ws_next[i];
             load_ws(s / U + 1);
         }
-        multiply(lds + b * BUF, bc);
+        multiply(lds + (c & 1 ? BUF : 0), std::integral_constant<int, c % WR>{});
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NF; i++) ws[i] = (int)((unsigned)ws[i] >> (8 * S));      // the next stage's scales to the low bytes
     };
+    constexpr std::false_type MORE{};
+    constexpr std::true_type LAST{};
     int s = first;                                       // a multiple of U: even
-    for (; s + 1 < stages; s += 2) {
-        stage(s, std::integral_constant<int, 0>{});
-        stage(s + 1, std::integral_constant<int, 1>{});
+    for (; s + 3 + WR - 1 < stages; s += 4) {            // every load is of a stage there is
+        stage(s, I0{}, MORE);
+        stage(s + 1, I1{}, MORE);
+        stage(s + 2, std::integral_constant<int, 2>{}, MORE);
+        stage(s + 3, std::integral_constant<int, 3>{}, MORE);
     }
-    if (s < stages) stage(s, std::integral_constant<int, 0>{});
+    for (; s < stages; s += 4) {
+        stage(s, I0{}, LAST);
+        if (s + 1 < stages) stage(s + 1, I1{}, LAST);
+        if (s + 2 < stages) stage(s + 2, std::integral_constant<int, 2>{}, LAST);
+        if (s + 3 < stages) stage(s + 3, std::integral_constant<int, 3>{}, LAST);
+    }
 
     const float scale = a.scale ? a.scale[0] : 1.0f;
 #pragma unroll

@@ -27,7 +27,7 @@ static int launch_small(MxArgs& a, int waves, hipStream_t stream) {
     return report_hip("mx_gemm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
-template <bool FP4, int NF, int MF, int WN, int WM, int WR = 2, int XR = 1>
+template <bool FP4, int NF, int MF, int WN, int WM, int WR, int XR>
 static int launch_tile(MxArgs& a, hipStream_t stream) {
     const unsigned grid = mx_grid(a, 16 * NF * WN, 16 * MF * WM);
     if (!grid) return SG_BAD_ARGUMENT;
@@ -59,37 +59,25 @@ static int launch_build(int build, MxArgs& a, hipStream_t stream) {
     const int waves = build % 100;
     if (build < 2000 && (waves < 1 || waves > 8)) return SG_INVALID_CONFIG;
     switch (build < 2000 ? build / 100 : build) {
-        case 11: return launch_small<FP4, 1, 1>(a, waves, stream);
-        case 12: return launch_small<FP4, 2, 1>(a, waves, stream);
-        case 13: return launch_small<FP4, 2, 2>(a, waves, stream);
-        case 14: return launch_small<FP4, 1, 2>(a, waves, stream);
-        case 15: return launch_small<FP4, 1, 4>(a, waves, stream);
-        case 16: return launch_small<FP4, 2, 4>(a, waves, stream);
-        case 17: return launch_small<FP4, 4, 1>(a, waves, stream);
-        case 2001: return launch_tile<FP4, 2, 4, 4, 2>(a, stream);   // 128 weight rows x 128 activation rows
-        case 2002: return launch_tile<FP4, 2, 2, 4, 2>(a, stream);   // 128 x 64
-        case 2003: return launch_tile<FP4, 1, 4, 4, 2>(a, stream);   //  64 x 128
-        case 2004: return launch_tile<FP4, 1, 2, 4, 2>(a, stream);   //  64 x 64
-        case 2005: return launch_tile<FP4, 2, 8, 4, 1>(a, stream);   // 128 x 128
-        case 2006: return launch_tile<FP4, 1, 2, 4, 1>(a, stream);   //  64 x 32
-        case 2007: return launch_tile<FP4, 1, 4, 4, 1>(a, stream);   //  64 x 64
-        case 2008: return launch_tile<FP4, 1, 4, 2, 1>(a, stream);   //  32 x 64
-        case 2009: return launch_tile<FP4, 1, 2, 2, 1>(a, stream);   //  32 x 32
-        case 2010: return launch_tile<FP4, 2, 4, 4, 1>(a, stream);   // 128 x 64
-        case 2011: return launch_tile<FP4, 2, 4, 4, 1, 4, 2>(a, stream);
-        case 2012: return launch_tile<FP4, 1, 2, 4, 1, 4, 2>(a, stream);
-        case 2013: return launch_tile<FP4, 1, 4, 4, 1, 4, 2>(a, stream);
-        case 2014: return launch_tile<FP4, 2, 8, 4, 1, 4, 2>(a, stream);
-        case 2015: return launch_tile<FP4, 2, 2, 4, 1, 4, 2>(a, stream);
-        case 2016: return launch_tile<FP4, 1, 4, 2, 1, 4, 2>(a, stream);
-        case 3001: return launch_mx_wide<FP4, 8, 8, FP4 ? 2 : 3, FP4 ? 2 : 3>(a, stream);
-        case 3002: return launch_mx_wide<FP4, 6, 4, 3, 3>(a, stream);
-        case 3003: return launch_mx_wide<FP4, 8, 4, 3, 3>(a, stream);
-        case 3004: return launch_mx_wide<FP4, 6, 8, 3, 2>(a, stream);
-        case 3005: return launch_mx_wide<FP4, 4, 8, 3, FP4 ? 2 : 3>(a, stream);
-        case 3006: return launch_mx_wide<FP4, 4, 4, 3, 3>(a, stream);
-        case 3007: return launch_mx_wide<FP4, 4, 4, 2, 2>(a, stream);
-        case 3008: return launch_mx_wide<FP4, 6, 4, 2, 2>(a, stream);
+        case 11: return launch_small<FP4, 1, 1>(a, waves, stream);   // 16 weight rows x 16 activation rows
+        case 12: return launch_small<FP4, 2, 1>(a, waves, stream);   // 32 x 16
+        case 13: return launch_small<FP4, 2, 2>(a, waves, stream);   // 32 x 32
+        case 14: return launch_small<FP4, 1, 2>(a, waves, stream);   // 16 x 32
+        case 16: return launch_small<FP4, 2, 4>(a, waves, stream);   // 32 x 64
+        case 17: return launch_small<FP4, 4, 1>(a, waves, stream);   // 64 x 16
+        case 2001: return launch_tile<FP4, 2, 4, 4, 2, 2, 1>(a, stream);   // 128 x 128, eight waves
+        case 2005: return launch_tile<FP4, 2, 8, 4, 1, 2, 1>(a, stream);   // 128 x 128, four
+        case 2010: return launch_tile<FP4, 2, 4, 4, 1, 2, 1>(a, stream);   // 128 x 64
+        case 2011: return launch_tile<FP4, 2, 4, 4, 1, 4, 2>(a, stream);   // 128 x 64, deep rings (and below)
+        case 2012: return launch_tile<FP4, 1, 2, 4, 1, 4, 2>(a, stream);   //  64 x 32
+        case 2013: return launch_tile<FP4, 1, 4, 4, 1, 4, 2>(a, stream);   //  64 x 64
+        case 2015: return launch_tile<FP4, 2, 2, 4, 1, 4, 2>(a, stream);   // 128 x 32
+        case 3001: return launch_mx_wide<FP4, 8, 8, FP4 ? 2 : 3, FP4 ? 2 : 3>(a, stream);   // 256 x 256
+        case 3002: return launch_mx_wide<FP4, 6, 4, 3, 3>(a, stream);                       // 192 x 128
+        case 3003: return launch_mx_wide<FP4, 8, 4, 3, 3>(a, stream);                       // 256 x 128
+        case 3004: return launch_mx_wide<FP4, 6, 8, 3, 2>(a, stream);                       // 192 x 256
+        case 3006: return launch_mx_wide<FP4, 4, 4, 3, 3>(a, stream);                       // 128 x 128
+        case 3007: return launch_mx_wide<FP4, 4, 4, 2, 2>(a, stream);                       // 128 x 128, two workgroups a CU
         default: return SG_INVALID_CONFIG;
     }
 }

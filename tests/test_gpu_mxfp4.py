@@ -436,6 +436,67 @@ def test_every_build(kind, m, n, k, splits):
             assert (D[m] == -7).all(), build
 
 
+@pytest.mark.parametrize("kind", ["mx", "fp8act"])
+@pytest.mark.parametrize("m,n,k", [(20, 70, 1120), (140, 200, 2080), (300, 300, 1536)])
+def test_every_build_keeps_nan_in_its_row_and_column(kind, m, n, k):
+    """A NaN in the last block of a row and in the last of a weight row: what stands in for columns beyond k may not spread it."""
+    rng = np.random.default_rng(m)
+    B, SB = some_mx(rng, n, k)
+    A, SA = some_mx(rng, m, k) if kind == "mx" else (some_e4m3(rng, m, k), None)
+    SB[n - 1, -1] = 255
+    if kind == "mx":
+        SA[m - 2, -1] = 255
+    else:
+        A[m - 2, -1] = 0x7f
+    P, a, sa = packed(B, SB), dev(A), None if SA is None else dev(SA)
+    want, slack = ref.gemm(ref.values(A, SA) if kind == "mx" else ref.e4m3(A), ref.values(B, SB), kind == "fp8act")
+    for build in SMALL + TILES + WIDE + [20000 + WIDE[0], 20000 + TILES[0], 20000 + SMALL[1]]:
+        D = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        assert lib.sg_debug_mxfp4_gemm(a.data_ptr(), 0 if sa is None else sa.data_ptr(), P.data_ptr(), D.data_ptr(), 0, 0, m, n, k, build,
+                                       torch.cuda.current_stream().cuda_stream) == 0
+        ref.check(bits(D), want, slack)
+        assert int(torch.isnan(D).sum()) == m + n - 1, build
+
+
+@pytest.mark.parametrize("kind,m,n,k", [("fp8act", 8, 256, 16384), ("mx", 200, 512, 8192 + 32), ("mx", 600, 2048, 2880),
+                                         ("mx", 1024, 4096, 5440)])
+def test_recorded_launches_take_none_of_the_librarys_memory(kind, m, n, k):
+    """Shapes that split K, or copy scales, in an eager call: recorded they do neither, and replay beside eager calls."""
+    rng = np.random.default_rng(k)
+    B, SB = some_mx(rng, n, k)
+    P = packed(B, SB)
+    if kind == "mx":
+        A, SA = some_mx(rng, m, k)
+        ops, v = (dev(A), dev(SA), P), ref.values(A, SA)
+        run = lambda D: sg.mxfp4_gemm(*ops, D, check=True)  # noqa: E731
+    else:
+        A = some_e4m3(rng, m, k)
+        ops, v = (dev(A), P), ref.e4m3(A)
+        run = lambda D: sg.mxfp4_gemm_fp8act(*ops, D, check=True)  # noqa: E731
+    want, slack = ref.gemm(v, ref.values(B, SB), kind == "fp8act")
+    D, E = (torch.zeros((m, n), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    side = torch.cuda.Stream()
+    sg.release_workspaces()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run(D)
+    assert sg.workspace_bytes() == 0
+    for _ in range(3):
+        D.zero_()
+        E.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        run(E)
+        run(E)
+        torch.cuda.synchronize()
+        for out in (D, E):
+            ref.check(bits(out), want, slack)
+    build = lib.sg_debug_mxfp4_choice(kind == "mx", m, n, k, 1)
+    assert (sg.workspace_bytes() > 0) == (build > 10000 or (kind == "mx" and build >= 3000 and k % 512 != 0))
+    sg.release_workspaces()
+
+
 def test_debug_entry_refuses_builds_that_do_not_exist():
     x = torch.zeros(4096, dtype=torch.uint8, device="cuda")
     p = x.data_ptr()

@@ -145,3 +145,31 @@ def test_registered_operators_infer_their_shapes():
     D = torch.ops.sgemm.mxfp4_gemm(Q, S, meta(100), 33)
     assert D.shape == (5, 33) and D.dtype == torch.bfloat16
     assert torch.ops.sgemm.mxfp4_gemm_fp8act(meta(5, 96), meta(100), 33).shape == (5, 33)
+
+
+SPLIT, WIDE = 10000, 3000
+
+
+@pytest.mark.parametrize("fp4", [0, 1])
+def test_choice_without_a_workspace_needs_none(fp4):
+    """Under capture: no K split, and no build that would have to copy scales."""
+    rng = np.random.default_rng(0)
+    for _ in range(300):
+        m, n, k = int(np.exp(rng.uniform(0, 8))), int(np.exp(rng.uniform(0, 11))), 32 * int(np.exp(rng.uniform(0, 7)))
+        build = lib.sg_debug_mxfp4_choice(fp4, m, n, k, 0)
+        assert 1100 < build < SPLIT
+        if fp4 and k % 512:
+            assert build < WIDE
+        splits, build = divmod(lib.sg_debug_mxfp4_choice(fp4, m, n, k, 1), SPLIT)
+        assert 1100 < build < 3100 and splits <= max(1, -(-k // 512))
+
+
+def test_choice_refuses_what_the_products_refuse():
+    for shape in ((0, 16, 64), (4, 0, 64), (4, 16, 0), (4, 16, 48)):
+        assert lib.sg_debug_mxfp4_choice(1, *shape, 1) == 0
+
+
+def test_choice_splits_few_tiles_with_a_long_k_only():
+    assert lib.sg_debug_mxfp4_choice(0, 8, 256, 16384, 1) >= SPLIT
+    assert lib.sg_debug_mxfp4_choice(0, 8, 28672, 4096, 1) < SPLIT
+    assert WIDE < lib.sg_debug_mxfp4_choice(1, 1024, 57344, 8192, 1) < SPLIT

@@ -374,7 +374,11 @@ int    sg_mxfp4_pack(const uint8_t* B, const uint8_t* B_scales, uint8_t* P, int 
  *                           (sg_fp8_encode_rows, whose scales are row_scales)
  * with fp32 sums in a fixed order and separately rounded fp32 products.  scale_tensor (one float) and row_scales ([m] floats) may be
  * NULL (factor 1).  Any m and n, k a multiple of 32; A and P 16-byte, D 8-byte aligned, A_scales at any address.  A NaN in an operand
- * (a block scale of 255, an E4M3 NaN) makes the outputs of its row or column NaN.  P must come from sg_mxfp4_pack with the same n and k. */
+ * (a block scale of 255, an E4M3 NaN) makes the outputs of its row or column NaN.  P must come from sg_mxfp4_pack with the same n and k.
+ * Few output tiles with a long k share it among workgroups, and many rows of MXFP4 activations whose k is no multiple of 512 have
+ * their scales copied first: both in the stream's workspace (above), except under capture, where a launch uses none - its sums
+ * may then be added up in another order than an eager call's - as a call does that can get no device memory.  E4M3 products are cut off about
+ * 14 binades below the largest of a run of 8, as in the E4M3 GEMMs. */
 int sg_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, void* D_bf16, const float* scale_tensor,
                   int m, int n, int k, void* stream);
 int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const float* scale_tensor, const float* row_scales,

@@ -9,6 +9,10 @@
 // LDS: row x 128 bytes, the 16-byte piece p of row x at p ^ ((x / 2) % 8), so that the 16 rows of a fragment's read meet all
 // banks; lane (r, g) reads pieces g and g + 4 - of E4M3 the 32 columns the instruction wants of it, of MXFP4 block g of
 // each of the stage's two steps.  MXFP4's block scales lie beside, 8 bytes a row in the order a lane reads them: 2 bytes, one a step.
+//
+// What bounds it is how much a CU has in flight: a weight stage asked for one stage ahead leaves a workgroup waiting for most of an
+// HBM round trip, so small tiles hold four stages of weights in registers (100 x 10944 x 3712 17.2 -> 13.8 us on 64 x 32, 32 x 28672 x 4096
+// 20.6 -> 15.9); 128 x 128 tiles have no registers for that and run several workgroups a CU.
 #pragma once
 
 #include "sg_mx_kernel.h"

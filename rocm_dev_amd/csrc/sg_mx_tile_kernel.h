@@ -20,19 +20,36 @@
 namespace sg {
 
 // The matrix instruction as text, accumulators in the accumulation registers: the builtin, which has no form that adds in place
-// for mixed formats, gives every accumulator of the tile two to four homes.  Scale bytes T of ws and XT of xs.  The two idle states
-// are what a vector instruction that wrote an operand would need.  The compiler does not know how long the result takes:
-// mx_drain ends every stage with the idle states of the longest one, and inside a stage an accumulator is touched by these
-// instructions only (tests/test_mx_codegen.py).
-template <int T, int XT>
+// for mixed formats, gives every accumulator of the tile two to four homes.  Scale bytes T of ws and XT of xs.
+//
+// The compiler knows none of its waits.  An operand that a vector instruction wrote has to be two states old: IDLE puts two idle
+// states in front of a stage's first product, and nothing else writes one so late - with them in front of every product a
+// launch of the wide kernel is 3 to 8 % longer (1024 x 10240 x 8192, MXFP4, 58.7 us, 53.8 without).  A result takes up to 19: mx_drain
+// ends every stage with as many, and inside a stage an accumulator is touched by these instructions only.
+// tests/test_mx_codegen.py checks both in the assembly.
+template <bool IDLE, int T, int XT>
 __device__ __forceinline__ void mfma_mx_acc(f32x4& c, const i32x4& w, const i32x4& x, int ws, int xs) {
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
-                 : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(XT & 1), "n"(T >> 1), "n"(XT >> 1));
+    if constexpr (IDLE)
+        asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                     : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(XT & 1), "n"(T >> 1), "n"(XT >> 1));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+                     : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(XT & 1), "n"(T >> 1), "n"(XT >> 1));
 }
-template <int T>
+template <bool IDLE, int T>
 __device__ __forceinline__ void mfma_mx_acc(f32x4& c, const i32x4& w, const i32x8& x, int ws, int xs) {
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,0,0] op_sel_hi:[%6,0,0] cbsz:4"
-                 : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(T >> 1));
+    if constexpr (IDLE)
+        asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,0,0] op_sel_hi:[%6,0,0] cbsz:4"
+                     : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(T >> 1));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,0,0] op_sel_hi:[%6,0,0] cbsz:4"
+                     : "+a"(c) : "v"(w), "v"(x), "v"(ws), "v"(xs), "n"(T & 1), "n"(T >> 1));
+}
+// scale 1 of E4M3 activations, in a register that the compiler cannot write anew in front of a product
+__device__ __forceinline__ int mx_scale_one() {
+    int one = 127;
+    asm volatile("" : "+v"(one));
+    return one;
 }
 template <int NF, int MF>
 __device__ __forceinline__ void mx_drain(f32x4 (&acc)[NF][MF]) {
@@ -136,6 +153,7 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
         for (int i = 0; i < NF; i++) ws_next[i] = *reinterpret_cast<const int*>(wsp[i] + (size_t)qq * kMxQuadBytes);
     };
 
+    const int one = mx_scale_one();
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
@@ -153,13 +171,19 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
             if constexpr (FP4) {
                 const int xs = *reinterpret_cast<const uint16_t*>(buf + BM * 128 + ((wm * MF + j) * 16 + r) * 8 + g * 2);
 #pragma unroll
-                for (int i = 0; i < NF; i++) mfma_mx_acc<0, 0>(acc[i][j], w[b][0][i], lo, ws[i], xs);
+                for (int i = 0; i < NF; i++) {
+                    if (i == 0 && j == 0) mfma_mx_acc<true, 0, 0>(acc[i][j], w[b][0][i], lo, ws[i], xs);
+                    else mfma_mx_acc<false, 0, 0>(acc[i][j], w[b][0][i], lo, ws[i], xs);
+                }
 #pragma unroll
-                for (int i = 0; i < NF; i++) mfma_mx_acc<1, 1>(acc[i][j], w[b][S - 1][i], hi, ws[i], xs);
+                for (int i = 0; i < NF; i++) mfma_mx_acc<false, 1, 1>(acc[i][j], w[b][S - 1][i], hi, ws[i], xs);
             } else {
                 const i32x8 x8 = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                for (int i = 0; i < NF; i++) mfma_mx_acc<0>(acc[i][j], w[b][0][i], x8, ws[i], 127);
+                for (int i = 0; i < NF; i++) {
+                    if (i == 0 && j == 0) mfma_mx_acc<true, 0>(acc[i][j], w[b][0][i], x8, ws[i], one);
+                    else mfma_mx_acc<false, 0>(acc[i][j], w[b][0][i], x8, ws[i], one);
+                }
             }
         }
         mx_drain(acc);

@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(256) mx_wide_kernel(const MxArgs a) {
     const uint8_t* const sx_lds = ring + SX_AT + (wm * MH * 16 + r) * 16;
     const unsigned pick = (unsigned)g | (unsigned)(4 + g) << 8;         // of a row's 8 scales of a stage: one a step
 
+    const int one = mx_scale_one();
     f32x4 acc[RGW][MH];
 #pragma unroll
     for (int i = 0; i < RGW; i++)
@@ -229,10 +230,10 @@ __global__ void __launch_bounds__(256) mx_wide_kernel(const MxArgs a) {
                 __builtin_amdgcn_sched_barrier(0);
                 const int j = e % MH;
                 if constexpr (FP4) {
-                    if (e < MH) mfma_mx_acc<0, 0>(acc[i][j], w[ring_at][0], x4[u][j][0], ws[ring_at], xs[j]);
-                    else mfma_mx_acc<1, 1>(acc[i][j], w[ring_at][S - 1], x4[u][j][1], ws[ring_at], xs[j]);
+                    if constexpr (e < MH) mfma_mx_acc<i == 0 && e == 0, 0, 0>(acc[i][j], w[ring_at][0], x4[u][j][0], ws[ring_at], xs[j]);
+                    else mfma_mx_acc<false, 1, 1>(acc[i][j], w[ring_at][S - 1], x4[u][j][1], ws[ring_at], xs[j]);
                 } else {
-                    mfma_mx_acc<0>(acc[i][j], w[ring_at][0], x8[u][j], ws[ring_at], 127);
+                    mfma_mx_acc<i == 0 && e == 0, 0>(acc[i][j], w[ring_at][0], x8[u][j], ws[ring_at], one);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             });

@@ -62,9 +62,21 @@ def test_no_accumulator_is_touched_while_it_is_being_written(kernels):
 
 
 def test_matrix_instructions_wait_for_vector_instructions_that_wrote_an_operand(kernels):
-    """Two idle states stand in front of every one of them."""
+    """Two wait states lie between a vector instruction and a matrix instruction that reads what it wrote."""
     for name, (code, _) in kernels.items():
-        for before, instruction in zip(code, code[1:]):
+        fresh = {}                               # (file, register) -> wait states since a vector instruction wrote it
+        checked = 0
+        for instruction in code:
+            if instruction.startswith(".LBB"):
+                continue
             if instruction.startswith("v_mfma"):
-                nop = re.match(r"s_nop (\d+)", before)
-                assert nop and int(nop.group(1)) >= 1, (name, instruction)
+                checked += 1
+                reads = {(f, r) for f in "va" for r in _registers(f, instruction.split(None, 1)[1])}
+                early = [k for k in reads if fresh.get(k, 2) < 2]
+                assert not early, (name, instruction, early)
+            nop = re.match(r"s_nop (\d+)", instruction)
+            fresh = {k: s + (int(nop.group(1)) + 1 if nop else 1) for k, s in fresh.items() if s < 2}
+            if instruction.startswith("v_") and not instruction.startswith(("v_mfma", "v_cmp")):
+                written = instruction.split(None, 1)[1].split(",")[0]
+                fresh.update({(f, r): 0 for f in "va" for r in _registers(f, written)})
+        assert checked > 0, name

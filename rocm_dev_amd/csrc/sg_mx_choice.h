@@ -6,8 +6,8 @@
 //     wide builds        a + ceil(w / workgroups a CU holds) * (e + steps * lat)   whole rounds
 //     both               at least bytes / 6.3 TB/s + 2.4;  2.4 more where the scales are copied first;  with a K split
 //                        s0 + KB of partial sums * s1 more
-// The constants are fitted to 53727 measured launches on 1200 random shapes (1..2048 rows, 128..65536 x 256..32768, cold weights,
-// every build and split there is room for); picking the least on those costs 3 to 4 % over the best of them in the geometric mean.
+// The constants are fitted to 49035 measured launches on 1100 random shapes (1..2048 rows, 128..65536 x 256..32768, cold weights,
+// every build and split there is room for); picking the least on those costs 3 to 4.5 % over the best of them in the geometric mean.
 #pragma once
 
 #include "sg_mx.h"
@@ -36,24 +36,24 @@ constexpr MxBuild kDecode[] = {
 };
 // more
 constexpr MxBuild kMore[] = {
-    {1301, 32, 32, 1, 0, {2.58f, 0.241f, 0.140f, 0.10f, 2.39f, 0.000525f}, {2.83f, 0.188f, 0.127f, 0.05f, 2.34f, 0.000482f}},
-    {1304, 32, 32, 4, 0, {2.80f, 0.016f, 0.142f, 0.03f, 2.15f, 0.000742f}, {3.06f, 0.077f, 0.127f, 0.04f, 2.25f, 0.000630f}},
-    {1404, 16, 32, 4, 0, {2.83f, 0.360f, 0.119f, 0.04f, 2.35f, 0.000703f}, {2.91f, 0.106f, 0.104f, 0.00f, 2.39f, 0.000869f}},
-    {1604, 32, 64, 4, 0, {2.82f, 0.849f, 0.236f, 0.54f, 1.64f, 0.000880f}, {2.70f, 0.710f, 0.223f, 0.38f, 1.77f, 0.000865f}},
-    {1702, 64, 16, 2, 0, {3.12f, 0.191f, 0.128f, 0.07f, 2.47f, 0.000369f}, {3.26f, 0.001f, 0.118f, 0.09f, 2.40f, 0.000336f}},
-    {2001, 128, 128, 1, 0, {3.55f, 0.511f, 0.599f, 1.31f, 1.53f, 0.000330f}, {3.34f, 0.475f, 0.460f, 1.37f, 1.18f, 0.000422f}},
-    {2005, 128, 128, 1, 0, {5.33f, 0.753f, 0.625f, 0.68f, 1.26f, 0.000308f}, {5.18f, 0.455f, 0.423f, 0.79f, 0.92f, 0.000375f}},
-    {2010, 128, 64, 1, 0, {3.69f, 0.487f, 0.282f, 0.99f, 1.83f, 0.000404f}, {3.49f, 0.329f, 0.239f, 0.98f, 1.83f, 0.000424f}},
-    {2011, 128, 64, 1, 0, {3.93f, 0.406f, 0.319f, 0.72f, 2.08f, 0.000370f}, {3.55f, 0.278f, 0.269f, 1.09f, 1.93f, 0.000406f}},
-    {2012, 64, 32, 1, 0, {2.70f, 0.241f, 0.135f, 0.18f, 2.38f, 0.000638f}, {2.93f, 0.172f, 0.116f, 0.29f, 2.57f, 0.000507f}},
-    {2013, 64, 64, 1, 0, {3.21f, 0.342f, 0.225f, 0.47f, 2.32f, 0.000468f}, {3.38f, 0.233f, 0.179f, 0.45f, 2.39f, 0.000464f}},
-    {2015, 128, 32, 1, 0, {2.81f, 0.297f, 0.192f, 0.51f, 2.40f, 0.000509f}, {3.07f, 0.206f, 0.188f, 0.70f, 2.38f, 0.000430f}},
-    {3001, 256, 256, 1, 1, {2.76f, 1.210f, 0.000f, 6.51f, 0.00f, 0.000283f}, {4.26f, 0.974f, 0.000f, 4.70f, 0.00f, 0.000334f}},
-    {3002, 192, 128, 1, 1, {2.12f, 0.602f, 0.000f, 4.30f, 0.59f, 0.000353f}, {2.47f, 0.466f, 0.000f, 4.37f, 0.30f, 0.000414f}},
-    {3003, 256, 128, 1, 1, {2.32f, 0.742f, 0.000f, 4.24f, 0.80f, 0.000326f}, {3.05f, 0.536f, 0.000f, 4.46f, 0.33f, 0.000401f}},
-    {3004, 192, 256, 1, 1, {2.85f, 0.945f, 0.000f, 5.97f, 0.00f, 0.000294f}, {2.93f, 0.685f, 0.000f, 6.03f, 0.00f, 0.000337f}},
-    {3006, 128, 128, 1, 1, {4.05f, 0.498f, 0.000f, 0.74f, 1.84f, 0.000365f}, {1.43f, 0.368f, 0.000f, 3.89f, 1.40f, 0.000440f}},
-    {3007, 128, 128, 1, 2, {0.00f, 0.938f, 0.000f, 4.29f, 1.30f, 0.000492f}, {0.00f, 0.598f, 0.000f, 4.72f, 1.06f, 0.000555f}},
+    {1301, 32, 32, 1, 0, {2.68f, 0.242f, 0.141f, 0.10f, 2.28f, 0.000544f}, {2.76f, 0.190f, 0.127f, 0.04f, 2.40f, 0.000485f}},
+    {1304, 32, 32, 4, 0, {2.81f, 0.068f, 0.143f, 0.06f, 1.96f, 0.000934f}, {2.96f, 0.222f, 0.127f, 0.03f, 2.30f, 0.000617f}},
+    {1404, 16, 32, 4, 0, {2.77f, 0.383f, 0.121f, 0.06f, 2.24f, 0.000949f}, {2.88f, 0.300f, 0.104f, 0.00f, 2.40f, 0.000781f}},
+    {1604, 32, 64, 4, 0, {2.80f, 0.000f, 0.236f, 0.52f, 1.75f, 0.000899f}, {2.88f, 0.620f, 0.210f, 0.33f, 1.87f, 0.000775f}},
+    {1702, 64, 16, 2, 0, {3.19f, 0.001f, 0.128f, 0.09f, 2.33f, 0.000371f}, {3.25f, 0.215f, 0.119f, 0.07f, 2.39f, 0.000374f}},
+    {2001, 128, 128, 1, 0, {3.62f, 0.598f, 0.595f, 1.21f, 1.38f, 0.000360f}, {2.45f, 0.112f, 0.448f, 2.13f, 1.21f, 0.000451f}},
+    {2005, 128, 128, 1, 0, {5.27f, 0.721f, 0.623f, 0.66f, 1.17f, 0.000329f}, {4.26f, 0.439f, 0.419f, 1.38f, 0.95f, 0.000397f}},
+    {2010, 128, 64, 1, 0, {3.53f, 0.487f, 0.288f, 0.98f, 1.75f, 0.000434f}, {3.27f, 0.329f, 0.244f, 1.03f, 1.79f, 0.000455f}},
+    {2011, 128, 64, 1, 0, {4.02f, 0.393f, 0.316f, 0.62f, 1.84f, 0.000424f}, {3.33f, 0.154f, 0.263f, 1.22f, 1.82f, 0.000452f}},
+    {2012, 64, 32, 1, 0, {2.77f, 0.239f, 0.136f, 0.18f, 2.23f, 0.000654f}, {2.89f, 0.172f, 0.112f, 0.26f, 2.49f, 0.000604f}},
+    {2013, 64, 64, 1, 0, {3.25f, 0.333f, 0.223f, 0.44f, 2.21f, 0.000483f}, {3.38f, 0.223f, 0.186f, 0.38f, 2.35f, 0.000467f}},
+    {2015, 128, 32, 1, 0, {2.86f, 0.299f, 0.196f, 0.50f, 2.32f, 0.000525f}, {3.05f, 0.206f, 0.185f, 0.64f, 2.34f, 0.000476f}},
+    {3001, 256, 256, 1, 1, {3.53f, 1.192f, 0.000f, 5.54f, 0.00f, 0.000302f}, {2.90f, 0.893f, 0.000f, 5.94f, 0.00f, 0.000334f}},
+    {3002, 192, 128, 1, 1, {1.99f, 0.598f, 0.000f, 4.30f, 0.58f, 0.000393f}, {1.71f, 0.416f, 0.000f, 4.91f, 0.35f, 0.000463f}},
+    {3003, 256, 128, 1, 1, {2.40f, 0.713f, 0.000f, 4.20f, 0.64f, 0.000369f}, {1.60f, 0.483f, 0.000f, 5.68f, 0.41f, 0.000426f}},
+    {3004, 192, 256, 1, 1, {3.03f, 0.923f, 0.000f, 5.57f, 0.00f, 0.000313f}, {2.80f, 0.620f, 0.000f, 5.98f, 0.00f, 0.000351f}},
+    {3006, 128, 128, 1, 1, {4.03f, 0.497f, 0.000f, 0.84f, 1.67f, 0.000406f}, {1.10f, 0.332f, 0.000f, 3.99f, 1.46f, 0.000475f}},
+    {3007, 128, 128, 1, 2, {0.00f, 0.930f, 0.000f, 4.31f, 1.21f, 0.000524f}, {0.00f, 0.554f, 0.000f, 4.71f, 1.10f, 0.000580f}},
 };
 // build + 10000 * splits (splits > 1).  workspace: the launch may use the stream's (a K split, copied scales); copy: the wide
 // kernel would need the scales copied.

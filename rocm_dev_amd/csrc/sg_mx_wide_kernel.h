@@ -16,7 +16,7 @@
 // multiple of 512 (or their address none of 16) a small launch copies them so first.
 //
 // 1024 x 57344 x 8192: E4M3 activations 366 us = 2.6 PFLOP/s on 192 x 256 tiles, 65 % of the instruction's rate and level with the E4M3
-// kernel of this shape; MXFP4 272-290 us = 3.4 PFLOP/s, 40 % of its rate: a stage of 1536 clocks of products takes 3500,
+// kernel of this shape; MXFP4 272-285 us = 3.4 PFLOP/s, 40 % of its rate: a stage of 1536 clocks of products takes 3500,
 // half of them waiting for operands (profiles/mxfp4_gemm_counters.md).  Tried there and not kept: stages of 64 bytes a row on rings of
 // four and five slots (300 us on 256 x 256, the others 8 to 17 % behind), lines asked for three stages ahead (286 to 314), weights
 // straight to registers on eight waves (366), two workgroups a CU (325).

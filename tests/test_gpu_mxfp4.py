@@ -346,6 +346,47 @@ def test_activation_scales_at_any_address(offset):
     ref.check(bits(D), want, slack)
 
 
+def test_threads_on_one_stream():
+    """Calls of several launches from threads that share a stream, and its workspace: each gets its own sums."""
+    import threading
+    shapes = [("fp8act", 8, 256, 16384), ("mx", 200, 512, 8192 + 32), ("mx", 64, 700, 9216), ("fp8act", 40, 384, 12288)]
+    jobs = []
+    for i, (kind, m, n, k) in enumerate(shapes):
+        assert lib.sg_debug_mxfp4_choice(kind == "mx", m, n, k, 1) > 10000          # K is split
+        rng = np.random.default_rng(i)
+        P = packed(*some_mx(rng, n, k))
+        D = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+        if kind == "mx":
+            A, SA = (dev(t) for t in some_mx(rng, m, k))
+            run = lambda D, A=A, SA=SA, P=P: sg.mxfp4_gemm(A, SA, P, D, check=True)  # noqa: E731
+        else:
+            A = dev(some_e4m3(rng, m, k))
+            run = lambda D, A=A, P=P: sg.mxfp4_gemm_fp8act(A, P, D, check=True)  # noqa: E731
+        run(D)
+        jobs.append((run, D, [torch.zeros_like(D) for _ in range(12)]))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(run, outs):
+        try:
+            for out in outs:
+                run(out)
+        except Exception as e:       # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(run, outs)) for run, _, outs in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for _, D, outs in jobs:
+        assert D.any()
+        for out in outs:
+            assert torch.equal(out.view(torch.int16), D.view(torch.int16))
+
+
 # ---- entry points -------------------------------------------------------------------------------------------
 
 def _operands():

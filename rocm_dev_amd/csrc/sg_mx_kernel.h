@@ -217,6 +217,17 @@ __global__ void __launch_bounds__(512) mx_gemm_kernel(const MxArgs a) {
         if (left > 2) multiply(T2{});
         if (left > 3) multiply(T3{});
     }
+    // A product's result may be read 12 wait states behind it.  Across the branches below the compiler counted one too few on two builds
+    // (E4M3 activations, 32 x 16 and 16 x 32), so that the idle states stand here; the ties keep products in front of them and uses behind.
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) asm volatile("" : "+v"(acc[i][j]));
+    asm volatile("s_nop 11" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) asm volatile("" : "+v"(acc[i][j]));
 
     // ---- the waves' sums, in wave order ----
     const float scale = a.scale ? a.scale[0] : 1.0f;

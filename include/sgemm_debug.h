@@ -90,6 +90,9 @@ int sg_debug_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t
  * the K splits where there are any; workspace = 0: under capture.  0 for a shape that they refuse. */
 int sg_debug_mxfp4_choice(int fp4_activations, int m, int n, int k, int workspace);
 
+/* How many products of the calling thread had to search for their build: it keeps the answers of its last 16 shapes. */
+int sg_debug_mxfp4_searches(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,7 @@ SIGNATURES = {
     "sg_debug_wide_choice": (_i, [_i, _i, _i, _i, _i, C.POINTER(_i * 3)]),
     "sg_debug_read_stream": (_i, [_vp, _i, _i, _i, _i, _vp]),
     "sg_debug_mxfp4_choice": (_i, [_i] * 5),
+    "sg_debug_mxfp4_searches": (_i, []),
     "sg_debug_mxfp4_gemm": (_i, [_vp] * 6 + [_i] * 4 + [_vp]),
     "sg_debug_cu_ingest": (_i, [_vp, _sz, _vp, _sz, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     "sg_skinny_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),

@@ -59,6 +59,7 @@ int launch_mx_pack(const uint8_t* B, const uint8_t* SB, uint8_t* P, int n, int k
 int launch_mx_scale_rows(const uint8_t* SA, uint8_t* out, int m, int k, int quads, hipStream_t stream);
 // fp4: activations in MXFP4, otherwise E4M3; build: 0 = the library's choice (sg_mx_gemm.hip)
 int mx_choice(bool fp4, int m, int n, int k, int cu_count, bool workspace);
+int mx_searches();
 int launch_mx_gemm(bool fp4, int build, MxArgs& a, int cu_count, hipStream_t stream);
 
 }  // namespace sg

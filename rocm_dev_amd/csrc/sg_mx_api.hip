@@ -83,4 +83,6 @@ int sg_debug_mxfp4_choice(int fp4_activations, int m, int n, int k, int workspac
     return mx_choice(fp4_activations != 0, m, n, k, 256, workspace != 0);
 }
 
+int sg_debug_mxfp4_searches(void) { return mx_searches(); }
+
 }  // extern "C"

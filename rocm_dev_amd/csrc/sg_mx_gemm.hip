@@ -82,18 +82,26 @@ static int launch_build(int build, MxArgs& a, hipStream_t stream) {
     }
 }
 
-// The build that a call without one runs.  The search takes about a microsecond of host time, so a thread keeps the last few
-// shapes' answers: a function of the shape, of nothing else.
+// The build that a call without one runs.  The search takes 0.2 to 0.9 us of host time, so a thread keeps the answers of its last
+// 16 shapes - a function of the shape, of nothing else - and looks through all of them, a few ns: the shapes of a layer's projections are
+// too much alike (multiples of powers of two) for a place by their value to keep them apart.
+static thread_local int t_searches = 0;
+int mx_searches() { return t_searches; }
+
 static int pick_mx(bool fp4, const MxArgs& a, int cu_count, bool workspace) {
     struct Kept {
         int m, n, k, flags, build;
     };
-    static thread_local Kept kept[16];
+    constexpr unsigned kKept = 16;
+    static thread_local Kept kept[kKept];
+    static thread_local unsigned oldest = 0;
     const bool copy = fp4 && !scales_lie_right(a);
-    const int flags = 1 | (fp4 ? 2 : 0) | (copy ? 4 : 0) | (workspace ? 8 : 0) | cu_count << 4;
-    Kept& e = kept[((unsigned)a.m * 31u + (unsigned)a.n * 17u + (unsigned)a.k / 32u + (unsigned)flags) % 16];
-    if (e.m != a.m || e.n != a.n || e.k != a.k || e.flags != flags)
-        e = Kept{a.m, a.n, a.k, flags, mx_choose(fp4, a.m, a.n, a.k, cu_count, workspace, copy)};
+    const int flags = 1 | (fp4 ? 2 : 0) | (copy ? 4 : 0) | (workspace ? 8 : 0) | cu_count << 4;      // (0: a place not yet taken)
+    for (const Kept& e : kept)
+        if (e.m == a.m && e.n == a.n && e.k == a.k && e.flags == flags) return e.build;
+    t_searches++;
+    Kept& e = kept[oldest++ % kKept];
+    e = Kept{a.m, a.n, a.k, flags, mx_choose(fp4, a.m, a.n, a.k, cu_count, workspace, copy)};
     return e.build;
 }
 

@@ -1,4 +1,6 @@
 """What the MXFP4 products launch, without a GPU: on the stand-in for the HIP runtime (launch_recorder.py)."""
+import re
+
 import pytest
 
 import launch_recorder
@@ -58,3 +60,55 @@ def builds_again(r, shapes):
 def test_a_kept_answer_is_the_shapes_own(fake):
     shapes = [(kind, m, n, k) for kind in ("mx", "fp8act") for m in (1, 33, 600) for n, k in LAYER_8B + LAYER_70B]
     assert launch_recorder.scenario(fake, "test_mx_launches", "builds_again", shapes) == [True, True, True]
+
+
+# ---- calls that get no workspace ----
+
+def kernels(launches):
+    return [re.search(r"sg::(mx_\w+)", name).group(1) for name, *_ in launches]
+
+
+def without_memory(r, shapes):
+    """[(shape, rc and launches with a workspace, with none to be had, under capture, allocations of the last two)]"""
+    out = []
+    for s in shapes:
+        with_memory = product(r, *s)
+        r.call("sg_release_workspaces")
+        before = r.fake.rec_allocations()
+        r.fake.rec_largest_allocation(1 << 16)
+        refused = product(r, *s)
+        r.fake.rec_largest_allocation(-1)
+        r.fake.rec_capturing(1)
+        recorded = product(r, *s)
+        r.fake.rec_capturing(0)
+        out.append([s, with_memory, refused, recorded, r.fake.rec_allocations() - before])
+    return out
+
+
+def test_a_call_without_device_memory_launches_what_a_recorded_one_does(fake):
+    split = [("fp8act", 8, 256, 16384), ("mx", 8, 256, 16384), ("mx", 128, 8192, 28672), ("mx", 200, 512, 8192 + 32)]
+    copied = [("mx", 1024, 4096, 5440), ("mx", 2048, 8192, 10944)]
+    for s, (rc, launches), refused, recorded, allocations in launch_recorder.scenario(fake, "test_mx_launches", "without_memory", split + copied):
+        names = kernels(launches)
+        assert rc == 0 and (names[-1] == "mx_sum_kernel" if tuple(s) in split else names[0] == "mx_scale_rows_kernel"), s
+        for code, alone in (refused, recorded):
+            assert code == 0 and len(alone) == 1 and kernels(alone)[0] in ("mx_gemm_kernel", "mx_tile_kernel"), s
+        assert refused == recorded and allocations == 0, s
+
+
+def over_the_limit(r, shapes):
+    out = []
+    for s in shapes:
+        before = r.fake.rec_allocations()
+        rc, launches = product(r, *s)
+        out.append([r.lib.sg_debug_mxfp4_choice(1, *s[1:], 1), rc, launches, r.fake.rec_allocations() - before,
+                    r.lib.sg_debug_mxfp4_choice(1, *s[1:], 0)])
+    return out
+
+
+def test_scales_too_large_for_a_workspace_are_not_copied(fake):
+    """More than 512 MB of copied scales: the build without a workspace, by size alone."""
+    for wanted, rc, launches, allocations, alone in launch_recorder.scenario(
+            fake, "test_mx_launches", "over_the_limit", [("mx", 1 << 20, 4096, 16416), ("mx", 140000, 512, 131104)]):
+        assert 3000 <= wanted % 10000 and alone < 3000
+        assert rc == 0 and allocations == 0 and kernels(launches) == ["mx_tile_kernel"]

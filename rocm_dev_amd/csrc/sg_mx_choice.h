@@ -75,7 +75,10 @@ inline int mx_choose(bool fp4, int m, int n, int k, int cu_count, bool workspace
         for (int splits : kSplits) {
             if (splits > quads || (splits > 1 && !workspace)) break;
             const float grid = groups * splits;
-            if (splits > 1 && (grid > (c.wide ? 520 : 1100) * (cu_count / 256.f) || frags * splits > 262144.f || quads / splits < c.waves / 2)) break;
+            // Builds most of whose waves have no columns were not fitted.  While a CU has two workgroups such waves cost nothing (14 x 170 x 1280
+            // 3.2 us on eight, 3.7 on one); beyond, they take others' places (557 x 10536 x 32 15.8 on four, 8.5 without).
+            if (quads / splits < c.waves / 2 && (splits > 1 || grid > 2 * cu_count)) break;
+            if (splits > 1 && (grid > (c.wide ? 520 : 1100) * (cu_count / 256.f) || frags * splits > 262144.f)) break;
             const int part = (quads + splits - 1) / splits * 4, s = part < steps ? part : steps;
             float us, w = grid / cu_count;
             if (c.wide) {

@@ -1,0 +1,28 @@
+"""The builds that MXFP4 products choose (csrc/sg_mx_choice.h), without a GPU."""
+import numpy as np
+import pytest
+
+from rocm_dev_amd._lib import lib
+
+# streaming builds: weight rows and activation rows of a workgroup's tile
+TILE = {11: (16, 16), 12: (32, 16), 13: (32, 32), 14: (16, 32), 16: (32, 64), 17: (64, 16)}
+
+
+def shapes(seed, count):
+    rng = np.random.default_rng(seed)
+    for _ in range(count):
+        yield int(2049 ** rng.random()), int(128 * 512 ** rng.random()), 32 * int(64 ** rng.random())
+
+
+@pytest.mark.parametrize("fp4", [0, 1])
+@pytest.mark.parametrize("workspace", [0, 1])
+def test_waves_without_columns_take_nobodys_place(fp4, workspace):
+    """Workgroups of several waves on fewer groups of 512 columns than half their waves: on two a CU at most."""
+    fixed = [(557, 10536, 32), (148, 46039, 96), (402, 33758, 96), (2, 48669, 32), (1, 128256, 96)]
+    for m, n, k in fixed + list(shapes(0, 2000)):
+        splits, build = divmod(lib.sg_debug_mxfp4_choice(fp4, m, n, k, workspace), 10000)
+        if build >= 2000:
+            continue
+        (bn, bm), waves = TILE[build // 100], build % 100
+        groups, quads = -(-n // bn) * -(-m // bm), -(-k // 512)
+        assert quads // max(1, splits) >= waves // 2 or splits == 0 and groups <= 512, (m, n, k, build, splits)

@@ -1,4 +1,6 @@
 """The builds that MXFP4 products choose (csrc/sg_mx_choice.h), without a GPU."""
+import os
+
 import numpy as np
 import pytest
 
@@ -26,3 +28,23 @@ def test_waves_without_columns_take_nobodys_place(fp4, workspace):
         (bn, bm), waves = TILE[build // 100], build % 100
         groups, quads = -(-n // bn) * -(-m // bm), -(-k // 512)
         assert quads // max(1, splits) >= waves // 2 or splits == 0 and groups <= 512, (m, n, k, build, splits)
+
+
+SAMPLES = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "mxfp4_choice_samples.csv")
+
+
+@pytest.mark.parametrize("rows,count,mean", [((1, 16), 480, 1.035), ((17, 2048), 550, 1.05)])
+def test_chosen_builds_are_near_the_best_of_the_samples(rows, count, mean):
+    """On the launches that the choice is fitted to, as the files under profiles/ state it."""
+    over = []
+    with open(SAMPLES) as f:
+        next(f)
+        for line in f:
+            activations, m, n, k, launches = line.split(",")
+            if rows[0] <= int(m) <= rows[1]:
+                us = {int(b): float(t) for b, t in (x.split(":") for x in launches.split())}
+                build = lib.sg_debug_mxfp4_choice(int(activations == "mxfp4"), int(m), int(n), int(k), 1)
+                if build in us:
+                    over.append(us[build] / min(us.values()))
+    assert len(over) >= count
+    assert np.exp(np.mean(np.log(over))) < mean and max(over) < 1.75

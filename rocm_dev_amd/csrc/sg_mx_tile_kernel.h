@@ -224,8 +224,9 @@ __global__ void __launch_bounds__(64 * WN * WM) mx_tile_kernel(const MxArgs a) {
     };
     constexpr std::false_type MORE{};
     constexpr std::true_type LAST{};
+    constexpr int REACH = WR - 1 > 1 + XR ? WR - 1 : 1 + XR;      // the farthest stage that a stage's loads are of
     int s = first;                                       // a multiple of U: even
-    for (; s + 3 + WR - 1 < stages; s += 4) {            // every load is of a stage there is
+    for (; s + 3 + REACH < stages; s += 4) {             // every load is of a stage there is
         stage(s, I0{}, MORE);
         stage(s + 1, I1{}, MORE);
         stage(s + 2, std::integral_constant<int, 2>{}, MORE);

@@ -1,5 +1,5 @@
 """E4M3 x MXFP4 products whose operands no matrix instruction cuts off (mx_uncut.py): as exact as MXFP4 x MXFP4 ones, and to the bit
-where every partial sum fits fp32."""
+where every partial sum fits fp32.  Other operands, against the same sums of products that are cut off as the instruction does."""
 import numpy as np
 import pytest
 import torch
@@ -58,3 +58,20 @@ def test_sums_of_fp32(m, n, k):
     want, slack = mx_uncut.gemm(a, b)
     ref.check(bits(D[:m]), want * factor, slack * factor)
     assert (D[m] == -7).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 33, 512), (8, 40, 4096), (33, 70, 1120), (130, 65, 2080), (260, 40, 1376)])
+def test_sums_of_cut_products(m, n, k):
+    """Operands of all sizes: the products are cut off as the model says, and nothing else is lost."""
+    rng = np.random.default_rng(m + n + k)
+    A = rng.integers(0, 256, (m, k), dtype=np.uint8)
+    A = np.where((A & 127) == 127, 0x38, A).astype(np.uint8)
+    B, SB = rng.integers(0, 256, (n, k // 2), dtype=np.uint8), rng.integers(121, 134, (n, k // 32), dtype=np.uint8)
+    P = torch.empty((sg.mxfp4_packed_bytes(n, k),), dtype=torch.uint8, device="cuda")
+    sg.mxfp4_pack(dev(B), dev(SB), P, check=True)
+    want, (_, slack) = mx_uncut.cut_sums(A, B, SB), mx_uncut.gemm(ref.e4m3(A), ref.values(B, SB))
+    a = dev(A)
+    for build in BUILDS:
+        D = torch.full((m, n), -7.0, dtype=torch.bfloat16, device="cuda")
+        assert lib.sg_debug_mxfp4_gemm(a.data_ptr(), 0, P.data_ptr(), D.data_ptr(), 0, 0, m, n, k, build, torch.cuda.current_stream().cuda_stream) == 0
+        ref.check(bits(D), want, slack)

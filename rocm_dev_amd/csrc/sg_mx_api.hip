@@ -7,8 +7,8 @@ using namespace sg;
 namespace {
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-int gemm(bool fp4, int build, const uint8_t* A, const uint8_t* SA, const uint8_t* P, void* D, const float* scale, const float* row_scales, int m, int n,
-         int k, void* stream) {
+int gemm(bool fp4, int build, const uint8_t* A, const uint8_t* SA, const uint8_t* P, void* D, const float* scale,
+         const float* row_scales, int m, int n, int k, void* stream) {
     if (!A || (fp4 && !SA) || !P || !D || m <= 0 || n <= 0 || k <= 0) return SG_BAD_ARGUMENT;
     if (k % kMxBlock) return SG_K_NOT_DIVISIBLE_BY_WARPTILE_K;
     if (off16(A) || off16(P) || (reinterpret_cast<uintptr_t>(D) & 7u)) return SG_BAD_ALIGNMENT;

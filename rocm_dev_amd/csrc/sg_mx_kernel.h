@@ -7,14 +7,14 @@
 // products are issued, so a wave keeps four steps in flight.  The waves of a workgroup share K by groups of four steps and
 // meet in LDS, partial sums added in wave order: the result does not depend on which wave is first.
 //
-// Measured, cold weights: 1 x 28672 x 4096 (MXFP4 activations) 11.2 us a launch among others = 5.6 TB/s, 1 x 4096 x 14336 7.7, 8 x 28672 x 4096
-// (E4M3) 12.5: what is above 2.2 us + bytes / 6.85 TB/s, a kernel that only reads, is the activations' way through the CUs' L1,
+// Measured, cold weights: 1 x 28672 x 4096 (MXFP4 activations) 12.2 us a call among others = 5.1 TB/s, 1 x 4096 x 14336 7.1, 8 x 28672 x 4096
+// (E4M3) 13.1: what is above 2.2 us + bytes / 6.85 TB/s, a kernel that only reads, is the activations' way through the CUs' L1,
 // as many bytes as the weights at 8 rows and one 16-row tile a wave.  Four tiles a wave (64 x 16) quarter that and win where there
-// are enough of them; eight waves of one tile win where a CU has one tile (8 x 4096 x 14336 9.1 against 15.4).
+// are enough of them; eight waves of one tile win where a CU has one tile (8 x 4096 x 14336 9.1 against 14.8).
 //
 // The instruction multiplies every block of 32 products by both operands' scales exactly and adds in 32 bits; E4M3
-// activations take the scale 1.  Inside a run of 8 E4M3 products it cuts products off about 14 binades below the largest
-// (as it does for E4M3 weights).
+// activations take the scale 1.  Inside an aligned run of 8 E4M3 products it cuts products off, towards zero, 13 binades below their
+// largest exponent sum (as it does for E4M3 weights): fewer than fp32's bits, and what no use of the instruction avoids.
 #pragma once
 
 #include "sg_mx.h"

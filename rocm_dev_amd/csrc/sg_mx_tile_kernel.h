@@ -2,17 +2,18 @@
 //
 // A workgroup of WN x WM waves owns 16 * NF * WN weight rows by 16 * MF * WM activation rows, a wave NF x MF fragments of
 // 16 x 16.  A stage is 128 bytes of every activation row: 128 columns of E4M3 (one step of the matrix instruction) or 256 of
-// MXFP4 (two).  The activations of a stage, which all waves along n read, go through LDS, two buffers, one barrier a stage (and through registers, so that the compiler's own waits order everything); the
-// weights, which only the WM waves along m share, go straight to registers by contiguous KBs of the packed buffer (sg_mx.h):
-// through LDS they would be a quarter (E4M3) to a half (MXFP4) of its traffic.
+// MXFP4 (two).  The activations of a stage, which all waves along n read, go through LDS, two buffers, one barrier a stage (and
+// through registers, so that the compiler's own waits order everything); the weights, which only the WM waves along m share, go
+// straight to registers by contiguous KBs of the packed buffer (sg_mx.h): through LDS they would be a quarter (E4M3) to a half
+// (MXFP4) of its traffic.
 //
 // LDS: row x 128 bytes, the 16-byte piece p of row x at p ^ ((x / 2) % 8), so that the 16 rows of a fragment's read meet all
 // banks; lane (r, g) reads pieces g and g + 4 - of E4M3 the 32 columns the instruction wants of it, of MXFP4 block g of
 // each of the stage's two steps.  MXFP4's block scales lie beside, 8 bytes a row in the order a lane reads them: 2 bytes, one a step.
 //
 // What bounds it is how much a CU has in flight: a weight stage asked for one stage ahead leaves a workgroup waiting for most of an
-// HBM round trip, so small tiles hold four stages of weights in registers (100 x 10944 x 3712 17.2 -> 13.8 us on 64 x 32, 32 x 28672 x 4096
-// 20.6 -> 15.9); 128 x 128 tiles have no registers for that and run several workgroups a CU.
+// HBM round trip, so small tiles hold four stages of weights in registers (E4M3 activations on 64 x 32: 100 x 10944 x 3712 16.9 -> 14.0 us,
+// 32 x 28672 x 4096 20.6 -> 15.6); 128 x 128 tiles have no registers for that and run several workgroups a CU.
 #pragma once
 
 #include "sg_mx_kernel.h"

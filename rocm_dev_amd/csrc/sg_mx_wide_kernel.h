@@ -15,11 +15,11 @@
 // bytes at a 16-byte address, so the scales of MXFP4 activations have to lie on rows of whole groups: where k is no
 // multiple of 512 (or their address none of 16) a small launch copies them so first.
 //
-// 1024 x 57344 x 8192: E4M3 activations 366 us = 2.6 PFLOP/s on 192 x 256 tiles, 65 % of the instruction's rate and level with the E4M3
-// kernel of this shape; MXFP4 272-285 us = 3.4 PFLOP/s, 40 % of its rate: a stage of 1536 clocks of products takes 3500,
-// half of them waiting for operands (profiles/mxfp4_gemm_counters.md).  Tried there and not kept: stages of 64 bytes a row on rings of
-// four and five slots (300 us on 256 x 256, the others 8 to 17 % behind), lines asked for three stages ahead (286 to 314), weights
-// straight to registers on eight waves (366), two workgroups a CU (325).
+// 1024 x 57344 x 8192: E4M3 activations 360 us = 2.7 PFLOP/s, 63 % of the instruction's rate and level with the E4M3 kernel of this shape;
+// MXFP4 268 us on 192 x 256 tiles = 3.6 PFLOP/s, 44 % of its rate: a stage of 1536 clocks of products takes 3500, a quarter of them
+// in waits and at barriers, a fifth before an instruction may issue (profiles/mxfp4_gemm_counters.md).  Tried there, against 272 to 285
+// at the time, and not kept: stages of 64 bytes a row on rings of four and five slots (300 us on 256 x 256, the others 8 to 17 % behind),
+// lines asked for three stages ahead (286 to 314), weights straight to registers on eight waves (366), two workgroups a CU (325).
 #pragma once
 
 #include <utility>
@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(256) mx_wide_kernel(const MxArgs a) {
     const unsigned lane16 = lane * 16;
     auto issue_w = [&](int i, int s, int slot, int on) __attribute__((always_inline)) {
         const int e = 4 * i + wave, t = tile0 + e / S < a.tiles ? tile0 + e / S : a.tiles - 1;
-        dma_1kb_if<true>(a.P + ((size_t)t * a.pitch + (S * (first + s) + e % S)) * kMxStepBytes, lane16, lds0 + (unsigned)slot * W_BYTES + e * 1024, on);
+        dma_1kb_if<true>(a.P + ((size_t)t * a.pitch + (S * (first + s) + e % S)) * kMxStepBytes, lane16,
+                         lds0 + (unsigned)slot * W_BYTES + e * 1024, on);
     };
     // Scales of a group: four tiles an instruction (beyond 2 * RGW tiles a copy that nobody reads), 64 activation rows an
     // instruction (a tile of 128 rows: fetched twice, the same bytes to the same place)

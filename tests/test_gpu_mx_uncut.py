@@ -32,8 +32,8 @@ def operands(rng, m, n, k, whole):
     return dev(A), P, ref.e4m3(A), ref.values(B, SB)
 
 
-@pytest.mark.parametrize("m,n,k,splits", [(1, 1, 32, (1,)), (3, 33, 512, (1,)), (16, 40, 4096, (1, 2, 5, 8)), (33, 70, 1120, (1, 3)), (130, 130, 2080, (1, 2, 5)),
-                                          (300, 515, 2400, (1, 2)), (129, 257, 3584, (1, 7))])
+@pytest.mark.parametrize("m,n,k,splits", [(1, 1, 32, (1,)), (3, 33, 512, (1,)), (16, 40, 4096, (1, 2, 5, 8)), (33, 70, 1120, (1, 3)),
+                                          (130, 130, 2080, (1, 2, 5)), (300, 515, 2400, (1, 2)), (129, 257, 3584, (1, 7))])
 def test_whole_sums_to_the_bit_on_every_build(m, n, k, splits):
     A, P, a, b = operands(np.random.default_rng(m + k), m, n, k, True)
     want = mx_uncut.bf16_bits(a @ b.T + 0.0)
@@ -73,5 +73,6 @@ def test_sums_of_cut_products(m, n, k):
     a = dev(A)
     for build in BUILDS:
         D = torch.full((m, n), -7.0, dtype=torch.bfloat16, device="cuda")
-        assert lib.sg_debug_mxfp4_gemm(a.data_ptr(), 0, P.data_ptr(), D.data_ptr(), 0, 0, m, n, k, build, torch.cuda.current_stream().cuda_stream) == 0
+        assert lib.sg_debug_mxfp4_gemm(a.data_ptr(), 0, P.data_ptr(), D.data_ptr(), 0, 0, m, n, k, build,
+                                       torch.cuda.current_stream().cuda_stream) == 0
         ref.check(bits(D), want, slack)

@@ -45,7 +45,8 @@ class Instruction:
         self.matrix = self.op.startswith("v_mfma")
         self.vector = self.op.startswith("v_") and not self.matrix
         loads = "load" in self.op and "lds" not in self.op or self.op.startswith("ds_read")
-        written = _registers(first) if self.matrix or loads or self.vector and not self.op.startswith(("v_cmp", "v_readlane", "v_readfirstlane")) else frozenset()
+        writes = self.matrix or loads or self.vector and not self.op.startswith(("v_cmp", "v_readlane", "v_readfirstlane"))
+        written = _registers(first) if writes else frozenset()
         self.writes, self.reads = written, _registers(rest if written else self.operands)
         if self.op.startswith("v_swap"):
             self.writes = self.reads = _registers(self.operands)

@@ -33,7 +33,7 @@ def test_waves_without_columns_take_nobodys_place(fp4, workspace):
 SAMPLES = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "mxfp4_choice_samples.csv")
 
 
-@pytest.mark.parametrize("rows,count,mean", [((1, 16), 480, 1.035), ((17, 2048), 550, 1.05)])
+@pytest.mark.parametrize("rows,count,mean", [((1, 16), 480, 1.035), ((17, 2048), 530, 1.05)])
 def test_chosen_builds_are_near_the_best_of_the_samples(rows, count, mean):
     """On the launches that the choice is fitted to, as the files under profiles/ state it."""
     over = []

@@ -7,8 +7,9 @@
 //     both               at least bytes / 6.3 TB/s + 2.4;  2.4 more where the scales are copied first;  with a K split
 //                        s0 + KB of partial sums * s1 more
 // The constants are fitted to 49035 measured launches on 1100 random shapes (1..2048 rows, 128..65536 x 256..32768, cold weights, every
-// build and split there is room for; nearly all of them in profiles/mxfp4_choice_samples.csv): the choice costs 3.3 % (to 16 rows) and 4.6 % over the best of
-// them in the geometric mean, as much on shapes left out of the fit.  They interpolate and describe no kernel: some came out at 0.
+// build and split there is room for; nearly all of them in profiles/mxfp4_choice_samples.csv): the choice costs 3.3 % (to 16 rows) and
+// 4.6 % over the best of them in the geometric mean, as much on shapes left out of the fit.  They interpolate and describe no kernel:
+// some came out at 0.
 #pragma once
 
 #include "sg_mx.h"

@@ -385,6 +385,60 @@ int sg_mxfp4_gemm(const uint8_t* A, const uint8_t* A_scales, const uint8_t* P, v
 int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const float* scale_tensor, const float* row_scales,
                          int m, int n, int k, void* stream);
 
+/* Root-mean-square norm of bf16 rows into E4M3 with a scale a row: what stands between two projections of a decoder layer whose
+ * activations are E4M3 (sg_skinny_gemm_rowcol, sg_mxfp4_gemm_fp8act), the residual's addition before it.  No counterpart in
+ * the reference.
+ *     v = X, or bf16(X + residual);   y = v * weight / sqrt(mean over the row of v^2 + eps)   (fp32)
+ *     scales[r] = absmax(y[r,:]) / 448 (1 if that is zero; NaNs do not count);   Q = e4m3_rne_sat(y / scales[r]), a NaN 0x7f
+ * and, each if its pointer is not NULL, sum = v (the next residual) and Y = bf16(y) (a router's input).  residual and weight
+ * ([cols]) may be NULL: nothing added, factors of 1.  sum may be X's or the residual's own memory; Q and Y overlap no input.
+ * A row whose squares' sum is no finite fp32 has y = 0, or NaN where v is not finite.  cols must be a multiple of 16, all
+ * matrices and weight 16-byte aligned, scales 4-byte, eps finite and not negative. */
+int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const void* weight_bf16, void* sum_bf16, void* Y_bf16,
+                        uint8_t* Q, float* scales, float eps, int rows, int cols, void* stream);
+
+/* Weights B [n][k] in 4-bit integers with a scale, and on request a zero, for each group of 32, 64 or 128 neighbouring columns of
+ * a row, times bf16 activations.  No counterpart in the reference.
+ *     D[i][j] = bf16( sum_k A[i][k] * (B[j][k] - zeros[j][g]) * scales[j][g] ),  g = k / group
+ * Codes are 0..15, two a byte, the even column in the low nibble ([n][k / 2], row stride b_stride bytes); scales [n][k / group] are
+ * bf16, or fp16 with SG_INT4_F16_SCALES; zeros [n][k / group] are bytes, used as they are, with SG_INT4_ZEROS, and 8 without.  k must be a
+ * multiple of group.  sg_int4_pack lays the weights out as the matrix instruction takes them: once, when a program loads them, into
+ * sg_int4_packed_bytes(n, k, group, flags) bytes (0 for what sg_int4_pack refuses), all of which are written.  sg_int4_gemm takes
+ * that P with the same n, k, group and flags.  Any m >= 1; it is made for few rows, and beyond 64 reads the weights again for every 64.
+ * Sums are fp32, in an order fixed by the shape: results are bit-reproducible.  Within a group the sum of A * (1 + B / 16) is corrected by the sum of A,
+ * so a row of A with an infinity or a NaN has NaN outputs.
+ * B, A and P 16-byte aligned (A's rows are k values apart), b_stride a multiple of 16 and at least k / 2, D 8-byte, scales 2-byte aligned. */
+#define SG_INT4_ZEROS 1
+#define SG_INT4_F16_SCALES 2
+size_t sg_int4_packed_bytes(int n, int k, int group, int flags);
+int    sg_int4_pack(const uint8_t* B, const void* scales, const uint8_t* zeros, uint8_t* P, int n, int k, int group, int flags,
+                    int b_stride, void* stream);
+int    sg_int4_gemm(const void* A_bf16, const uint8_t* P, void* D_bf16, int m, int n, int k, int group, int flags, void* stream);
+
+/* A mixture-of-experts layer for a few tokens (m <= 64): bf16 activations, experts in E4M3 with a scale an output channel.  No counterpart in the reference.
+ *   sg_moe_route    logits = X x R^T (X [m][hidden], R [experts][hidden] bf16; summed in 64 bits, rounded to fp32);  ids [m][top_k] = the
+ *                   experts of the largest logits, the largest first, ties to the lower index, NaNs last;  weights [m][top_k] = softmax of the chosen logits
+ *                   (renormalize != 0), or the chosen ones' part of the softmax over all experts
+ *   sg_moe_experts  h = bf16( silu(S1_gate * (W1_gate x)) * (S1_up * (W1_up x)) ) for every token and expert chosen,
+ *                   D = bf16( sum over the chosen of weight * S2 * (W2 h) ), fp32 sums, in an order fixed by the arguments: bit-reproducible.
+ *                   W1 [experts][2 * inner][hidden], the gate's rows first, W2 [experts][hidden][inner], both E4M3;  S1 [experts][2 * inner] and
+ *                   S2 [experts][hidden] floats, or NULL (factors of 1).  ids may come from any router: an id outside 0..experts-1 is no
+ *                   expert, a token with none has a row of zeros, and an expert that a token names twice counts with both weights.
+ *   sg_moe_layer    both;  ids and weights are outputs
+ * workspace: sg_moe_workspace_bytes(...) bytes of device memory (0 for sizes that are refused), 256-byte aligned, no content needed; calls in
+ * stream order may share it, calls that overlap - recorded graphs that replay side by side too - need one each.  Nothing else is
+ * allocated or kept.  1 <= m <= 64, hidden and inner multiples of 16, experts <= 512, top_k <= 16 and <= experts; X, R, W1, W2 and D
+ * 16-byte aligned, floats and ids 4-byte.  D must not overlap an input. */
+size_t sg_moe_workspace_bytes(int m, int hidden, int inner, int experts, int top_k);
+int sg_moe_route(const void* X_bf16, const void* R_bf16, int32_t* ids, float* weights, int m, int hidden, int experts, int top_k,
+                 int renormalize, void* workspace, size_t workspace_bytes, void* stream);
+int sg_moe_experts(const void* X_bf16, const int32_t* ids, const float* weights, const uint8_t* W1, const float* S1, const uint8_t* W2,
+                   const float* S2, void* D_bf16, int m, int hidden, int inner, int experts, int top_k, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int sg_moe_layer(const void* X_bf16, const void* R_bf16, const uint8_t* W1, const float* S1, const uint8_t* W2, const float* S2,
+                 void* D_bf16, int32_t* ids, float* weights, int m, int hidden, int inner, int experts, int top_k, int renormalize,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,7 +24,7 @@ if host.torch_version != torch.__version__:    # it reads torch's own structures
     raise ImportError("%s was built against torch %s, this is %s: build it again" % (HOST_PATH, host.torch_version, torch.__version__))
 host.bind(lib._handle)
 
-_vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
+_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
 
 SIGNATURES = {
     "sg_strerror": (C.c_char_p, [_i]),
@@ -81,6 +81,14 @@ SIGNATURES = {
     "sg_mxfp4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "sg_mxfp4_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "sg_mxfp4_gemm_fp8act": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "sg_rmsnorm_fp8_rows": (_i, [_vp] * 7 + [_f, _i, _i, _vp]),
+    "sg_int4_packed_bytes": (_sz, [_i] * 4),
+    "sg_int4_pack": (_i, [_vp] * 4 + [_i] * 5 + [_vp]),
+    "sg_int4_gemm": (_i, [_vp] * 3 + [_i] * 5 + [_vp]),
+    "sg_moe_workspace_bytes": (_sz, [_i] * 5),
+    "sg_moe_route": (_i, [_vp] * 4 + [_i] * 5 + [_vp, _sz, _vp]),
+    "sg_moe_experts": (_i, [_vp] * 8 + [_i] * 5 + [_vp, _sz, _vp]),
+    "sg_moe_layer": (_i, [_vp] * 9 + [_i] * 6 + [_vp, _sz, _vp]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():

@@ -646,3 +646,205 @@ def mxfp4_gemm_fp8act(A, P, D, scale_tensor=None, row_scales=None, check=False):
                                       None if scale_tensor is None else _dev(scale_tensor, torch.float32),
                                       None if row_scales is None else _dev(row_scales, torch.float32), m, n, k, _stream())
     return _done(rc, check)
+
+
+def _matrix(t, rows, cols, name):
+    if tuple(t.shape) != (rows, cols):
+        raise ValueError("%s must be [%d, %d], got %s" % (name, rows, cols, tuple(t.shape)))
+    _row_major(t, name)
+
+
+def _ptr(t, *dtypes):
+    return None if t is None else _dev(t, *dtypes)
+
+
+def rmsnorm_fp8_rows(X, Q, scales, weight=None, residual=None, sum_out=None, Y=None, eps=1e-6, check=False):
+    """Root-mean-square norm of X (+ residual) [rows, cols] bfloat16, times weight [cols], into E4M3 rows Q with scales [rows]
+    (float32): what fp8_encode_rows gives of the norm in 32 bits.  sum_out, if given, receives X + residual (it may be X or
+    residual itself), Y the norm in bfloat16."""
+    rc = host.rmsnorm_fp8_rows(X, Q, scales, weight, residual, sum_out, Y, eps)
+    if rc is not None:
+        return _done(rc, check)
+    if X.dim() != 2 or X.shape[1] % 16:
+        raise ValueError("X must be [rows, cols] with cols a multiple of 16, got %s" % (tuple(X.shape),))
+    rows, cols = X.shape
+    for t, name in ((X, "X"), (Q, "Q"), (residual, "residual"), (sum_out, "sum_out"), (Y, "Y")):
+        if t is not None:
+            _matrix(t, rows, cols, name)
+    _vector(scales, rows, "scales")
+    if weight is not None and (tuple(weight.shape) != (cols,) or not weight.is_contiguous()):
+        raise ValueError("weight must be a contiguous vector of %d values, got shape %s strides %s"
+                         % (cols, tuple(weight.shape), tuple(weight.stride())))
+    _same_device(X, Q, scales, weight, residual, sum_out, Y)
+    with torch.cuda.device(X.device):
+        rc = lib.sg_rmsnorm_fp8_rows(_dev(X, torch.bfloat16), _ptr(residual, torch.bfloat16), _ptr(weight, torch.bfloat16),
+                                     _ptr(sum_out, torch.bfloat16), _ptr(Y, torch.bfloat16), _dev(Q, *_FP8), _dev(scales, torch.float32),
+                                     eps, rows, cols, _stream())
+    return _done(rc, check)
+
+
+# 4-bit integers with group scales (include/sgemm.h): codes two a byte, a scale and on request a zero for each group of a row's columns.
+_INT4_ZEROS, _INT4_F16_SCALES = 1, 2
+
+
+def _int4_flags(zeros, scale_dtype):
+    if scale_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("scales must be bfloat16 or float16, got %s" % scale_dtype)
+    return (_INT4_ZEROS if zeros else 0) | (_INT4_F16_SCALES if scale_dtype == torch.float16 else 0)
+
+
+def int4_packed_bytes(n, k, group=128, zeros=False):
+    """Bytes of the packed form of n x k weights in groups of 32, 64 or 128 columns (k a multiple of the group), with zeros or without."""
+    need = lib.sg_int4_packed_bytes(n, k, group, _INT4_ZEROS if zeros else 0)
+    if need == 0:
+        raise ValueError("packed weights need n > 0, a group of 32, 64 or 128 and k a positive multiple of it, got n = %d, k = %d, group = %d"
+                         % (n, k, group))
+    return need
+
+
+def _int4_packed(P, n, k, group, zeros):
+    need = int4_packed_bytes(n, k, group, zeros)
+    if P.dim() != 1 or P.numel() != need or not P.is_contiguous():
+        raise ValueError("P must be a contiguous vector of %d bytes (%d x %d weights packed in groups of %d%s), got shape %s strides %s"
+                         % (need, n, k, group, " with zeros" if zeros else "", tuple(P.shape), tuple(P.stride())))
+
+
+def int4_pack(B, scales, P, zeros=None, check=False):
+    """Weights B [n, k/2] (codes two a byte, the even column in the low nibble; rows at any stride that 16 divides) with scales
+    [n, k/group] in bfloat16 or float16 and zeros [n, k/group] in uint8 (None: 8) -> P, a contiguous uint8 vector of
+    int4_packed_bytes(n, k, group, zeros is not None) that int4_gemm reads.  Once per weight matrix; the group is what the scales'
+    shape says."""
+    if B.dim() != 2 or scales.dim() != 2 or scales.shape[1] == 0 or (2 * B.shape[1]) % scales.shape[1]:
+        raise ValueError("B must be [n, k/2] and scales [n, k/group], got %s and %s" % (tuple(B.shape), tuple(scales.shape)))
+    n, k = B.shape[0], 2 * B.shape[1]
+    group = k // scales.shape[1]
+    b_stride = _weights(B, k // 2)
+    _matrix(scales, n, k // group, "scales")
+    if zeros is not None:
+        _matrix(zeros, n, k // group, "zeros")
+    _int4_packed(P, n, k, group, zeros is not None)
+    flags = _int4_flags(zeros is not None, scales.dtype)
+    _same_device(B, scales, zeros, P)
+    with torch.cuda.device(B.device):
+        rc = lib.sg_int4_pack(_dev(B, torch.uint8), _dev(scales), _ptr(zeros, torch.uint8), _dev(P, torch.uint8), n, k, group, flags, b_stride,
+                              _stream())
+    return _done(rc, check)
+
+
+def int4_gemm(A, P, D, group=128, zeros=False, scale_dtype=torch.bfloat16, check=False):
+    """D[m,n] = bf16(A @ B^T), A [m, k] bfloat16, B packed into P (int4_pack) in groups of `group` columns, with zeros or without, its
+    scales in scale_dtype."""
+    flags = _int4_flags(zeros, scale_dtype)
+    rc = host.int4_gemm(A, P, D, group, flags)
+    if rc is not None:
+        return _done(rc, check)
+    if A.dim() != 2 or D.dim() != 2 or D.shape[0] != A.shape[0]:
+        raise ValueError("A and D must be matrices of as many rows, got %s and %s" % (tuple(A.shape), tuple(D.shape)))
+    (m, k), n = A.shape, D.shape[1]
+    _int4_packed(P, n, k, group, zeros)
+    _row_major(A, "A")
+    _row_major(D, "D")
+    _same_device(A, P, D)
+    with torch.cuda.device(A.device):
+        rc = lib.sg_int4_gemm(_dev(A, torch.bfloat16), _dev(P, torch.uint8), _dev(D, torch.bfloat16), m, n, k, group, flags, _stream())
+    return _done(rc, check)
+
+
+# A mixture-of-experts layer for up to 64 tokens (include/sgemm.h).
+def moe_workspace_bytes(m, hidden, inner, experts, top_k):
+    """Bytes of workspace that moe_layer and moe_experts take for these sizes."""
+    need = lib.sg_moe_workspace_bytes(m, hidden, inner, experts, top_k)
+    if need == 0:
+        raise ValueError("1 <= m <= 64 tokens, hidden and inner multiples of 16, up to 512 experts and top_k <= 16 of them are taken, got m = %d, "
+                         "hidden = %d, inner = %d, experts = %d, top_k = %d" % (m, hidden, inner, experts, top_k))
+    return need
+
+
+def _moe_workspace(workspace, need, device):
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.dim() != 1 or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 vector, got %s %s" % (workspace.dtype, tuple(workspace.shape)))
+    return workspace
+
+
+def _moe_choice(X, ids, weights):
+    if X.dim() != 2 or ids.dim() != 2 or ids.shape[0] != X.shape[0]:
+        raise ValueError("X must be [m, hidden] and ids [m, top_k], got %s and %s" % (tuple(X.shape), tuple(ids.shape)))
+    _row_major(X, "X")
+    _matrix(ids, *ids.shape, "ids")
+    _matrix(weights, *ids.shape, "weights")
+    return (*X.shape, ids.shape[1])
+
+
+def _moe_experts(X, W1, W2, D, S1, S2):
+    m, hidden = X.shape
+    if W1.dim() != 3 or W1.shape[1] % 2 or W1.shape[2] != hidden:
+        raise ValueError("W_gate_up must be [experts, 2 * inner, %d], got %s" % (hidden, tuple(W1.shape)))
+    experts, inner = W1.shape[0], W1.shape[1] // 2
+    if tuple(W2.shape) != (experts, hidden, inner):
+        raise ValueError("W_down must be [%d, %d, %d], got %s" % (experts, hidden, inner, tuple(W2.shape)))
+    _row_major(W1, "W_gate_up")
+    _row_major(W2, "W_down")
+    _matrix(D, m, hidden, "D")
+    if S1 is not None:
+        _matrix(S1, experts, 2 * inner, "gate_up_scales")
+    if S2 is not None:
+        _matrix(S2, experts, hidden, "down_scales")
+    return experts, inner
+
+
+def moe_route(X, router, ids, weights, renormalize=True, workspace=None, check=False):
+    """The router of a mixture-of-experts layer: X [m, hidden] and router [experts, hidden] bfloat16 -> ids [m, top_k] int32, the experts
+    of the largest logits in their order (ties: the lower index), and weights [m, top_k] float32, their softmax (renormalize=False:
+    their part of the softmax over all experts)."""
+    m, hidden, top_k = _moe_choice(X, ids, weights)
+    if router.dim() != 2 or router.shape[1] != hidden:
+        raise ValueError("router must be [experts, %d], got %s" % (hidden, tuple(router.shape)))
+    _row_major(router, "router")
+    experts = router.shape[0]
+    moe_workspace_bytes(m, hidden, 16, experts, top_k)
+    _same_device(X, router, ids, weights, workspace)
+    with torch.cuda.device(X.device):
+        ws = _moe_workspace(workspace, 4 * m * experts, X.device)
+        rc = lib.sg_moe_route(_dev(X, torch.bfloat16), _dev(router, torch.bfloat16), _dev(ids, torch.int32), _dev(weights, torch.float32), m, hidden,
+                              experts, top_k, int(bool(renormalize)), _dev(ws), ws.numel(), _stream())
+    return _done(rc, check)
+
+
+def moe_experts(X, ids, weights, W_gate_up, W_down, D, gate_up_scales=None, down_scales=None, workspace=None, check=False):
+    """D [m, hidden] = sum over a token's experts of weight * down(silu(gate(x)) * up(x)): X [m, hidden] bfloat16, ids [m, top_k] int32
+    (outside 0..experts-1: none), weights [m, top_k] float32, W_gate_up [experts, 2 * inner, hidden] (the gate's rows first) and W_down
+    [experts, hidden, inner] E4M3 with a scale a row ([experts, 2 * inner], [experts, hidden] float32, or None)."""
+    m, hidden, top_k = _moe_choice(X, ids, weights)
+    experts, inner = _moe_experts(X, W_gate_up, W_down, D, gate_up_scales, down_scales)
+    need = moe_workspace_bytes(m, hidden, inner, experts, top_k)
+    _same_device(X, ids, weights, W_gate_up, W_down, D, gate_up_scales, down_scales, workspace)
+    with torch.cuda.device(X.device):
+        ws = _moe_workspace(workspace, need, X.device)
+        rc = lib.sg_moe_experts(_dev(X, torch.bfloat16), _dev(ids, torch.int32), _dev(weights, torch.float32), _dev(W_gate_up, *_FP8),
+                                _ptr(gate_up_scales, torch.float32), _dev(W_down, *_FP8), _ptr(down_scales, torch.float32),
+                                _dev(D, torch.bfloat16), m, hidden, inner, experts, top_k, _dev(ws), ws.numel(), _stream())
+    return _done(rc, check)
+
+
+def moe_layer(X, router, W_gate_up, W_down, D, ids, weights, gate_up_scales=None, down_scales=None, renormalize=True, workspace=None,
+              check=False):
+    """moe_route and moe_experts in one call; ids [m, top_k] int32 and weights [m, top_k] float32 are outputs.  workspace: a uint8
+    vector of moe_workspace_bytes(m, hidden, inner, experts, top_k), allocated for the call if it is None; calls that may overlap need
+    one each."""
+    rc = host.moe_layer(X, router, W_gate_up, W_down, D, ids, weights, gate_up_scales, down_scales, renormalize, workspace)
+    if rc is not None:
+        return _done(rc, check)
+    m, hidden, top_k = _moe_choice(X, ids, weights)
+    experts, inner = _moe_experts(X, W_gate_up, W_down, D, gate_up_scales, down_scales)
+    _matrix(router, experts, hidden, "router")
+    need = moe_workspace_bytes(m, hidden, inner, experts, top_k)
+    _same_device(X, router, W_gate_up, W_down, D, ids, weights, gate_up_scales, down_scales, workspace)
+    with torch.cuda.device(X.device):
+        ws = _moe_workspace(workspace, need, X.device)
+        rc = lib.sg_moe_layer(_dev(X, torch.bfloat16), _dev(router, torch.bfloat16), _dev(W_gate_up, *_FP8), _ptr(gate_up_scales, torch.float32),
+                              _dev(W_down, *_FP8), _ptr(down_scales, torch.float32), _dev(D, torch.bfloat16), _dev(ids, torch.int32),
+                              _dev(weights, torch.float32), m, hidden, inner, experts, top_k, int(bool(renormalize)), _dev(ws), ws.numel(),
+                              _stream())
+    return _done(rc, check)

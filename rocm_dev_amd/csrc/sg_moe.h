@@ -1,0 +1,66 @@
+// A mixture-of-experts layer for a few tokens: what its translation units share (include/sgemm.h says what it computes).
+//
+// Launches: the router's logits; the plan, made by one workgroup - the chosen experts (moe_route, moe_layer), then which experts are
+// reached and by which tokens -; gate and up projections of every reached expert; down projections, added up over a token's
+// experts.  Each hands over through the caller's workspace and the end of a launch: nothing waits on the device, so calls
+// that overlap cannot wait for each other.
+#pragma once
+
+#include "sg_device.h"
+#include "sg_host.h"
+
+namespace sg {
+
+constexpr int kMoeTokens = 64;      // a token is a bit of 64 in the plan
+constexpr int kMoeExperts = 512;
+constexpr int kMoeTopK = 16;
+
+// The plan: dwords [reached experts' number][expert of each: id | (number of its tokens) << 16][its first entry][entries: row of h = token *
+// top_k + the choice that names the expert first][entries' weights].  At most one entry a token and choice.
+struct MoePlanLayout {
+    int experts_at, first_at, rows_at, weights_at, dwords;
+};
+__host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int top_k) {
+    const int pairs = m * top_k, most = experts < pairs ? experts : pairs;      // experts that can be reached
+    MoePlanLayout l;
+    l.experts_at = 4;
+    l.first_at = l.experts_at + most;
+    l.rows_at = l.first_at + most;
+    l.weights_at = l.rows_at + pairs;
+    l.dwords = (l.weights_at + pairs + 3) / 4 * 4;
+    return l;
+}
+
+struct MoeLayout {
+    size_t plan_at, h_at, bytes;     // logits first
+};
+inline bool moe_takes(int m, int hidden, int inner, int experts, int top_k) {
+    return m > 0 && m <= kMoeTokens && hidden > 0 && hidden % 16 == 0 && inner > 0 && inner % 16 == 0 && inner <= (1 << 26) &&
+           hidden <= (1 << 26) && experts > 0 && experts <= kMoeExperts && top_k > 0 && top_k <= kMoeTopK && top_k <= experts;
+}
+inline MoeLayout moe_layout(int m, int inner, int experts, int top_k) {
+    MoeLayout l;
+    l.plan_at = ((size_t)m * experts * 4 + 255) / 256 * 256;
+    l.h_at = l.plan_at + ((size_t)moe_plan_layout(m, experts, top_k).dwords * 4 + 255) / 256 * 256;
+    l.bytes = l.h_at + (size_t)m * top_k * inner * 2;
+    return l;
+}
+
+struct MoeArgs {
+    const uint8_t* X;                // [m][hidden] bf16
+    const uint8_t* R;                // [experts][hidden] bf16
+    const uint8_t* W1;               // [experts][2 * inner][hidden] E4M3
+    const float* S1;                 // [experts][2 * inner], or NULL
+    const uint8_t* W2;               // [experts][hidden][inner] E4M3
+    const float* S2;                 // [experts][hidden], or NULL
+    uint16_t* D;                     // [m][hidden] bf16
+    int32_t* ids;                    // [m][top_k]
+    float* weights;                  // [m][top_k]
+    float* logits;                   // [m][experts]
+    int32_t* plan;
+    uint8_t* H;                      // [m * top_k][inner] bf16
+    int m, hidden, inner, experts, top_k, renormalize;
+    int items;                       // gate and up: 16-row tiles of inner times experts that may be reached
+};
+
+}  // namespace sg

@@ -26,7 +26,8 @@ namespace {
 #define SG_ENTRIES(X)                                                                                               \
     X(sg_skinny_gemm_auto) X(sg_skinny_gemm_rowcol) X(sg_skinny_gemm_bf16act) X(sg_sparse24_gemm)                   \
     X(sg_sparse24_compress) X(sg_fp8_encode_rows) X(sg_fp8_decode_rows) X(sg_fp8_reduce_rows) X(sg_tiled_sum_reduce)    \
-    X(sg_mxfp4_packed_bytes) X(sg_mxfp4_encode_rows) X(sg_mxfp4_decode_rows) X(sg_mxfp4_gemm) X(sg_mxfp4_gemm_fp8act)
+    X(sg_mxfp4_packed_bytes) X(sg_mxfp4_encode_rows) X(sg_mxfp4_decode_rows) X(sg_mxfp4_gemm) X(sg_mxfp4_gemm_fp8act)    \
+    X(sg_rmsnorm_fp8_rows) X(sg_int4_packed_bytes) X(sg_int4_gemm) X(sg_moe_workspace_bytes) X(sg_moe_layer)
 #define SG_POINTER(name) decltype(&::name) p_##name = nullptr;
 SG_ENTRIES(SG_POINTER)
 #undef SG_POINTER
@@ -408,6 +409,96 @@ PyObject* mxfp4_gemm_fp8act(PyObject*, Args v, Py_ssize_t nargs) {
     });
 }
 
+// X, Q, scales, weight or None, residual or None, sum_out or None, Y or None, eps
+PyObject* rmsnorm_fp8_rows(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 8, [&]() -> PyObject* {
+        Operands o;
+        const Codec c(o, v[0], v[1], v[2], false);
+        const at::Tensor* weight = o.tensor(v[3], 1, kOptional);
+        if (weight) o.need(weight->scalar_type() == at::kBFloat16 && weight->size(0) == c.cols && weight->is_contiguous());
+        const at::Tensor* like[3];
+        for (int i = 0; i < 3; i++) {
+            const at::Tensor* t = like[i] = o.tensor(v[4 + i], 2, kOptional);
+            if (t) o.need(t->scalar_type() == at::kBFloat16 && t->size(0) == c.rows && t->size(1) == c.cols && t->is_contiguous());
+        }
+        if (!o.ready() || !PyFloat_Check(v[7])) return nullptr;
+        const float eps = (float)PyFloat_AS_DOUBLE(v[7]);
+        const void *x = c.X->const_data_ptr(), *w = weight ? weight->const_data_ptr() : nullptr;
+        const void* res = like[0] ? like[0]->const_data_ptr() : nullptr;
+        void *sum = like[1] ? like[1]->mutable_data_ptr() : nullptr, *y = like[2] ? like[2]->mutable_data_ptr() : nullptr;
+        uint8_t* q = static_cast<uint8_t*>(c.Q->mutable_data_ptr());
+        float* s = static_cast<float*>(c.S->mutable_data_ptr());
+        void* st = o.stream();
+        return enqueue([&] { return p_sg_rmsnorm_fp8_rows(x, res, w, sum, y, q, s, eps, c.rows, c.cols, st); });
+    });
+}
+
+// a Python int of a few bits, or false
+bool small_int(PyObject* o, int* out) {
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    const long t = PyLong_AsLongAndOverflow(o, &over);
+    *out = (int)t;
+    return !over && t >= 0 && t <= 1 << 20;
+}
+
+// A, P, D, group, flags
+PyObject* int4_gemm(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 5, [&]() -> PyObject* {
+        Operands o;
+        const at::Tensor* A = o.row_major(v[0], 2);
+        const at::Tensor* P = o.row_major(v[1], 1);
+        const at::Tensor* D = o.row_major(v[2], 2);
+        int group = 0, flags = 0;
+        if (!o.plain || !small_int(v[3], &group) || !small_int(v[4], &flags)) return nullptr;
+        o.need(A->scalar_type() == at::kBFloat16 && P->scalar_type() == at::kByte && D->scalar_type() == at::kBFloat16);
+        o.need(A->size(0) == D->size(0));
+        const int m = o.size(A->size(0)), n = o.size(D->size(1)), k = o.size(A->size(1));
+        if (!o.plain) return nullptr;
+        const size_t need = p_sg_int4_packed_bytes(n, k, group, flags);
+        o.need(need > 0 && (size_t)P->numel() == need);
+        if (!o.ready()) return nullptr;
+        const void* a = A->const_data_ptr();
+        const uint8_t* p = bytes(*P);
+        void *d = D->mutable_data_ptr(), *st = o.stream();
+        return enqueue([&] { return p_sg_int4_gemm(a, p, d, m, n, k, group, flags, st); });
+    });
+}
+
+// X, router, W_gate_up, W_down, D, ids, weights, gate_up_scales or None, down_scales or None, renormalize, workspace
+PyObject* moe_layer(PyObject*, Args v, Py_ssize_t nargs) {
+    return entry(nargs, 11, [&]() -> PyObject* {
+        Operands o;
+        const at::Tensor *X = o.row_major(v[0], 2), *R = o.row_major(v[1], 2), *W1 = o.row_major(v[2], 3), *W2 = o.row_major(v[3], 3);
+        const at::Tensor *D = o.row_major(v[4], 2), *ids = o.row_major(v[5], 2), *weights = o.row_major(v[6], 2);
+        const at::Tensor *S1 = o.tensor(v[7], 2, kOptional), *S2 = o.tensor(v[8], 2, kOptional), *ws = o.row_major(v[10], 1);
+        if (!o.plain || !PyBool_Check(v[9])) return nullptr;
+        o.need(X->scalar_type() == at::kBFloat16 && R->scalar_type() == at::kBFloat16 && D->scalar_type() == at::kBFloat16);
+        o.need(fp8(W1->scalar_type()) && fp8(W2->scalar_type()) && ids->scalar_type() == at::kInt && weights->scalar_type() == at::kFloat &&
+               ws->scalar_type() == at::kByte);
+        const int64_t m = X->size(0), hidden = X->size(1), experts = W1->size(0), inner = W2->size(2), top_k = ids->size(1);
+        o.need(R->size(0) == experts && R->size(1) == hidden && W1->size(1) == 2 * inner && W1->size(2) == hidden);
+        o.need(W2->size(0) == experts && W2->size(1) == hidden && D->size(0) == m && D->size(1) == hidden);
+        o.need(ids->size(0) == m && weights->size(0) == m && weights->size(1) == top_k);
+        if (S1) o.need(S1->scalar_type() == at::kFloat && S1->size(0) == experts && S1->size(1) == 2 * inner && S1->is_contiguous());
+        if (S2) o.need(S2->scalar_type() == at::kFloat && S2->size(0) == experts && S2->size(1) == hidden && S2->is_contiguous());
+        const int im = o.size(m), ih = o.size(hidden), ii = o.size(inner), ie = o.size(experts), ik = o.size(top_k);
+        if (!o.plain) return nullptr;
+        const size_t room = (size_t)ws->numel(), need = p_sg_moe_workspace_bytes(im, ih, ii, ie, ik);
+        o.need(need > 0 && room >= need);
+        if (!o.ready()) return nullptr;
+        const void *x = X->const_data_ptr(), *r = R->const_data_ptr();
+        const uint8_t *w1 = bytes(*W1), *w2 = bytes(*W2);
+        const float* s1 = S1 ? static_cast<const float*>(S1->const_data_ptr()) : nullptr;
+        const float* s2 = S2 ? static_cast<const float*>(S2->const_data_ptr()) : nullptr;
+        int32_t* id = static_cast<int32_t*>(ids->mutable_data_ptr());
+        float* wt = static_cast<float*>(weights->mutable_data_ptr());
+        void *d = D->mutable_data_ptr(), *space = ws->mutable_data_ptr(), *st = o.stream();
+        const int renormalize = v[9] == Py_True;
+        return enqueue([&] { return p_sg_moe_layer(x, r, w1, s1, w2, s2, d, id, wt, im, ih, ii, ie, ik, renormalize, space, room, st); });
+    });
+}
+
 // bind(handle of libsgemm.so)
 PyObject* bind(PyObject*, PyObject* arg) {
     void* handle = PyLong_AsVoidPtr(arg);
@@ -438,6 +529,9 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          SG_METHOD(mxfp4_decode_rows),
                          SG_METHOD(mxfp4_gemm),
                          SG_METHOD(mxfp4_gemm_fp8act),
+                         SG_METHOD(rmsnorm_fp8_rows),
+                         SG_METHOD(int4_gemm),
+                         SG_METHOD(moe_layer),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_host", nullptr, -1, methods};
 

@@ -17,6 +17,11 @@ their output shapes through fake (meta) implementations, and launch on torch's c
     P = torch.ops.sgemm.mxfp4_pack(W_codes, W_scales)                       # once per weight matrix
     D = torch.ops.sgemm.mxfp4_gemm(Q, S, P, n, scale)                       # [m, n] bf16
     D = torch.ops.sgemm.mxfp4_gemm_fp8act(A_fp8, P, n, scale, row_scales)
+    Q, s, total, Y = torch.ops.sgemm.rmsnorm_fp8_rows(X_bf16, weight, residual, eps)    # E4M3 rows, X + residual, the norm in bf16
+    P = torch.ops.sgemm.int4_pack(W_codes, W_scales, W_zeros)               # once per weight matrix
+    D = torch.ops.sgemm.int4_gemm(X_bf16, P, n, group, zeros, f16_scales)
+    ids, w = torch.ops.sgemm.moe_route(X_bf16, router, top_k)
+    D = torch.ops.sgemm.moe_experts(X_bf16, ids, w, W_gate_up, W_down, gate_up_scales, down_scales)
 
 FP8 operands are uint8 or float8_e4m3fn tensors holding OCP E4M3 codes; weights are [n, k] with k contiguous.
 """
@@ -181,3 +186,72 @@ def mxfp4_gemm_fp8act(A: torch.Tensor, P: torch.Tensor, n: int, scale: Optional[
 @mxfp4_gemm_fp8act.register_fake
 def _(A, P, n, scale=None, row_scales=None):
     return A.new_empty((A.shape[0], n), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("sgemm::rmsnorm_fp8_rows", mutates_args=())
+def rmsnorm_fp8_rows(X: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    Q = torch.empty(X.shape, dtype=torch.uint8, device=X.device)
+    s = torch.empty((X.shape[0],), dtype=torch.float32, device=X.device)
+    total, Y = torch.empty_like(X, memory_format=torch.contiguous_format), torch.empty_like(X, memory_format=torch.contiguous_format)
+    api.rmsnorm_fp8_rows(X.contiguous(), Q, s, None if weight is None else weight.contiguous(), None if residual is None else residual.contiguous(),
+                         total, Y, eps, check=True)
+    return Q, s, total, Y
+
+
+@rmsnorm_fp8_rows.register_fake
+def _(X, weight=None, residual=None, eps=1e-6):
+    return (X.new_empty(X.shape, dtype=torch.uint8), X.new_empty((X.shape[0],), dtype=torch.float32), X.new_empty(X.shape), X.new_empty(X.shape))
+
+
+@torch.library.custom_op("sgemm::int4_pack", mutates_args=())
+def int4_pack(B: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> torch.Tensor:
+    n, k = B.shape[0], 2 * B.shape[1]
+    P = torch.empty((api.int4_packed_bytes(n, k, k // max(scales.shape[1], 1), zeros is not None),), dtype=torch.uint8, device=B.device)
+    api.int4_pack(B, scales.contiguous(), P, None if zeros is None else zeros.contiguous(), check=True)
+    return P
+
+
+@int4_pack.register_fake
+def _(B, scales, zeros=None):
+    steps, groups = (2 * B.shape[1] + 127) // 128, 128 // (2 * B.shape[1] // scales.shape[1])
+    return B.new_empty(((B.shape[0] + 15) // 16 * steps * (1024 + groups * (32 if zeros is None else 48)),), dtype=torch.uint8)
+
+
+@torch.library.custom_op("sgemm::int4_gemm", mutates_args=())
+def int4_gemm(A: torch.Tensor, P: torch.Tensor, n: int, group: int = 128, zeros: bool = False, f16_scales: bool = False) -> torch.Tensor:
+    D = torch.empty((A.shape[0], n), dtype=torch.bfloat16, device=A.device)
+    api.int4_gemm(A.contiguous(), P, D, group, zeros, torch.float16 if f16_scales else torch.bfloat16, check=True)
+    return D
+
+
+@int4_gemm.register_fake
+def _(A, P, n, group=128, zeros=False, f16_scales=False):
+    return A.new_empty((A.shape[0], n), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("sgemm::moe_route", mutates_args=())
+def moe_route(X: torch.Tensor, router: torch.Tensor, top_k: int, renormalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    ids = torch.empty((X.shape[0], top_k), dtype=torch.int32, device=X.device)
+    weights = torch.empty((X.shape[0], top_k), dtype=torch.float32, device=X.device)
+    api.moe_route(X.contiguous(), router, ids, weights, renormalize, check=True)
+    return ids, weights
+
+
+@moe_route.register_fake
+def _(X, router, top_k, renormalize=True):
+    return X.new_empty((X.shape[0], top_k), dtype=torch.int32), X.new_empty((X.shape[0], top_k), dtype=torch.float32)
+
+
+@torch.library.custom_op("sgemm::moe_experts", mutates_args=())
+def moe_experts(X: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, W_gate_up: torch.Tensor, W_down: torch.Tensor,
+                gate_up_scales: Optional[torch.Tensor] = None, down_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    D = torch.empty(X.shape, dtype=torch.bfloat16, device=X.device)
+    api.moe_experts(X.contiguous(), ids.contiguous(), weights.contiguous(), _weights(W_gate_up), _weights(W_down), D, _rows(gate_up_scales),
+                    _rows(down_scales), check=True)
+    return D
+
+
+@moe_experts.register_fake
+def _(X, ids, weights, W_gate_up, W_down, gate_up_scales=None, down_scales=None):
+    return X.new_empty(X.shape, dtype=torch.bfloat16)

@@ -1,9 +1,9 @@
 // A mixture-of-experts layer for a few tokens: what its translation units share (include/sgemm.h says what it computes).
 //
-// Launches: the router's logits; the plan, made by one workgroup - the chosen experts (moe_route, moe_layer), then which experts are
-// reached and by which tokens -; gate and up projections of every reached expert; down projections, added up over a token's
-// experts.  Each hands over through the caller's workspace and the end of a launch: nothing waits on the device, so calls
-// that overlap cannot wait for each other.
+// Launches: the router's logits (moe_route, moe_layer); the choice of experts, for more than kMoeFused tokens one of its own; gate and
+// up projections of every reached expert, whose workgroups each make the plan - who goes where - and, for few tokens, the choice for
+// themselves; down projections, added up over a token's experts.  Each hands over through the caller's workspace and the
+// end of a launch: nothing waits on the device, so calls that overlap cannot wait for each other.
 #pragma once
 
 #include "sg_device.h"
@@ -15,17 +15,22 @@ constexpr int kMoeTokens = 64;      // a token is a bit of 64 in the plan
 constexpr int kMoeExperts = 512;
 constexpr int kMoeTopK = 16;
 
-// The plan: dwords [reached experts' number][expert of each: id | (number of its tokens) << 16][its first entry][entries: row of h = token *
-// top_k + the choice that names the expert first][entries' weights].  At most one entry a token and choice.
+constexpr int kMoeSide = 1 << 20;   // hidden, inner: rows of a tile, of all activations and of W1's count within 32 bits
+constexpr int kMoeFused = 8;        // tokens whose experts every workgroup chooses for itself
+
+// The plan: dwords [number of parts][part: expert | entries << 16][its first entry][entry: row of h = token * top_k + the choice that
+// names the expert first][its weight].  An entry is a token and an expert that it names; a part is up to 16 * MB entries of one
+// expert, the columns of one product: an expert with more is read once for each part.
 struct MoePlanLayout {
-    int experts_at, first_at, rows_at, weights_at, dwords;
+    int parts_at, first_at, rows_at, weights_at, dwords, most;
 };
 __host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int top_k) {
-    const int pairs = m * top_k, most = experts < pairs ? experts : pairs;      // experts that can be reached
+    const int pairs = m * top_k;
     MoePlanLayout l;
-    l.experts_at = 4;
-    l.first_at = l.experts_at + most;
-    l.rows_at = l.first_at + most;
+    l.most = (experts < pairs ? experts : pairs) + pairs / 16;      // parts
+    l.parts_at = 4;
+    l.first_at = l.parts_at + l.most;
+    l.rows_at = l.first_at + l.most;
     l.weights_at = l.rows_at + pairs;
     l.dwords = (l.weights_at + pairs + 3) / 4 * 4;
     return l;
@@ -35,8 +40,8 @@ struct MoeLayout {
     size_t plan_at, h_at, bytes;     // logits first
 };
 inline bool moe_takes(int m, int hidden, int inner, int experts, int top_k) {
-    return m > 0 && m <= kMoeTokens && hidden > 0 && hidden % 16 == 0 && inner > 0 && inner % 16 == 0 && inner <= (1 << 26) &&
-           hidden <= (1 << 26) && experts > 0 && experts <= kMoeExperts && top_k > 0 && top_k <= kMoeTopK && top_k <= experts;
+    return m > 0 && m <= kMoeTokens && hidden > 0 && hidden % 16 == 0 && hidden <= kMoeSide && inner > 0 && inner % 16 == 0 &&
+           inner <= kMoeSide && experts > 0 && experts <= kMoeExperts && top_k > 0 && top_k <= kMoeTopK && top_k <= experts;
 }
 inline MoeLayout moe_layout(int m, int inner, int experts, int top_k) {
     MoeLayout l;
@@ -60,7 +65,7 @@ struct MoeArgs {
     int32_t* plan;
     uint8_t* H;                      // [m * top_k][inner] bf16
     int m, hidden, inner, experts, top_k, renormalize;
-    int items;                       // gate and up: 16-row tiles of inner times experts that may be reached
+    int share;                       // gate and up: waves that share an item's columns (1, 2, 4)
 };
 
 }  // namespace sg

@@ -1,47 +1,57 @@
 // A mixture-of-experts layer for a few tokens: launches and C entry points (include/sgemm.h).
 #include "sg_moe_kernel.h"
-#include "sg_moe_route_kernel.h"
 
 namespace sg {
 
 static int launched(const char* what) { return report_hip(what, hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED; }
 
 static int launch_logits(const MoeArgs& a, hipStream_t stream) {
-    const unsigned groups = (unsigned)(a.experts + 3) / 4;
-    if (a.m == 1) moe_logits_kernel<1><<<dim3(groups, 1), 256, 0, stream>>>(a);
-    else if (a.m <= 4) moe_logits_kernel<4><<<dim3(groups, 1), 256, 0, stream>>>(a);
-    else moe_logits_kernel<8><<<dim3(groups, (unsigned)(a.m + 7) / 8), 256, 0, stream>>>(a);
+    if (a.m == 1) moe_logits_kernel<1><<<dim3((unsigned)a.experts, 1), 256, 0, stream>>>(a);
+    else moe_logits_kernel<8><<<dim3((unsigned)a.experts, (unsigned)(a.m + 7) / 8), 256, 0, stream>>>(a);
     return launched("moe_logits launch");
 }
 
-template <int MB>
-static int launch_gate_up(const MoeArgs& a, int cu_count, hipStream_t stream) {
-    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs;
-    const long long items = (long long)most * (a.inner / 16);
-    const int steps = (a.hidden + 127) / 128, waves = steps >= 16 ? 8 : steps >= 8 ? 4 : steps >= 4 ? 2 : 1;
-    const unsigned grid = items < 2ll * cu_count ? (unsigned)items : 2u * cu_count;
-    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (size_t)waves * 2 * MB * 1024;
+static int launch_choose(const MoeArgs& a, hipStream_t stream) {
+    moe_choose_kernel<<<(unsigned)a.m, 64, 0, stream>>>(a);
+    return launched("moe_choose launch");
+}
+
+template <int MB, bool CHOOSE>
+static int launch_gate_up(MoeArgs& a, int cu_count, hipStream_t stream) {
+    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
+    const long long items = (long long)most * (a.inner / 16), waves = (MB == 1 ? 16ll : 12ll) * cu_count;
+    a.share = 1;
+    while (a.share < 4 && items * a.share < 2 * waves && steps >= 4 * a.share) a.share *= 2;
+    const long long groups = (items * a.share + 3) / 4;
+    const unsigned grid = groups < waves / 4 ? (unsigned)groups : (unsigned)(waves / 4);
+    const size_t room = moe_plan_room(pairs), part = a.share > 1 ? 4 * 2 * MB * 1024 : 0;
+    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (room > part ? room : part);
     static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<MB>), lds, granted)) return rc;
-    moe_gate_up_kernel<MB><<<grid, 64 * waves, lds, stream>>>(a);
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<MB, CHOOSE>), lds, granted)) return rc;
+    moe_gate_up_kernel<MB, CHOOSE><<<grid, 256, lds, stream>>>(a);
     return launched("moe_gate_up launch");
 }
 
-template <int MB>
-static int launch_down(const MoeArgs& a, int cu_count, hipStream_t stream) {
-    (void)cu_count;
-    const int waves = 8;
-    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (size_t)waves * a.m * 64;
+template <int MB, int DEPTH, int WAVES>
+static int launch_down(const MoeArgs& a, hipStream_t stream) {
+    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
+    const size_t lds = (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64;
     static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<MB>), lds, granted)) return rc;
-    moe_down_kernel<MB><<<a.hidden / 16, 64 * waves, lds, stream>>>(a);
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<MB, DEPTH, WAVES>), lds, granted)) return rc;
+    moe_down_kernel<MB, DEPTH, WAVES><<<a.hidden / 16, 64 * WAVES, lds, stream>>>(a);
     return launched("moe_down launch");
 }
 
-static int launch_experts(const MoeArgs& a, int cu_count, hipStream_t stream) {
-    if (int rc = a.m <= 16 ? launch_gate_up<1>(a, cu_count, stream) : a.m <= 32 ? launch_gate_up<2>(a, cu_count, stream) : launch_gate_up<4>(a, cu_count, stream))
-        return rc;
-    return a.m <= 16 ? launch_down<1>(a, cu_count, stream) : a.m <= 32 ? launch_down<2>(a, cu_count, stream) : launch_down<4>(a, cu_count, stream);
+template <int MB>
+static int launch_both(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
+    if (int rc = choose ? launch_gate_up<MB, true>(a, cu_count, stream) : launch_gate_up<MB, false>(a, cu_count, stream)) return rc;
+    if constexpr (MB == 1) return a.hidden / 16 <= cu_count ? launch_down<1, 3, 16>(a, stream) : launch_down<1, 3, 8>(a, stream);
+    else return a.hidden / 16 <= cu_count ? launch_down<2, 3, 12>(a, stream) : launch_down<2, 3, 8>(a, stream);
+}
+// choose: by the logits, in the gate's launch
+static int launch_experts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
+    // parts of 32 tokens where an expert may well have more than 16: it would be read twice
+    return a.m > 16 && a.m * a.top_k > 8 * a.experts ? launch_both<2>(a, choose, cu_count, stream) : launch_both<1>(a, choose, cu_count, stream);
 }
 
 }  // namespace sg
@@ -107,8 +117,7 @@ int sg_moe_route(const void* X, const void* R, int32_t* ids, float* weights, int
     if (int rc = get_device_info(&dev)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (int rc = launch_logits(a, st)) return rc;
-    moe_plan_kernel<true, false><<<(unsigned)(m + 7) / 8, 512, 0, st>>>(a);
-    return launched("moe_choose launch");
+    return launch_choose(a, st);
 }
 
 int sg_moe_experts(const void* X, const int32_t* ids, const float* weights, const uint8_t* W1, const float* S1, const uint8_t* W2,
@@ -121,10 +130,7 @@ int sg_moe_experts(const void* X, const int32_t* ids, const float* weights, cons
     if (int rc = take_experts(a, W1, S1, W2, S2, D)) return rc;
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    moe_plan_kernel<false, true><<<1, 512, 0, st>>>(a);
-    if (int rc = launched("moe_plan launch")) return rc;
-    return launch_experts(a, dev->cu_count, st);
+    return launch_experts(a, false, dev->cu_count, static_cast<hipStream_t>(stream));
 }
 
 int sg_moe_layer(const void* X, const void* R, const uint8_t* W1, const float* S1, const uint8_t* W2, const float* S2, void* D, int32_t* ids,
@@ -140,9 +146,10 @@ int sg_moe_layer(const void* X, const void* R, const uint8_t* W1, const float* S
     if (int rc = get_device_info(&dev)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (int rc = launch_logits(a, st)) return rc;
-    moe_plan_kernel<true, true><<<1, 512, 0, st>>>(a);
-    if (int rc = launched("moe_plan launch")) return rc;
-    return launch_experts(a, dev->cu_count, st);
+    const bool fused = m <= kMoeFused;
+    if (!fused)
+        if (int rc = launch_choose(a, st)) return rc;
+    return launch_experts(a, fused, dev->cu_count, st);
 }
 
 }  // extern "C"

@@ -19,7 +19,7 @@ constexpr int kMoeSide = 1 << 20;   // hidden, inner: rows of a tile, of all act
 constexpr int kMoeFused = 8;        // tokens whose experts every workgroup chooses for itself
 
 // The plan: dwords [number of parts][part: expert | entries << 16][its first entry][entry: row of h = token * top_k + the choice that
-// names the expert first][its weight].  An entry is a token and an expert that it names; a part is up to 16 * MB entries of one
+// names the expert first][its weight].  An entry is a token and an expert that it names; a part is up to COLS entries of one
 // expert, the columns of one product: an expert with more is read once for each part.
 struct MoePlanLayout {
     int parts_at, first_at, rows_at, weights_at, dwords, most;
@@ -27,7 +27,7 @@ struct MoePlanLayout {
 __host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int top_k) {
     const int pairs = m * top_k;
     MoePlanLayout l;
-    l.most = (experts < pairs ? experts : pairs) + pairs / 16;      // parts
+    l.most = (experts < pairs ? experts : pairs) + pairs / 4;       // parts; COLS is at least 4
     l.parts_at = 4;
     l.first_at = l.parts_at + l.most;
     l.rows_at = l.first_at + l.most;

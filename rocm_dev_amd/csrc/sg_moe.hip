@@ -1,4 +1,6 @@
 // A mixture-of-experts layer for a few tokens: launches and C entry points (include/sgemm.h).
+#include <math.h>
+
 #include "sg_moe_kernel.h"
 
 namespace sg {
@@ -16,42 +18,57 @@ static int launch_choose(const MoeArgs& a, hipStream_t stream) {
     return launched("moe_choose launch");
 }
 
-template <int MB, bool CHOOSE>
-static int launch_gate_up(MoeArgs& a, int cu_count, hipStream_t stream) {
-    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
-    const long long items = (long long)most * (a.inner / 16), waves = (MB == 1 ? 16ll : 12ll) * cu_count;
-    a.share = 1;
-    while (a.share < 4 && items * a.share < 2 * waves && steps >= 4 * a.share) a.share *= 2;
-    const long long groups = (items * a.share + 3) / 4;
-    const unsigned grid = groups < waves / 4 ? (unsigned)groups : (unsigned)(waves / 4);
-    const size_t room = moe_plan_room(pairs), part = a.share > 1 ? 4 * 2 * MB * 1024 : 0;
-    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (room > part ? room : part);
+constexpr size_t kLdsBytes = 160 * 1024;      // a CU's
+
+template <int XU, int DEPTH, bool CHOOSE>
+static int launch_gate_up(const MoeArgs& a, int cu_count, hipStream_t stream) {
+    using Stages = MoeStages<2, XU>;
+    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs;
+    const size_t ring = (size_t)4 * DEPTH * Stages::kBytes, room = moe_plan_room(pairs);
+    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) +
+                       (room > ring ? room : ring);
+    const long long groups = ((long long)most * (a.inner / 16) * a.share + 3) / 4, at_once = (long long)(kLdsBytes / lds) * cu_count;
+    const unsigned grid = (unsigned)(groups < at_once ? groups : at_once);
     static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<MB, CHOOSE>), lds, granted)) return rc;
-    moe_gate_up_kernel<MB, CHOOSE><<<grid, 256, lds, stream>>>(a);
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<XU, DEPTH, CHOOSE>), lds, granted)) return rc;
+    moe_gate_up_kernel<XU, DEPTH, CHOOSE><<<grid, 256, lds, stream>>>(a);
     return launched("moe_gate_up launch");
 }
 
-template <int MB, int DEPTH, int WAVES>
-static int launch_down(const MoeArgs& a, hipStream_t stream) {
+template <int XU, int DEPTH, int WAVES>
+static size_t down_lds(const MoeArgs& a) {
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
-    const size_t lds = (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64;
+    return (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64 + (size_t)WAVES * DEPTH * MoeStages<1, XU>::kBytes;
+}
+template <int XU, int DEPTH, int WAVES>
+static int launch_down(const MoeArgs& a, hipStream_t stream) {
+    const size_t lds = down_lds<XU, DEPTH, WAVES>(a);
     static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<MB, DEPTH, WAVES>), lds, granted)) return rc;
-    moe_down_kernel<MB, DEPTH, WAVES><<<a.hidden / 16, 64 * WAVES, lds, stream>>>(a);
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<XU, DEPTH, WAVES>), lds, granted)) return rc;
+    moe_down_kernel<XU, DEPTH, WAVES><<<a.hidden / 16, 64 * WAVES, lds, stream>>>(a);
     return launched("moe_down launch");
 }
 
-template <int MB>
-static int launch_both(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
-    if (int rc = choose ? launch_gate_up<MB, true>(a, cu_count, stream) : launch_gate_up<MB, false>(a, cu_count, stream)) return rc;
-    if constexpr (MB == 1) return a.hidden / 16 <= cu_count ? launch_down<1, 3, 16>(a, stream) : launch_down<1, 3, 8>(a, stream);
-    else return a.hidden / 16 <= cu_count ? launch_down<2, 3, 12>(a, stream) : launch_down<2, 3, 8>(a, stream);
+// Parts of up to 4 * XU tokens; G and N stages in flight a wave.
+template <int XU, int G, int N>
+static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
+    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
+    a.share = 1;
+    while (a.share < 4 && (long long)most * (a.inner / 16) * a.share < 16ll * cu_count && steps >= 4 * a.share) a.share *= 2;
+    if (int rc = choose ? launch_gate_up<XU, G, true>(a, cu_count, stream) : launch_gate_up<XU, G, false>(a, cu_count, stream)) return rc;
+    if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, 8>(a, stream);
+    if (down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, 8>(a, stream);
+    return launch_down<XU, 2, 4>(a, stream);
 }
 // choose: by the logits, in the gate's launch
 static int launch_experts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
-    // parts of 32 tokens where an expert may well have more than 16: it would be read twice
-    return a.m > 16 && a.m * a.top_k > 8 * a.experts ? launch_both<2>(a, choose, cu_count, stream) : launch_both<1>(a, choose, cu_count, stream);
+    // Columns for an expert's tokens: as many as independent choices of m * top_k / experts on average rarely exceed.
+    const float mean = (float)a.m * a.top_k / a.experts, want = mean + 3.0f * sqrtf(mean);
+    const float columns = want < a.m ? want : a.m;
+    if (columns <= 4) return launch_parts<1, 3, 5>(a, choose, cu_count, stream);
+    if (columns <= 8) return launch_parts<2, 3, 4>(a, choose, cu_count, stream);
+    if (columns <= 16) return launch_parts<4, 2, 3>(a, choose, cu_count, stream);
+    return launch_parts<8, 2, 2>(a, choose, cu_count, stream);
 }
 
 }  // namespace sg

@@ -5,10 +5,15 @@
 // their 16 bits, and the products lose nothing that fp32 sums hold.  An expert's tokens are the columns of the product: MB blocks
 // of 16.
 //
-// Lane (r, g) of a wave takes row r of a 16-row tile and, of a step of 128 columns, columns 16 g .. + 15 and 64 + 16 g .. + 15: 16 contiguous bytes
-// each, two instructions each; the activations' lanes take the same columns, 32 contiguous bytes each.
+// Operands reach LDS by direct loads, 1 KB an instruction: 8 rows x 128 bytes of weights, 4 rows x 256 bytes of activations, so that every
+// line is asked for once and whole.  (Lane (r, g) loading 16 bytes of row r straight into its operand register asks for every line in
+// pieces: 1.29 GB of gate and up 277 us, 4.7 TB/s, however much is in flight.)  Every wave has a ring of its own, DEPTH stages of
+// 128 columns, filled and emptied by itself in order, with no barrier.  The hardware puts lane l's 16 bytes at slot + 16 l; which piece of
+// its row a lane fetches is free, and the pieces of row i stand permuted by i so that the 16 lanes (r, g) of a fragment's read hit
+// 16 bank groups.
 #pragma once
 
+#include "sg_lds_kernel.h"
 #include "sg_moe_route_kernel.h"
 
 namespace sg {
@@ -29,59 +34,106 @@ __device__ __forceinline__ u32x4 moe_widen(uint32_t lo, uint32_t hi) {
     return v;
 }
 
-// A step of 128 columns of RT row tiles and MB activation blocks.
-template <int RT, int MB>
-struct MoeStep {
-    u32x4 w[RT][2], x[MB][2][2];
+// a pointer that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const uint8_t* moe_uniform(const uint8_t* p) {
+    const uint64_t v = reinterpret_cast<uintptr_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
 
-    // wb: the tiles' first rows, xb: the activations, both the wave's; wo, xo: the lane's rows, bytes from there.  pieces: 16-column pieces
-    // a row; a piece beyond the row's end is the last one again.  live: all ones, or 0 where there is nothing to load: the loads of all
-    // lanes go to the first bytes then, since a load that may not be issued would make every wait one for all loads.
-    __device__ __forceinline__ void load(const uint8_t* const (&wb)[RT], uint32_t wo, const uint8_t* xb, const uint32_t (&xo)[MB], int blocks,
-                                         int step, int pieces, uint32_t live = ~0u) {
-        const int g = lane_id() >> 4;
-        uint32_t p[2];
+// Stages of 128 columns of RT 16-row tiles of weights and of 4 * XU rows of activations.
+// Columns: lane (r, g) takes the 16-byte pieces g and 4 + g of its weight row, codes 64 h + 16 g + 8 t .. + 7 for instruction (h, t), and
+// of its activations' row the same columns, piece 8 h + 2 g + t.
+template <int RT, int XU>
+struct MoeStages {
+    static constexpr int kRows = 4 * XU, kBlocks = XU < 4 ? 1 : XU / 4;      // activation rows, blocks of 16 columns of the product
+    static constexpr int kLoads = 2 * RT + XU, kBytes = kLoads * 1024;
+    int pieces;                       // 16-column pieces a row
+    uint32_t wo[2];                   // the lane's rows of a tile's loads, bytes from the first row
+    int wp[2], xp[XU];                // ... and its pieces of stage 0
+    int wr[2], xr[4];                 // where its fragments lie in a slot: pieces g and 4 + g; pieces (h, t) at 2 h + t
+
+    __device__ __forceinline__ void init(int columns) {
+        const int l = lane_id(), r = l & 15, g = l >> 4;
+        pieces = columns / 16;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int row = 8 * u + (l >> 3);
+            wo[u] = (uint32_t)(row * columns);
+            wp[u] = (l & 7) ^ (row >> 1);
+        }
+#pragma unroll
+        for (int u = 0; u < XU; u++) xp[u] = (l & 15) ^ (4 * u + (l >> 4) & 15);
+        const int at = r % (kRows < 16 ? kRows : 16);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int piece = 8 * step + 4 * h + g;
-            p[h] = (uint32_t)(piece < pieces ? piece : pieces - 1) * 16;
+            wr[h] = r * 128 + ((4 * h + g) ^ (r >> 1)) * 16;
+#pragma unroll
+            for (int t = 0; t < 2; t++) xr[2 * h + t] = at * 256 + ((8 * h + 2 * g + t) ^ at) * 16;
+        }
+    }
+    // wb: the tiles' first rows; xb, xo: the activations and the lane's rows there, bytes.  A piece beyond a row's end is its last one again.
+    __device__ __forceinline__ void issue(unsigned slot, const uint8_t* const (&wb)[RT], const uint8_t* xb, const uint32_t (&xo)[XU], int step) const {
+        uint32_t p[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int piece = 8 * step + wp[u];
+            p[u] = wo[u] + (uint32_t)(piece < pieces ? piece : pieces - 1) * 16;
         }
 #pragma unroll
         for (int i = 0; i < RT; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) w[i][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wb[i] + ((wo + p[h]) & live)));
+            for (int u = 0; u < 2; u++) dma_1kb_stream_at(moe_uniform(wb[i]), p[u], slot + (2 * i + u) * 1024);
 #pragma unroll
-        for (int j = 0; j < MB; j++)
-            if (j < blocks || MB == 1)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) x[j][h][u] = *reinterpret_cast<const u32x4*>(xb + ((xo[j] + 2 * p[h] + 16 * u) & live));
+        for (int u = 0; u < XU; u++) {
+            const int piece = 16 * step + xp[u];
+            dma_1kb_at(xb, xo[u] + (uint32_t)(piece < 2 * pieces ? piece : 2 * pieces - 1) * 16, slot + (2 * RT + u) * 1024);
+        }
     }
-    // Beyond the row's end the activations are zeros.  (The weights there are the row's last ones again: a NaN among them is in the row's
-    // sum already, and there is no infinity in E4M3.)
-    __device__ __forceinline__ void multiply(f32x4 (&acc)[RT][MB], int blocks, int step, int pieces) const {
+    // Beyond the row's end the activations count as zeros.  (The weights there are the row's last ones again: a NaN among them is in the
+    // row's sum already, and there is no infinity in E4M3.)
+    __device__ __forceinline__ void multiply(const uint8_t* slot, f32x4 (&acc)[RT][kBlocks], int blocks, int step) const {
         const int g = lane_id() >> 4;
+        u32x4 w[RT][2], x[kBlocks][4];
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[i][h] = *reinterpret_cast<const u32x4*>(slot + 2048 * i + wr[h]);
+#pragma unroll
+        for (int j = 0; j < kBlocks; j++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[j][t] = *reinterpret_cast<const u32x4*>(slot + 2048 * RT + 4096 * j + xr[t]);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const bool inside = 8 * step + 4 * h + g < pieces;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int t = 0; t < 2; t++) {
                 u32x4 v[RT];
 #pragma unroll
-                for (int i = 0; i < RT; i++) v[i] = moe_widen(w[i][h][2 * u], w[i][h][2 * u + 1]);
+                for (int i = 0; i < RT; i++) v[i] = moe_widen(w[i][h][2 * t], w[i][h][2 * t + 1]);
 #pragma unroll
-                for (int j = 0; j < MB; j++)
-                    if (j < blocks || MB == 1) {
-                        const u32x4 y = inside ? x[j][h][u] : u32x4{0, 0, 0, 0};
+                for (int j = 0; j < kBlocks; j++)
+                    if (j < blocks || kBlocks == 1) {
+                        const u32x4 y = inside ? x[j][2 * h + t] : u32x4{0, 0, 0, 0};
 #pragma unroll
                         for (int i = 0; i < RT; i++) acc[i][j] = moe_mfma(v[i], y, acc[i][j]);
                     }
             }
         }
-        __builtin_amdgcn_sched_barrier(0);       // steps are not mixed: their temporaries would not fit
     }
 };
+
+// Stage `at` of `total` has landed when at most the younger ones' loads are outstanding.
+template <int DEPTH, int LOADS>
+__device__ __forceinline__ void moe_wait(int at, int total) {
+    if (at + DEPTH <= total) wait_vmcnt<(DEPTH - 1) * LOADS>();
+    else wait_vmcnt_upto((total - 1 - at) * LOADS);
+}
+// All fragments are read: the slot may be filled again.
+__device__ __forceinline__ void moe_slot_read() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // A product's result may be read 12 wait states behind it, counted across branches here: the ties keep products in front of the
 // idle states and uses behind them.
@@ -104,20 +156,37 @@ __device__ __forceinline__ float moe_silu(float v) {
     return v * ((v < 0.0f ? t : 1.0f) / (1.0f + t));
 }
 
+// 16 floats of a row scale: what lane (r, g) multiplies its rows 4 g .. 4 g + 3 with.  Scalar loads: a vector load here would be waited for
+// behind every stage in flight.
+__device__ __forceinline__ f32x4 moe_scales(const float* s, int g) {
+    if (!s) return f32x4{1.f, 1.f, 1.f, 1.f};
+    const __attribute__((address_space(4))) float* const c = (const __attribute__((address_space(4))) float*)s;
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = c[i], b = c[4 + i], d = c[8 + i], e = c[12 + i];
+        v[i] = g & 2 ? (g & 1 ? e : d) : (g & 1 ? b : a);
+    }
+    return v;
+}
+
 // h = bf16( silu(S1 * (gate x)) * (S1 * (up x)) ).  An item is 16 gate rows and their 16 up rows of a part of the plan; `share` of a
-// workgroup's four waves share its columns, step by step in turn, and meet in LDS.  A wave has two steps of 4 KB of weights in flight,
-// from one item into the next.
-// LDS: plan, then the room that it is made in, then in its place [4 waves][2 * MB][64 lanes] f32x4.
-template <int MB, bool CHOOSE>
-__global__ void __launch_bounds__(256, MB == 1 ? 4 : 3) moe_gate_up_kernel(const MoeArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+// workgroup's four waves share its columns, stage by stage in turn, and meet in LDS.  A wave's ring runs from one item into the next.
+// LDS: plan, [4 waves][2 * blocks][64 lanes] f32x4 where waves share, then the rings, and before them in their place the room for the plan.
+template <int XU, int DEPTH, bool CHOOSE>
+__global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
+    using Stages = MoeStages<2, XU>;
+    constexpr int BLOCKS = Stages::kBlocks;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
+    const int share = a.share;
     f32x4* const part = reinterpret_cast<f32x4*>(lds + (size_t)l.dwords * 4);
+    uint8_t* const rings = lds + (size_t)l.dwords * 4 + (share > 1 ? 4 * 2 * BLOCKS * 1024 : 0);
     const int lane = lane_id(), r = lane & 15, g = lane >> 4, wave = wave_id();
     {
-        const MoePlanRoom room = moe_room(lds + (size_t)l.dwords * 4, a.m * a.top_k);
-        moe_make_plan<MB, CHOOSE>(a, l, room, plan);
+        const MoePlanRoom room = moe_room(rings, a.m * a.top_k);
+        moe_make_plan<Stages::kRows, CHOOSE>(a, l, room, plan);
         if (blockIdx.x == 0) {       // for the second launch, and the caller
             for (int i = (int)threadIdx.x; i < l.dwords; i += 256) a.plan[i] = plan[i];
             if (CHOOSE)
@@ -126,215 +195,194 @@ __global__ void __launch_bounds__(256, MB == 1 ? 4 : 3) moe_gate_up_kernel(const
         __syncthreads();
     }
     const int tiles = a.inner / 16, items = __builtin_amdgcn_readfirstlane(plan[0]) * tiles;
-    const int pieces = a.hidden / 16, steps = (a.hidden + 127) / 128, share = a.share;
-    const int sharer = wave % share, stride = (int)gridDim.x * (4 / share);
-    const int mine = ((steps - 1) / share + 2) / 2 * 2;        // steps of a wave and item, beyond the last: the last one again, times zeros
+    const int steps = (a.hidden + 127) / 128, sharer = wave % share, stride = (int)gridDim.x * (4 / share);
+    const int first = (int)blockIdx.x * (4 / share) + wave / share;
+    const int of_item = (steps - 1 - sharer) / share + 1;       // stages of an item (there are more steps than sharers)
+    const int total = first < items ? ((items - 1 - first) / stride + 1) * of_item : 0;
+    Stages stages;
+    stages.init(a.hidden);
+    uint8_t* const ring = rings + wave * (DEPTH * Stages::kBytes);
+    const unsigned ring_at = lds_addr(ring);
 
-    struct Item {
-        const uint8_t* wb[2];
-        uint32_t xo[MB], live;
-        int row, first, tile, count, blocks;      // row of W1's rows of all experts: below 2^31
-    };
-    auto find = [&](int item) __attribute__((always_inline)) {
-        Item t;
-        t.live = item < items ? ~0u : 0u;
-        const int at = item < items ? item : 0, which = at / tiles;
-        t.tile = at - which * tiles;
-        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]);
-        const int e = packed & 0xffff;
-        t.count = packed >> 16;
-        t.blocks = (t.count + 15) / 16;
-        t.first = l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
-        t.row = e * 2 * a.inner + t.tile * 16;
-        t.wb[0] = a.W1 + (size_t)t.row * a.hidden;
-        t.wb[1] = t.wb[0] + (size_t)a.inner * a.hidden;
+    // ---- what to load next ----
+    const uint8_t* wb[2] = {};
+    uint32_t xo[XU] = {};
+    int next_item = first, next_step = sharer, next_slot = 0, issued = 0;
+    auto find = [&]() __attribute__((always_inline)) {
+        const int which = next_item / tiles, tile = next_item - which * tiles;
+        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]), e = packed & 0xffff, count = packed >> 16;
+        const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
+        wb[0] = a.W1 + ((size_t)e * 2 * a.inner + tile * 16) * a.hidden;
+        wb[1] = wb[0] + (size_t)a.inner * a.hidden;
 #pragma unroll
-        for (int j = 0; j < MB; j++)
-            t.xo[j] = (uint32_t)plan[t.first + (16 * j + r < t.count ? 16 * j + r : t.count - 1)] / (uint32_t)a.top_k * (uint32_t)(a.hidden * 2);
-        return t;
+        for (int u = 0; u < XU; u++) {
+            const int row = 4 * u + g;
+            xo[u] = (uint32_t)rows[row < count ? row : count - 1] / (uint32_t)a.top_k * (uint32_t)(a.hidden * 2);
+        }
     };
-    MoeStep<2, MB> s0, s1;
-    f32x4 acc[2][MB];
-    const uint32_t wo = (uint32_t)(r * a.hidden);
-    auto load = [&](MoeStep<2, MB>& s, const Item& t, int i) __attribute__((always_inline)) {
-        const int step = sharer + i * share;
-        s.load(t.wb, wo, a.X, t.xo, t.blocks, step < steps ? step : steps - 1, pieces, t.live);
+    auto issue = [&]() __attribute__((always_inline)) {
+        stages.issue(ring_at + next_slot * Stages::kBytes, wb, a.X, xo, next_step);
+        next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
+        issued++;
+        next_step += share;
+        if (next_step >= steps) {
+            next_step = sharer;
+            next_item += stride;
+            if (issued < total) find();
+        }
     };
-    auto multiply = [&](const MoeStep<2, MB>& s, const Item& t, int i) __attribute__((always_inline)) {
-        s.multiply(acc, t.blocks, sharer + i * share, pieces);
-    };
-
-    if (items == 0) return;
-    int item = (int)blockIdx.x * (4 / share) + wave / share;
-    Item now = find(item);
-    load(s0, now, 0);
-    load(s1, now, 1);
+    if (total > 0) {
+        find();
+        for (int d = 0; d < DEPTH && d < total; d++) issue();
+    }
+    int at = 0, slot = 0, item = first;
     for (int round = (int)blockIdx.x * (4 / share); round < items; round += stride, item += stride) {
-        const Item next = find(item + stride);
-        f32x4 scale[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};      // loaded here, in front of the next item's steps
-        if (a.S1) {
-            using f32x4_at4 = f32x4 __attribute__((aligned(4)));
-            scale[0] = *reinterpret_cast<const f32x4_at4*>(a.S1 + now.row + 4 * g);
-            scale[1] = *reinterpret_cast<const f32x4_at4*>(a.S1 + now.row + a.inner + 4 * g);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < MB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        int i = 0;
-        for (; i + 2 < mine; i += 2) {
-            multiply(s0, now, i);
-            load(s0, now, i + 2);
-            multiply(s1, now, i + 1);
-            load(s1, now, i + 3);
-        }
-        multiply(s0, now, i);
-        load(s0, next, 0);
-        multiply(s1, now, i + 1);
-        load(s1, next, 1);
-        moe_settle(acc);
-        auto finish = [&](f32x4 gate, f32x4 up, int j) __attribute__((always_inline)) {
-            if (!now.live || 16 * j + r >= now.count) return;
-            gate *= scale[0];
-            up *= scale[1];
-            const u32x2 o = {pack_bf16x2(moe_silu(gate[0]) * up[0], moe_silu(gate[1]) * up[1]),
-                             pack_bf16x2(moe_silu(gate[2]) * up[2], moe_silu(gate[3]) * up[3])};
-            *reinterpret_cast<u32x2*>(a.H + ((size_t)plan[now.first + 16 * j + r] * a.inner + now.tile * 16 + 4 * g) * 2) = o;
-        };
-        if (share == 1) {
-#pragma unroll
-            for (int j = 0; j < MB; j++) finish(acc[0][j], acc[1][j], j);
-        } else {
+        f32x4 acc[2][BLOCKS];
+        int count = 0, blocks = 0, entry = 0, tile = 0, row = 0;       // row of W1's rows of all experts: below 2^31
+        if (item < items) {
+            const int which = item / tiles;
+            tile = item - which * tiles;
+            const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]);
+            count = packed >> 16;
+            blocks = (count + 15) / 16;
+            entry = l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
+            row = (packed & 0xffff) * 2 * a.inner + tile * 16;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int j = 0; j < MB; j++) part[(wave * 2 * MB + i * MB + j) * 64 + lane] = acc[i][j];
+                for (int j = 0; j < BLOCKS; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int step = sharer; step < steps; step += share, at++) {
+                moe_wait<DEPTH, Stages::kLoads>(at, total);
+                stages.multiply(ring + slot * Stages::kBytes, acc, blocks, step);
+                slot = slot + 1 == DEPTH ? 0 : slot + 1;
+                moe_slot_read();
+                if (issued < total) issue();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            moe_settle(acc);
+        }
+        auto finish = [&](f32x4 gate, f32x4 up, int j) __attribute__((always_inline)) {
+            gate *= moe_scales(a.S1 ? a.S1 + row : nullptr, g);
+            up *= moe_scales(a.S1 ? a.S1 + row + a.inner : nullptr, g);
+            const u32x2 o = {pack_bf16x2(moe_silu(gate[0]) * up[0], moe_silu(gate[1]) * up[1]),
+                             pack_bf16x2(moe_silu(gate[2]) * up[2], moe_silu(gate[3]) * up[3])};
+            if (16 * j + r < count) *reinterpret_cast<u32x2*>(a.H + ((size_t)plan[entry + 16 * j + r] * a.inner + tile * 16 + 4 * g) * 2) = o;
+        };
+        if (share == 1) {
+#pragma unroll
+            for (int j = 0; j < BLOCKS; j++)
+                if (j < blocks) finish(acc[0][j], acc[1][j], j);
+        } else {
+            if (item < items)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < BLOCKS; j++) part[(wave * 2 * BLOCKS + i * BLOCKS + j) * 64 + lane] = acc[i][j];
             __syncthreads();
-            const f32x4* const p = part + (wave - sharer) * 2 * MB * 64 + lane;
-            for (int j = sharer; j < now.blocks; j += share) {
-                f32x4 gate = p[j * 64], up = p[(MB + j) * 64];
+            const f32x4* const p = part + (wave - sharer) * 2 * BLOCKS * 64 + lane;
+            for (int j = sharer; j < blocks; j += share) {
+                f32x4 gate = p[j * 64], up = p[(BLOCKS + j) * 64];
 #pragma unroll 1
                 for (int w = 1; w < share; w++) {
-                    gate += p[(w * 2 * MB + j) * 64];
-                    up += p[(w * 2 * MB + MB + j) * 64];
+                    gate += p[(w * 2 * BLOCKS + j) * 64];
+                    up += p[(w * 2 * BLOCKS + BLOCKS + j) * 64];
                 }
                 finish(gate, up, j);
             }
             __syncthreads();
         }
-        now = next;
     }
 }
 
-// D = bf16( sum over experts of weight * S2 * (W2 h) ): a workgroup has 16 rows of hidden for all tokens, its waves share the steps of all
-// parts, in one range each, DEPTH steps of 2 KB of weights in flight.  A wave adds a part's product, scaled, to sums of its own - [tokens][16 rows]
-// in LDS, where no other wave and no second lane writes -, the waves' sums are added in wave order: no atomics, one order.
-// LDS: plan, S2 of the tile [parts][16], then [waves][m][16] floats.
-template <int MB, int DEPTH, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, MB == 1 ? 4 : WAVES / 4) moe_down_kernel(const MoeArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+// D = bf16( sum over experts of weight * S2 * (W2 h) ): a workgroup has 16 rows of hidden for all tokens, its waves share the stages of all
+// parts, in one range each.  A wave adds a part's product, scaled, to sums of its own - [tokens][16 rows] in LDS, where no other wave and
+// no second lane writes -, the waves' sums are added in wave order: no atomics, one order.
+// LDS: plan, S2 of the tile [parts][16], sums [waves][m][16], the rings.
+template <int XU, int DEPTH, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
+    using Stages = MoeStages<1, XU>;
+    constexpr int BLOCKS = Stages::kBlocks;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
     float* const scales = reinterpret_cast<float*>(lds + (size_t)l.dwords * 4);
-    float* const total = scales + l.most * 16;
+    float* const sums = scales + l.most * 16;
     const int tid = (int)threadIdx.x, lane = lane_id(), r = lane & 15, g = lane >> 4, wave = wave_id();
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(sums + WAVES * a.m * 16) + wave * (DEPTH * Stages::kBytes);
+    const unsigned ring_at = lds_addr(ring);
     const int tile = xcd_order((int)blockIdx.x, (int)gridDim.x);
     for (int i = tid * 4; i < l.dwords; i += 64 * WAVES * 4) *reinterpret_cast<i32x4*>(plan + i) = *reinterpret_cast<const i32x4*>(a.plan + i);
-    float* const own = total + wave * a.m * 16;
+    float* const own = sums + wave * a.m * 16;
     for (int i = lane; i < a.m * 16; i += 64) own[i] = 0.0f;
     __syncthreads();
-    const int parts = __builtin_amdgcn_readfirstlane(plan[0]), pieces = a.inner / 16, steps = (a.inner + 127) / 128;
-    auto scale_of = [&](int i) {      // row i % 16 of part i / 16
-        return a.S2 ? a.S2[(size_t)(plan[l.parts_at + (i >> 4)] & 0xffff) * a.hidden + tile * 16 + (i & 15)] : 1.0f;
-    };
-    const float first_scale = tid < parts * 16 ? scale_of(tid) : 1.0f;
+    const int parts = __builtin_amdgcn_readfirstlane(plan[0]), steps = (a.inner + 127) / 128;
+    for (int i = tid; i < parts * 16; i += 64 * WAVES)      // row i % 16 for part i / 16
+        scales[i] = a.S2 ? a.S2[(size_t)(plan[l.parts_at + (i >> 4)] & 0xffff) * a.hidden + tile * 16 + (i & 15)] : 1.0f;
 
-    const long long all = (long long)parts * steps;
-    const long long begin = all * wave / WAVES;
-    const int steps_here = (int)(all * (wave + 1) / WAVES - begin);
-    // ---- where to load next ----
+    const long long all = (long long)parts * steps, begin = all * wave / WAVES;
+    const int total = (int)(all * (wave + 1) / WAVES - begin);
+    Stages stages;
+    stages.init(a.inner);
+    // ---- what to load next ----
     const uint8_t* wb[1] = {};
-    uint32_t xo[MB] = {};
-    const uint32_t wo = (uint32_t)(r * a.inner);
-    int which = (int)(begin / steps), step = (int)(begin - (long long)which * steps), blocks = 0;
+    uint32_t xo[XU] = {};
+    int next_part = (int)(begin / steps), next_step = (int)(begin - (long long)next_part * steps), next_slot = 0, issued = 0;
+    int part = next_part, step = next_step;                  // what to multiply next
     auto find = [&]() __attribute__((always_inline)) {
-        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]), e = packed & 0xffff, count = packed >> 16;
-        const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
-        blocks = (count + 15) / 16;
+        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + next_part]), e = packed & 0xffff, count = packed >> 16;
+        const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + next_part]);
         wb[0] = a.W2 + ((size_t)e * a.hidden + tile * 16) * a.inner;
 #pragma unroll
-        for (int j = 0; j < MB; j++) xo[j] = (uint32_t)rows[16 * j + r < count ? 16 * j + r : count - 1] * (uint32_t)(a.inner * 2);
-    };
-    MoeStep<1, MB> s[DEPTH];
-    auto load = [&](MoeStep<1, MB>& to) __attribute__((always_inline)) {
-        to.load(wb, wo, a.H, xo, blocks, step, pieces);
-        if (++step == steps) {
-            step = 0;
-            if (++which < parts) find();
+        for (int u = 0; u < XU; u++) {
+            const int row = 4 * u + g;
+            xo[u] = (uint32_t)rows[row < count ? row : count - 1] * (uint32_t)(a.inner * 2);
         }
     };
-    // ---- where to multiply ----
-    int part = which, at = step, part_count = 0, part_first = 0;
-    f32x4 acc[1][MB];
-    auto open = [&]() __attribute__((always_inline)) {
-        part_count = __builtin_amdgcn_readfirstlane(plan[l.parts_at + part]) >> 16;
-        part_first = __builtin_amdgcn_readfirstlane(plan[l.first_at + part]);
-#pragma unroll
-        for (int j = 0; j < MB; j++) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto issue = [&]() __attribute__((always_inline)) {
+        stages.issue(ring_at + next_slot * Stages::kBytes, wb, a.H, xo, next_step);
+        next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
+        issued++;
+        if (++next_step == steps) {
+            next_step = 0;
+            next_part++;
+            if (issued < total) find();
+        }
     };
-    auto close = [&]() __attribute__((always_inline)) {
+    if (total > 0) {
+        find();
+        for (int d = 0; d < DEPTH && d < total; d++) issue();
+    }
+    __syncthreads();                                         // the scales
+    for (int at = 0, slot = 0; at < total; part++, step = 0) {
+        const int count = __builtin_amdgcn_readfirstlane(plan[l.parts_at + part]) >> 16, blocks = (count + 15) / 16;
+        const int first = __builtin_amdgcn_readfirstlane(plan[l.first_at + part]);
+        f32x4 acc[1][BLOCKS];
+#pragma unroll
+        for (int j = 0; j < BLOCKS; j++) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (; step < steps && at < total; step++, at++) {
+            moe_wait<DEPTH, Stages::kLoads>(at, total);
+            stages.multiply(ring + slot * Stages::kBytes, acc, blocks, step);
+            slot = slot + 1 == DEPTH ? 0 : slot + 1;
+            moe_slot_read();
+            if (issued < total) issue();
+            __builtin_amdgcn_sched_barrier(0);
+        }
         moe_settle(acc);
         const f32x4 scale = *reinterpret_cast<const f32x4*>(scales + part * 16 + 4 * g);
 #pragma unroll
-        for (int j = 0; j < MB; j++)
-            if (16 * j + r < part_count) {
-                const int entry = part_first + 16 * j + r, token = plan[l.rows_at + entry] / a.top_k;
+        for (int j = 0; j < BLOCKS; j++)
+            if (16 * j + r < count) {
+                const int entry = first + 16 * j + r, token = (int)((uint32_t)plan[l.rows_at + entry] / (uint32_t)a.top_k);
                 const float weight = __uint_as_float((uint32_t)plan[l.weights_at + entry]);
                 f32x4* const sum = reinterpret_cast<f32x4*>(own + token * 16 + 4 * g);
                 *sum += acc[0][j] * scale * weight;
             }
-    };
-    auto multiply = [&](MoeStep<1, MB>& from) __attribute__((always_inline)) {
-        from.multiply(acc, (part_count + 15) / 16, at, pieces);
-        if (++at == steps) {
-            close();
-            at = 0;
-            if (++part < parts) open();
-        }
-    };
-    if (steps_here > 0) {
-        find();
-        open();
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (d < steps_here) load(s[d]);
-    }
-    if (tid < parts * 16) scales[tid] = first_scale;
-    for (int i = tid + 64 * WAVES; i < parts * 16; i += 64 * WAVES) scales[i] = scale_of(i);
-    __syncthreads();
-    if (steps_here > 0) {
-        int left = steps_here;
-        for (; left >= 2 * DEPTH; left -= DEPTH)
-#pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                multiply(s[d]);
-                load(s[d]);
-            }
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            if (d < left) multiply(s[d]);
-            if (d + DEPTH < left) load(s[d]);
-        }
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++)
-            if (d + DEPTH < left) multiply(s[d]);
-        if (at != 0) close();
     }
     __syncthreads();
     for (int i = tid; i < a.m * 4; i += 64 * WAVES) {
         const int token = i >> 2, c = i & 3;
-        f32x4 v = *reinterpret_cast<const f32x4*>(total + token * 16 + 4 * c);
-        for (int w = 1; w < WAVES; w++) v += *reinterpret_cast<const f32x4*>(total + (w * a.m + token) * 16 + 4 * c);
+        f32x4 v = *reinterpret_cast<const f32x4*>(sums + token * 16 + 4 * c);
+        for (int w = 1; w < WAVES; w++) v += *reinterpret_cast<const f32x4*>(sums + (w * a.m + token) * 16 + 4 * c);
         const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
         *reinterpret_cast<u32x2*>(a.D + (size_t)token * a.hidden + tile * 16 + 4 * c) = o;
     }

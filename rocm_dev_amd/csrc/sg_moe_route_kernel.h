@@ -186,7 +186,7 @@ __device__ __forceinline__ MoePlanRoom moe_room(uint8_t* at, int pairs) {
 }
 
 // Who goes where, by a workgroup of 256 threads: the choices (made here, or the caller's) into the room, the plan into `plan`, both LDS.
-template <int MB, bool CHOOSE>
+template <int COLS, bool CHOOSE>
 __device__ __forceinline__ void moe_make_plan(const MoeArgs& a, const MoePlanLayout& l, const MoePlanRoom& room, int32_t* plan) {
     const int tid = (int)threadIdx.x, pairs = a.m * a.top_k;
     if (CHOOSE) {
@@ -210,7 +210,7 @@ __device__ __forceinline__ void moe_make_plan(const MoeArgs& a, const MoePlanLay
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         count[i] = __popc(room.tokens[4 * tid + 2 * i]) + __popc(room.tokens[4 * tid + 2 * i + 1]);
-        parts += (count[i] + 16 * MB - 1) / (16 * MB);
+        parts += (count[i] + COLS - 1) / COLS;
         entries += count[i];
     }
     const int own_parts = parts, own_entries = entries, lane = lane_id(), wave = wave_id();
@@ -227,8 +227,8 @@ __device__ __forceinline__ void moe_make_plan(const MoeArgs& a, const MoePlanLay
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         room.place[2 * tid + i] = first;
-        for (int left = count[i]; left > 0; left -= 16 * MB) {
-            const int here = left < 16 * MB ? left : 16 * MB;
+        for (int left = count[i]; left > 0; left -= COLS) {
+            const int here = left < COLS ? left : COLS;
             plan[l.parts_at + part] = (2 * tid + i) | here << 16;
             plan[l.first_at + part] = first;
             part++;

@@ -7,27 +7,31 @@
 
 namespace sg {
 
-template <int FLAGS, int NF, int MF, int DEPTH>
-static int launch_build(Int4Args& a, int waves, hipStream_t stream) {
-    a.n_groups = (a.tiles - 1) / NF + 1;
-    a.m_groups = (a.m - 1) / (16 * MF) + 1;
+// kw groups of NW waves share K
+template <int FLAGS, int NF, int XU, int NW>
+static int launch_build(Int4Args& a, int kw, hipStream_t stream) {
+    a.n_groups = (a.tiles - 1) / (NF * NW) + 1;
+    a.m_groups = (a.m - 1) / (4 * XU) + 1;
     const long long grid = (long long)a.n_groups * a.m_groups;
     if (grid > INT_MAX) return SG_BAD_ARGUMENT;
-    const size_t lds = waves > 1 ? (size_t)waves * NF * MF * 1024 : 0;
-    auto* const kernel = int4_gemm_kernel<SG_GPS, FLAGS, NF, MF, DEPTH>;
+    constexpr int MF = XU < 4 ? 1 : XU / 4;
+    const size_t acts = (size_t)kw * (NW > 1 ? 2 : 1) * XU * 1024, sums = kw > 1 ? (size_t)kw * NW * NF * MF * 1024 : 0;
+    const size_t lds = acts > sums ? acts : sums;
+    auto* const kernel = int4_gemm_kernel<SG_GPS, FLAGS, NF, XU, NW>;
     static LdsGranted granted;
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, granted)) return rc;
-    kernel<<<(unsigned)grid, 64 * waves, lds, stream>>>(a);
+    kernel<<<(unsigned)grid, 64 * kw * NW, lds, stream>>>(a);
     return report_hip("int4_gemm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
 template <int FLAGS>
 static int launch_flags(Int4Args& a, int cu_count, hipStream_t stream) {
-    (void)cu_count;
-    const int waves = a.steps >= 16 ? 8 : a.steps >= 8 ? 4 : a.steps >= 4 ? 2 : 1;
-    if (a.m <= 16) return launch_build<FLAGS, 2, 1, 2>(a, waves, stream);
-    if (a.m <= 32) return launch_build<FLAGS, 2, 2, 2>(a, waves, stream);
-    return launch_build<FLAGS, 2, 4, 1>(a, waves, stream);
+    const int share = a.steps >= 16 ? 8 : a.steps >= 8 ? 4 : a.steps >= 4 ? 2 : 1;
+    if (a.m <= 4) return a.tiles >= 4 * cu_count ? launch_build<FLAGS, 2, 1, 1>(a, share, stream) : launch_build<FLAGS, 1, 1, 1>(a, share, stream);
+    if (a.m <= 8) return a.tiles >= 4 * cu_count ? launch_build<FLAGS, 2, 2, 1>(a, share, stream) : launch_build<FLAGS, 1, 2, 1>(a, share, stream);
+    if (a.m <= 16) return a.tiles >= 4 * cu_count ? launch_build<FLAGS, 2, 4, 1>(a, share, stream) : launch_build<FLAGS, 1, 4, 1>(a, share, stream);
+    if (a.m <= 32) return a.tiles >= 4 * cu_count ? launch_build<FLAGS, 2, 8, 4>(a, share < 2 ? share : 2, stream) : launch_build<FLAGS, 2, 8, 2>(a, share < 4 ? share : 4, stream);
+    return a.tiles >= 4 * cu_count ? launch_build<FLAGS, 2, 16, 4>(a, share < 2 ? share : 2, stream) : launch_build<FLAGS, 2, 16, 2>(a, share < 4 ? share : 4, stream);
 }
 
 #define SG_INT4_CAT_(a, b) a##b

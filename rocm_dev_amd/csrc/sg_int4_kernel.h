@@ -8,9 +8,10 @@
 // The correction cancels: both of its terms are up to 16 * sum|A| / |sum A (q - z)| times the result, about 50 at
 // groups of 128 of noise, so that 2^-24 of fp32 becomes 2^-18 of a group's sum, against 2^-9 of the output's rounding.
 //
-// A wave takes NF 16-row weight tiles and MF 16-row activation tiles and walks a part of K in steps of 128 columns; operands go
-// from memory to registers as they lie, DEPTH steps in flight.  The waves of a workgroup share K by steps and meet in LDS,
-// partial sums added in wave order: the result does not depend on which wave is first.
+// A wave takes NF 16-row weight tiles and all rows of an activation tile, and walks a part of K in steps of 128 columns.  Weights go from
+// memory to registers as they lie, two steps in flight.  Activations come by 4 rows x 256 bytes a load, whole lines, and go through
+// LDS: NW waves with weight tiles of their own share them (and a barrier a step), KW such groups share K by steps and meet in LDS,
+// partial sums added in their order: the result does not depend on which wave is first.
 #pragma once
 
 #include "sg_int4.h"
@@ -82,15 +83,19 @@ __device__ __forceinline__ void int4_store4(const Int4Args& a, int m_idx, int n_
     }
 }
 
-// FLAGS: SG_INT4_ZEROS, SG_INT4_F16_SCALES
-template <int GPS, int FLAGS, int NF, int MF, int DEPTH>
+// FLAGS: SG_INT4_ZEROS, SG_INT4_F16_SCALES.  The tile has 4 * XU activation rows.
+// LDS: [KW][NW > 1 ? 2 : 1][XU KB] activations, then in its place [KW][NW][NF * MF][64 lanes] f32x4.
+template <int GPS, int FLAGS, int NF, int XU, int NW>
 __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     constexpr bool ZEROS = FLAGS & SG_INT4_ZEROS, F16 = FLAGS & SG_INT4_F16_SCALES;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];     // [waves][NF * MF][64 lanes] f32x4
+    constexpr int MF = XU < 4 ? 1 : XU / 4, LOADS = XU / NW, ROWS = 4 * XU < 16 ? 4 * XU : 16, BUFFERS = NW > 1 ? 2 : 1;
+    static_assert(XU % NW == 0);
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
-    const int wave = wave_id(), waves = (int)(blockDim.x >> 6);
+    const int wave = wave_id(), waves = (int)(blockDim.x >> 6), KW = waves / NW, kg = wave / NW, nw = wave % NW;
     const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
     const int tn = at / a.m_groups, tm = at - tn * a.m_groups;       // neighbours share the weights
+    const int first_tile = (tn * NW + nw) * NF;
 
     // ---- operands of lane (r, g): tiles beyond the last and rows beyond m take the last one again, and are not stored ----
     const uint8_t* wp[NF];
@@ -98,21 +103,29 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     const uint8_t* zp[NF];
 #pragma unroll
     for (int i = 0; i < NF; i++) {
-        const size_t tile = (size_t)(tn * NF + i < a.tiles ? tn * NF + i : a.tiles - 1) * a.steps;
+        const size_t tile = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
         wp[i] = a.P + tile * 1024 + lane * 16;
         sp[i] = a.PS + (tile * 4 + g) * GPS * 8;
         zp[i] = ZEROS ? a.PZ + (tile * 4 + g) * GPS * 4 : nullptr;
     }
-    const uint8_t* xp[MF];
+    // Activations: load u of the tile has rows 4 u .. 4 u + 3, lane l piece l % 16 (8 columns) of row l / 16; in LDS the pieces of row i stand
+    // permuted by i, so that the 16 lanes (r, g) of a fragment's read hit 16 bank groups.
+    const uint8_t* xp[LOADS];
+    uint32_t xw[LOADS], xr[4];
+    const int piece = lane & 15, pieces = a.k / 8;       // k is a multiple of 32
 #pragma unroll
-    for (int j = 0; j < MF; j++) {
-        const int row = (tm * MF + j) * 16 + r < a.m ? (tm * MF + j) * 16 + r : a.m - 1;
-        xp[j] = reinterpret_cast<const uint8_t*>(a.A + (size_t)row * a.k);
+    for (int u = 0; u < LOADS; u++) {
+        const int in = 4 * (nw * LOADS + u) + g, row = tm * 4 * XU + in;
+        xp[u] = reinterpret_cast<const uint8_t*>(a.A + (size_t)(row < a.m ? row : a.m - 1) * a.k);
+        xw[u] = (uint32_t)(in * 256 + (piece ^ (in & 15)) * 16);
     }
-    const int pieces = a.k / 8;       // of 8 columns; k is a multiple of 32
+    const int xrow = r % ROWS;
+#pragma unroll
+    for (int t = 0; t < 4; t++) xr[t] = (uint32_t)(xrow * 256 + ((4 * t + g) ^ xrow) * 16);
+    uint8_t* const xbuf = lds + kg * (BUFFERS * XU * 1024);
 
-    u32x4 w[DEPTH][NF], x[DEPTH][MF][4];
-    uint32_t s[DEPTH][NF][2 * GPS], z[DEPTH][NF][GPS];
+    u32x4 w[2][NF], x[2][LOADS];
+    uint32_t s[2][NF][2 * GPS], z[2][NF][GPS];
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
@@ -122,37 +135,45 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     // `step` is inside the matrix.  A piece of a row beyond its end takes the last piece: its weights' scales are zero.
     auto load = [&](auto dc, int step) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value;
+        const int p = 16 * step + piece;
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xp[u] + (size_t)(p < pieces ? p : pieces - 1) * 16);
 #pragma unroll
         for (int i = 0; i < NF; i++) {
             w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp[i] + (size_t)step * 1024));
             int4_take(s[d][i], sp[i] + (size_t)step * (GPS * 32));
             if (ZEROS) int4_take(z[d][i], zp[i] + (size_t)step * (GPS * 16));
         }
+    };
+    // LDS operations of a wave are carried out in order: with NW = 1 the next step's pieces may be written behind this step's reads.
+    auto share_x = [&](auto dc) __attribute__((always_inline)) {
+        constexpr int d = decltype(dc)::value;
 #pragma unroll
-        for (int j = 0; j < MF; j++)
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int p = 16 * step + 4 * t + g;
-                x[d][j][t] = *reinterpret_cast<const u32x4*>(xp[j] + (size_t)(p < pieces ? p : pieces - 1) * 16);
-            }
+        for (int u = 0; u < LOADS; u++) *reinterpret_cast<u32x4*>(xbuf + (NW > 1 ? d * XU * 1024 : 0) + xw[u]) = x[d][u];
+        if (NW > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
     auto multiply = [&](auto dc) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value;
         constexpr int PER = 4 / GPS;          // instructions a group
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
         const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        const uint8_t* const from = xbuf + (NW > 1 ? d * XU * 1024 : 0);
 #pragma unroll
         for (int q = 0; q < GPS; q++) {
             f32x4 sum[MF], part[NF][MF];
 #pragma unroll
             for (int t = 0; t < PER; t++) {
+                u32x4 y[MF];
 #pragma unroll
-                for (int j = 0; j < MF; j++) sum[j] = mfma_bf16_16x16x32(ones, x[d][j][q * PER + t], t ? sum[j] : zero);
+                for (int j = 0; j < MF; j++) {
+                    y[j] = *reinterpret_cast<const u32x4*>(from + j * 4096 + xr[q * PER + t]);
+                    sum[j] = mfma_bf16_16x16x32(ones, y[j], t ? sum[j] : zero);
+                }
 #pragma unroll
                 for (int i = 0; i < NF; i++) {
                     const u32x4 v = int4_widen(w[d][i][q * PER + t]);
 #pragma unroll
-                    for (int j = 0; j < MF; j++) part[i][j] = mfma_bf16_16x16x32(v, x[d][j][q * PER + t], t ? part[i][j] : zero);
+                    for (int j = 0; j < MF; j++) part[i][j] = mfma_bf16_16x16x32(v, y[j], t ? part[i][j] : zero);
                 }
             }
 #pragma unroll
@@ -168,50 +189,53 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
         __builtin_amdgcn_sched_barrier(0);    // steps are not mixed: their temporaries would not fit
     };
     using D0 = std::integral_constant<int, 0>;
-    using D1 = std::integral_constant<int, 1 % DEPTH>;
-    static_assert(DEPTH <= 2);
+    using D1 = std::integral_constant<int, 1>;
 
-    // Steps wave, wave + waves, ...: `left` of them.
-    int step = wave, left = wave < a.steps ? (a.steps - 1 - wave) / waves + 1 : 0;
+    // Steps kg, kg + KW, ...: `left` of them; a group that has one fewer than another goes through the other's barriers.
+    int step = kg, left = kg < a.steps ? (a.steps - 1 - kg) / KW + 1 : 0;
+    int rounds = NW > 1 ? (a.steps - 1) / KW + 1 : left;
     if (left > 0) load(D0{}, step);
-    if (DEPTH > 1 && left > 1) load(D1{}, step + waves);
-    for (; left >= 2 * DEPTH; left -= DEPTH, step += DEPTH * waves) {
+    if (left > 1) load(D1{}, step + KW);
+    for (; left >= 4; left -= 2, rounds -= 2, step += 2 * KW) {
+        share_x(D0{});
         multiply(D0{});
-        load(D0{}, step + DEPTH * waves);
-        if (DEPTH > 1) {
-            multiply(D1{});
-            load(D1{}, step + (DEPTH + 1) * waves);
-        }
+        load(D0{}, step + 2 * KW);
+        share_x(D1{});
+        multiply(D1{});
+        load(D1{}, step + 3 * KW);
     }
-    // fewer than 2 * DEPTH are left, the first DEPTH of them loaded
-    if (left > 0) {
-        multiply(D0{});
-        if (left > DEPTH) load(D0{}, step + DEPTH * waves);
-        if (DEPTH > 1 && left > 1) multiply(D1{});
-        if (left > DEPTH) multiply(D0{});
-    }
+    // at most three are left, the first two of them loaded
+    if (rounds > 0) share_x(D0{});
+    if (left > 0) multiply(D0{});
+    if (left > 2) load(D0{}, step + 2 * KW);
+    if (rounds > 1) share_x(D1{});
+    if (left > 1) multiply(D1{});
+    if (rounds > 2) share_x(D0{});
+    if (left > 2) multiply(D0{});
+    if (rounds > 3) share_x(D1{});
 
-    // ---- the waves' sums, in wave order ----
+    // ---- the groups' sums, in their order ----
     auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) {
-        const int n_idx = (tn * NF + i) * 16 + 4 * g, m_idx = (tm * MF + j) * 16 + r;
-        if (m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * 16.0f);
+        const int n_idx = (first_tile + i) * 16 + 4 * g, m_idx = tm * 4 * XU + 16 * j + r;
+        if (r < ROWS && m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * 16.0f);
     };
-    if (waves == 1) {
+    if (KW == 1) {
 #pragma unroll
         for (int i = 0; i < NF; i++)
 #pragma unroll
             for (int j = 0; j < MF; j++) finish(acc[i][j], i, j);
         return;
     }
+    __syncthreads();          // the activations' place is taken over
     f32x4* const part = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
-        for (int j = 0; j < MF; j++) part[(wave * NF * MF + i * MF + j) * 64 + lane] = acc[i][j];
+        for (int j = 0; j < MF; j++) part[((kg * NW + nw) * NF * MF + i * MF + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    for (int f = wave; f < NF * MF; f += waves) {
-        f32x4 v = part[f * 64 + lane];
-        for (int u = 1; u < waves; u++) v += part[(u * NF * MF + f) * 64 + lane];
+    for (int f = kg; f < NF * MF; f += KW) {
+        f32x4 v = part[(nw * NF * MF + f) * 64 + lane];
+        for (int u = 1; u < KW; u++) v += part[((u * NW + nw) * NF * MF + f) * 64 + lane];
         finish(v, f / MF, f % MF);
     }
 }

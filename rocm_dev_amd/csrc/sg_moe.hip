@@ -20,14 +20,16 @@ static int launch_choose(const MoeArgs& a, hipStream_t stream) {
 
 constexpr size_t kLdsBytes = 160 * 1024;      // a CU's
 
-template <int XU, int DEPTH, bool CHOOSE>
-static int launch_gate_up(const MoeArgs& a, int cu_count, hipStream_t stream) {
+template <int XU, int DEPTH>
+static size_t gate_up_lds(const MoeArgs& a) {
     using Stages = MoeStages<2, XU>;
-    const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs;
-    const size_t ring = (size_t)4 * DEPTH * Stages::kBytes, room = moe_plan_room(pairs);
-    const size_t lds = (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) +
-                       (room > ring ? room : ring);
-    const long long groups = ((long long)most * (a.inner / 16) * a.share + 3) / 4, at_once = (long long)(kLdsBytes / lds) * cu_count;
+    const size_t ring = (size_t)4 * DEPTH * Stages::kBytes, room = moe_plan_room(a.m * a.top_k);
+    return (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) + (room > ring ? room : ring);
+}
+template <int XU, int DEPTH, bool CHOOSE>
+static int launch_gate_up(const MoeArgs& a, long long groups, int cu_count, hipStream_t stream) {
+    const size_t lds = gate_up_lds<XU, DEPTH>(a);
+    const long long at_once = (long long)(kLdsBytes / lds) * cu_count;
     const unsigned grid = (unsigned)(groups < at_once ? groups : at_once);
     static LdsGranted granted;
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<XU, DEPTH, CHOOSE>), lds, granted)) return rc;
@@ -53,9 +55,16 @@ static int launch_down(const MoeArgs& a, hipStream_t stream) {
 template <int XU, int G, int N>
 static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
     const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
+    const long long items = (long long)most * (a.inner / 16);
     a.share = 1;
-    while (a.share < 4 && (long long)most * (a.inner / 16) * a.share < 16ll * cu_count && steps >= 4 * a.share) a.share *= 2;
-    if (int rc = choose ? launch_gate_up<XU, G, true>(a, cu_count, stream) : launch_gate_up<XU, G, false>(a, cu_count, stream)) return rc;
+    while (a.share < 4 && items * a.share < 16ll * cu_count && steps >= 4 * a.share) a.share *= 2;
+    const long long groups = (items * a.share + 3) / 4;
+    // A few workgroups more than fit at once would take as long again: shorter rings then, if all fit with them.
+    const bool shorter = groups > (long long)(kLdsBytes / gate_up_lds<XU, G>(a)) * cu_count && groups <= (long long)(kLdsBytes / gate_up_lds<XU, 2>(a)) * cu_count;
+    int rc;
+    if (choose) rc = shorter ? launch_gate_up<XU, 2, true>(a, groups, cu_count, stream) : launch_gate_up<XU, G, true>(a, groups, cu_count, stream);
+    else rc = shorter ? launch_gate_up<XU, 2, false>(a, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, groups, cu_count, stream);
+    if (rc) return rc;
     if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, 8>(a, stream);
     if (down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, 8>(a, stream);
     return launch_down<XU, 2, 4>(a, stream);

@@ -21,7 +21,7 @@ struct Int4Layout {
     size_t scales_at, zeros_at, bytes;
 };
 inline bool int4_takes(int n, int k, int group, int flags) {
-    return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && !(flags & ~(SG_INT4_ZEROS | SG_INT4_F16_SCALES));
+    return n > 0 && k > 0 && k <= 1 << 24 && (group == 32 || group == 64 || group == 128) && k % group == 0 && !(flags & ~(SG_INT4_ZEROS | SG_INT4_F16_SCALES));
 }
 inline Int4Layout int4_layout(int n, int k, int group, int flags) {
     Int4Layout l;

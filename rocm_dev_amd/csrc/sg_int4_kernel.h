@@ -3,37 +3,48 @@
 // What bounds it is the stream of weights, half a byte a value and the groups' scales.  The matrix instruction takes bf16, so the
 // codes are widened on the way: 1 + q / 16 by a rotation and a mask a pair (sg_int4.h), and the product of a group is set right behind it,
 //     sum A * (q - z) = 16 * ( sum A * (1 + q / 16)  -  (1 + z / 16) * sum A ),
-// the activations' own sum by the same instruction on a matrix of ones, once for all tiles of a wave.  Seven vector operations a
-// dword of eight codes: a third of the clocks at the rate at which the memory delivers.
+// the activations' own sum by the same instruction on a matrix of ones, once for all tiles of a wave - or, where waves share the activations,
+// by those that bring them.  Seven vector operations a dword of eight codes: a third of the clocks at the rate at which the memory
+// delivers, up to 16 rows.  Beyond, the two fp32 multiply-adds an output and group are what the vector units are busy with.
 // The correction cancels: both of its terms are up to 16 * sum|A| / |sum A (q - z)| times the result, about 50 at
 // groups of 128 of noise, so that 2^-24 of fp32 becomes 2^-18 of a group's sum, against 2^-9 of the output's rounding.
 //
 // A wave takes NF 16-row weight tiles and all rows of an activation tile, and walks a part of K in steps of 128 columns.  Weights go from
-// memory to registers as they lie, two steps in flight.  Activations come by 4 rows x 256 bytes a load, whole lines, and go through
+// memory to registers as they lie, four steps in flight.  Activations come by 4 rows x 256 bytes a load, whole lines, and go through
 // LDS: NW waves with weight tiles of their own share them (and a barrier a step), KW such groups share K by steps and meet in LDS,
 // partial sums added in their order: the result does not depend on which wave is first.
 #pragma once
+
+#include <type_traits>
 
 #include "sg_int4.h"
 
 namespace sg {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_vec __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4 mfma_bf16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// eight codes of a dword as 1 + q / 16
-__device__ __forceinline__ u32x4 int4_widen(uint32_t d) {
-    u32x4 v;
+// eight codes of a dword as 1 + q / 16; `ones` are two bf16 ones in a vector register, so that mask and ones are one instruction
+// (it takes one constant from elsewhere)
+__device__ __forceinline__ u32x4 int4_widen(uint32_t d, uint32_t ones) {
+    return u32x4{(d & 0x00780078u) | ones, (d >> 4 & 0x00780078u) | ones, (d >> 8 & 0x00780078u) | ones,
+                 (__builtin_amdgcn_alignbit(d, d, 12) & 0x00780078u) | ones};
+}
+// the sum of eight bf16
+__device__ __forceinline__ float int4_sum8(u32x4 v, uint32_t ones) {
+    const bf16x2_vec one = __builtin_bit_cast(bf16x2_vec, ones);
+    float sum = 0.0f;
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-        const uint32_t at = p ? __builtin_amdgcn_alignbit(d, d, 4 * p) : d;
-        v[p] = (at & 0x00780078u) | 0x3f803f80u;
+    for (int c = 0; c < 4; c++) {
+        const uint32_t two = v[c];          // (a bit cast of v[c] itself takes element 0)
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_vec, two), one, sum, false);
     }
-    return v;
+    return sum;
 }
 // four scales of two dwords, four zeros of one
 template <bool F16>
@@ -83,13 +94,31 @@ __device__ __forceinline__ void int4_store4(const Int4Args& a, int m_idx, int n_
     }
 }
 
+// a step's activations in LDS, and where waves share them, the sums of their groups
+__host__ __device__ constexpr int int4_buffer(int gps, int xu, int nw) { return xu * 1024 + (nw > 1 ? (gps * xu * 16 + 1023) / 1024 * 1024 : 0); }
+
+// the sum over 4 * N neighbouring lanes, in all of them
+template <int N>
+__device__ __forceinline__ float int4_over_lanes(float v) {
+    auto from = [&](float w, auto ctrl) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(w), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    v += from(v, std::integral_constant<int, 0xb1>{});                  // the lane beside it, then the pair beside it
+    v += from(v, std::integral_constant<int, 0x4e>{});
+    if (N > 1) v += from(v, std::integral_constant<int, 0x141>{});      // mirrored in 8 and in 16 lanes: the other half
+    if (N > 2) v += from(v, std::integral_constant<int, 0x140>{});
+    return v;
+}
+
 // FLAGS: SG_INT4_ZEROS, SG_INT4_F16_SCALES.  The tile has 4 * XU activation rows.
-// LDS: [KW][NW > 1 ? 2 : 1][XU KB] activations, then in its place [KW][NW][NF * MF][64 lanes] f32x4.
-template <int GPS, int FLAGS, int NF, int XU, int NW>
+// LDS: [KW][NW > 1 ? 2 : 1][XU KB activations, NW > 1: [4 * XU][GPS] sums of groups], then in its place [KW][NW][NF * MF][64 lanes] f32x4.
+template <int GPS, int FLAGS, int NF, int XU, int NW, int DX>
 __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     constexpr bool ZEROS = FLAGS & SG_INT4_ZEROS, F16 = FLAGS & SG_INT4_F16_SCALES;
-    constexpr int MF = XU < 4 ? 1 : XU / 4, LOADS = XU / NW, ROWS = 4 * XU < 16 ? 4 * XU : 16, BUFFERS = NW > 1 ? 2 : 1;
-    static_assert(XU % NW == 0);
+    constexpr int MF = XU < 4 ? 1 : XU / 4, LOADS = XU / NW, ROWS = 4 * XU < 16 ? 4 * XU : 16, PER = 4 / GPS;     // PER: instructions a group
+    constexpr bool SHARED = NW > 1;
+    constexpr int BUFFER = int4_buffer(GPS, XU, NW);
+    static_assert(XU % NW == 0 && (DX == 2 || DX == 4));
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int wave = wave_id(), waves = (int)(blockDim.x >> 6), KW = waves / NW, kg = wave / NW, nw = wave % NW;
@@ -97,122 +126,146 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     const int tn = at / a.m_groups, tm = at - tn * a.m_groups;       // neighbours share the weights
     const int first_tile = (tn * NW + nw) * NF;
 
-    // ---- operands of lane (r, g): tiles beyond the last and rows beyond m take the last one again, and are not stored ----
-    const uint8_t* wp[NF];
-    const uint8_t* sp[NF];
-    const uint8_t* zp[NF];
+    // ---- operands: tiles beyond the last and rows beyond m take the last one again, and are not stored ----
+    size_t tile_at[NF];               // the tile's first step
 #pragma unroll
-    for (int i = 0; i < NF; i++) {
-        const size_t tile = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
-        wp[i] = a.P + tile * 1024 + lane * 16;
-        sp[i] = a.PS + (tile * 4 + g) * GPS * 8;
-        zp[i] = ZEROS ? a.PZ + (tile * 4 + g) * GPS * 4 : nullptr;
-    }
+    for (int i = 0; i < NF; i++) tile_at[i] = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
     // Activations: load u of the tile has rows 4 u .. 4 u + 3, lane l piece l % 16 (8 columns) of row l / 16; in LDS the pieces of row i stand
     // permuted by i, so that the 16 lanes (r, g) of a fragment's read hit 16 bank groups.
-    const uint8_t* xp[LOADS];
-    uint32_t xw[LOADS], xr[4];
-    const int piece = lane & 15, pieces = a.k / 8;       // k is a multiple of 32
+    const uint8_t* const xb = reinterpret_cast<const uint8_t*>(a.A + (size_t)tm * 4 * XU * a.k);
+    uint32_t xo[LOADS], xw[LOADS], xr[4];
+    const int piece = lane & 15, pieces = a.k / 8, rows_left = a.m - tm * 4 * XU;       // k is a multiple of 32
 #pragma unroll
     for (int u = 0; u < LOADS; u++) {
-        const int in = 4 * (nw * LOADS + u) + g, row = tm * 4 * XU + in;
-        xp[u] = reinterpret_cast<const uint8_t*>(a.A + (size_t)(row < a.m ? row : a.m - 1) * a.k);
-        xw[u] = (uint32_t)(in * 256 + (piece ^ (in & 15)) * 16);
+        const int row = 4 * (nw * LOADS + u) + g;
+        xo[u] = (uint32_t)(row < rows_left ? row : rows_left - 1) * (uint32_t)(2 * a.k);
+        xw[u] = (uint32_t)(row * 256 + (piece ^ (row & 15)) * 16);
     }
     const int xrow = r % ROWS;
 #pragma unroll
     for (int t = 0; t < 4; t++) xr[t] = (uint32_t)(xrow * 256 + ((4 * t + g) ^ xrow) * 16);
-    uint8_t* const xbuf = lds + kg * (BUFFERS * XU * 1024);
+    uint8_t* const xbuf = lds + kg * (SHARED ? 2 : 1) * BUFFER;
 
-    u32x4 w[2][NF], x[2][LOADS];
-    uint32_t s[2][NF][2 * GPS], z[2][NF][GPS];
+    uint32_t ones = 0x3f803f80u;
+    asm volatile("" : "+v"(ones));
+    u32x4 w[4][NF], x[DX][LOADS];
+    uint32_t s[4][NF][2 * GPS], z[4][NF][GPS];
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
         for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // `step` is inside the matrix.  A piece of a row beyond its end takes the last piece: its weights' scales are zero.
-    auto load = [&](auto dc, int step) __attribute__((always_inline)) {
-        constexpr int d = decltype(dc)::value;
-        const int p = 16 * step + piece;
+    // A step beyond the matrix loads the buffer's first bytes, which are not multiplied: a load that may not be issued would make every
+    // wait one for all loads.  A piece of a row beyond its end is the last piece again: its weights' scales are zero.
+    auto load_x = [&](auto dc, int step) __attribute__((always_inline)) {
+        constexpr int d = decltype(dc)::value % DX;
+        const int p = (step < a.steps ? 16 * step : 0) + piece;
+        const uint32_t po = (uint32_t)(p < pieces ? p : pieces - 1) * 16;
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xp[u] + (size_t)(p < pieces ? p : pieces - 1) * 16);
+        for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xb + (xo[u] + po));
+    };
+    auto load_w = [&](auto dc, int step) __attribute__((always_inline)) {
+        constexpr int d = decltype(dc)::value;
 #pragma unroll
         for (int i = 0; i < NF; i++) {
-            w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp[i] + (size_t)step * 1024));
-            int4_take(s[d][i], sp[i] + (size_t)step * (GPS * 32));
-            if (ZEROS) int4_take(z[d][i], zp[i] + (size_t)step * (GPS * 16));
+            const size_t from = step < a.steps ? tile_at[i] + step : 0;
+            w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.P + from * 1024 + (uint32_t)(lane * 16)));
+            int4_take(s[d][i], a.PS + from * (GPS * 32) + (uint32_t)(g * GPS * 8));
+            if (ZEROS) int4_take(z[d][i], a.PZ + from * (GPS * 16) + (uint32_t)(g * GPS * 4));
         }
     };
-    // LDS operations of a wave are carried out in order: with NW = 1 the next step's pieces may be written behind this step's reads.
+    // LDS operations of a wave are carried out in order: with one wave a group the next step's pieces may be written behind this step's reads.
     auto share_x = [&](auto dc) __attribute__((always_inline)) {
-        constexpr int d = decltype(dc)::value;
+        constexpr int d = decltype(dc)::value % DX;
+        uint8_t* const to = xbuf + (SHARED ? d % 2 * BUFFER : 0);
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) *reinterpret_cast<u32x4*>(xbuf + (NW > 1 ? d * XU * 1024 : 0) + xw[u]) = x[d][u];
-        if (NW > 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int u = 0; u < LOADS; u++) *reinterpret_cast<u32x4*>(to + xw[u]) = x[d][u];
+        if constexpr (SHARED) {
+            // the sums of the groups: 4 * PER neighbouring lanes have a group's pieces
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                const float sum = int4_over_lanes<PER>(int4_sum8(x[d][u], ones));
+                if (piece % (4 * PER) == 0)
+                    reinterpret_cast<float*>(to + XU * 1024)[piece / (4 * PER) * (4 * XU) + 4 * (nw * LOADS + u) + g] = sum;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
     };
     auto multiply = [&](auto dc) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value;
-        constexpr int PER = 4 / GPS;          // instructions a group
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-        const uint8_t* const from = xbuf + (NW > 1 ? d * XU * 1024 : 0);
-#pragma unroll
-        for (int q = 0; q < GPS; q++) {
-            f32x4 sum[MF], part[NF][MF];
-#pragma unroll
-            for (int t = 0; t < PER; t++) {
-                u32x4 y[MF];
+        const uint8_t* const from = xbuf + (SHARED ? d % 2 * BUFFER : 0);
+        // A unit is a group of a tile; a unit's scales are applied behind the next one's products, whose results take their time.
+        u32x4 y[2][PER][MF];
+        float sum[2][MF];
+        f32x4 part[2][MF];
+        auto products = [&](int unit) __attribute__((always_inline)) {
+            const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2;
+            if (i == 0) {
 #pragma unroll
                 for (int j = 0; j < MF; j++) {
-                    y[j] = *reinterpret_cast<const u32x4*>(from + j * 4096 + xr[q * PER + t]);
-                    sum[j] = mfma_bf16_16x16x32(ones, y[j], t ? sum[j] : zero);
-                }
 #pragma unroll
-                for (int i = 0; i < NF; i++) {
-                    const u32x4 v = int4_widen(w[d][i][q * PER + t]);
+                    for (int t = 0; t < PER; t++) y[h][t][j] = *reinterpret_cast<const u32x4*>(from + j * 4096 + xr[q * PER + t]);
+                    if constexpr (SHARED) {
+                        sum[h][j] = reinterpret_cast<const float*>(from + XU * 1024)[q * (4 * XU) + 16 * j + r];
+                    } else {
+                        f32x4 of_all = zero;
 #pragma unroll
-                    for (int j = 0; j < MF; j++) part[i][j] = mfma_bf16_16x16x32(v, y[j], t ? part[i][j] : zero);
+                        for (int t = 0; t < PER; t++) of_all = mfma_bf16_16x16x32(u32x4{ones, ones, ones, ones}, y[h][t][j], of_all);
+                        sum[h][j] = of_all[0];
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < NF; i++) {
-                const f32x4 scale = int4_scales<F16>(s[d][i][2 * q], s[d][i][2 * q + 1]);
-                const f32x4 zb = ZEROS ? int4_zeros(z[d][i][q]) : f32x4{1.5f, 1.5f, 1.5f, 1.5f};
+            for (int t = 0; t < PER; t++) {
+                const u32x4 v = int4_widen(w[d][i][q * PER + t], ones);
 #pragma unroll
-                for (int j = 0; j < MF; j++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(scale[c], fmaf(-zb[c], sum[j][c], part[i][j][c]), acc[i][j][c]);
+                for (int j = 0; j < MF; j++) part[u][j] = mfma_bf16_16x16x32(v, y[h][t][j], t ? part[u][j] : zero);
             }
+        };
+        auto apply = [&](int unit) __attribute__((always_inline)) {
+            const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2;
+            const f32x4 scale = int4_scales<F16>(s[d][i][2 * q], s[d][i][2 * q + 1]);
+            const f32x4 zb = ZEROS ? int4_zeros(z[d][i][q]) : f32x4{1.5f, 1.5f, 1.5f, 1.5f};
+#pragma unroll
+            for (int j = 0; j < MF; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(scale[c], fmaf(-zb[c], sum[h][j], part[u][j][c]), acc[i][j][c]);
+        };
+#pragma unroll
+        for (int unit = 0; unit <= GPS * NF; unit++) {
+            if (unit < GPS * NF) products(unit);
+            if (unit > 0) apply(unit - 1);
         }
         __builtin_amdgcn_sched_barrier(0);    // steps are not mixed: their temporaries would not fit
     };
+    // Steps kg, kg + KW, ...  A group with one fewer than another goes through the other's barriers.
+    const int end = SHARED ? (a.steps - 1) / KW * KW + KW : a.steps;
+    int step = kg;
+    auto turn = [&](auto dc) __attribute__((always_inline)) {
+        share_x(dc);
+        if (!SHARED || step < a.steps) multiply(dc);
+        load_x(dc, step + DX * KW);
+        load_w(dc, step + 4 * KW);
+        step += KW;
+        return step < end;
+    };
     using D0 = std::integral_constant<int, 0>;
     using D1 = std::integral_constant<int, 1>;
-
-    // Steps kg, kg + KW, ...: `left` of them; a group that has one fewer than another goes through the other's barriers.
-    int step = kg, left = kg < a.steps ? (a.steps - 1 - kg) / KW + 1 : 0;
-    int rounds = NW > 1 ? (a.steps - 1) / KW + 1 : left;
-    if (left > 0) load(D0{}, step);
-    if (left > 1) load(D1{}, step + KW);
-    for (; left >= 4; left -= 2, rounds -= 2, step += 2 * KW) {
-        share_x(D0{});
-        multiply(D0{});
-        load(D0{}, step + 2 * KW);
-        share_x(D1{});
-        multiply(D1{});
-        load(D1{}, step + 3 * KW);
+    using D2 = std::integral_constant<int, 2>;
+    using D3 = std::integral_constant<int, 3>;
+    if (step < end) {
+        load_x(D0{}, step);
+        load_w(D0{}, step);
+        load_x(D1{}, step + KW);
+        load_w(D1{}, step + KW);
+        if (DX > 2) load_x(D2{}, step + 2 * KW);
+        load_w(D2{}, step + 2 * KW);
+        if (DX > 2) load_x(D3{}, step + 3 * KW);
+        load_w(D3{}, step + 3 * KW);
+        while (turn(D0{}) && turn(D1{}) && turn(D2{}) && turn(D3{})) {}
     }
-    // at most three are left, the first two of them loaded
-    if (rounds > 0) share_x(D0{});
-    if (left > 0) multiply(D0{});
-    if (left > 2) load(D0{}, step + 2 * KW);
-    if (rounds > 1) share_x(D1{});
-    if (left > 1) multiply(D1{});
-    if (rounds > 2) share_x(D0{});
-    if (left > 2) multiply(D0{});
-    if (rounds > 3) share_x(D1{});
 
     // ---- the groups' sums, in their order ----
     auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) {

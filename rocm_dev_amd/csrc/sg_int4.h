@@ -44,11 +44,22 @@ struct Int4Args {
     int m, n, k;
     int tiles, steps;
     int n_groups, m_groups;          // workgroup tiles along n and m
+    int splits;                      // workgroups that share K of a tile
+    float* ws;                       // splits > 1: their sums, [split][m / 16][n / 16][64 lanes][4], added by a second launch
 };
 
+constexpr int kInt4Splits = 8;       // at most
+
+// How a product is carried out: workgroups of kw * nw waves, nw of them with nf weight tiles each, on 4 * xu activation rows.
+struct Int4Plan {
+    int nf, xu, nw, kw, splits;
+};
+Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace);
+
 // one build of kernels for each number of groups a step (sg_int4_inst.hip)
-int launch_int4_1(Int4Args& a, int flags, int cu_count, hipStream_t stream);
-int launch_int4_2(Int4Args& a, int flags, int cu_count, hipStream_t stream);
-int launch_int4_4(Int4Args& a, int flags, int cu_count, hipStream_t stream);
+int launch_int4_1(Int4Args& a, int flags, const Int4Plan& plan, hipStream_t stream);
+int launch_int4_2(Int4Args& a, int flags, const Int4Plan& plan, hipStream_t stream);
+int launch_int4_4(Int4Args& a, int flags, const Int4Plan& plan, hipStream_t stream);
+int launch_int4_sum(const Int4Args& a, hipStream_t stream);
 
 }  // namespace sg

@@ -52,6 +52,85 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
     if (a.zeros) a.PZ[to] = inside ? a.zeros[from] : (uint8_t)0;
 }
 
+// The build, its waves and its K splits by the shape; us below are of one MI355X, medians of graph replays on cold weights.
+//
+// Up to 16 rows: one tile a wave where there are at most as many tiles as CUs (4096 x 4096 at one row 4.9, two tiles 5.6), two elsewhere
+// (28672 x 4096 14.2, 15.5), on as many waves as leave each a few steps.  K splits where idle CUs can take them and the steps that a
+// wave has left outweigh the second launch: 1 x 1024 x 32768 14.3 -> 9.8, 8 x 512 x 16384 10.9 -> 7.3.
+//
+// Beyond, the waves' vector units bound what a workgroup does, so that its time is its steps times that of one, and a product's that of
+// its rounds of workgroups.  The four ways - two or four waves of one tile and groups of them that share K, eight of one tile, eight of two -
+// and their K splits are compared by that: 64 rows of 57344 x 8192 98 (two tiles on eight waves; 203 on two waves of one), 10240 x 8192
+// 32.5 (the same, six splits; unsplit 91, 39 on four waves), 8192 x 28672 60 (eight splits; 97 on two waves).
+Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
+    Int4Plan p{1, a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : a.m <= 32 ? 8 : 16, 1, 1, 1};
+#ifdef SG_SWEEP
+    {
+        p.nf = atoi(getenv("SW_NF")), p.nw = atoi(getenv("SW_NW")), p.kw = atoi(getenv("SW_KW")), p.splits = atoi(getenv("SW_SPLITS"));
+        return p;
+    }
+#endif
+    if (p.xu <= 4) {
+        p.nf = a.tiles > cu_count ? 2 : 1;
+        const int groups = (a.tiles - 1) / p.nf + 1;
+        if (p.nf == 1) p.kw = p.xu == 1 && (a.steps >= 96 || (a.steps >= 48 && a.tiles <= cu_count / 2)) ? 16 : 8;
+        else p.kw = groups <= cu_count ? 8 : groups <= 2 * cu_count || a.steps >= 48 ? 4 : 2;
+        while (p.kw > a.steps) p.kw /= 2;
+        if (!workspace || 2 * groups > cu_count) return p;
+        const int splits = cu_count / groups < kInt4Splits ? cu_count / groups : kInt4Splits;
+        const float left = (float)a.steps / p.kw, a_step = p.xu == 4 ? 0.7f : 0.45f;
+        if (left * a_step * (1.0f - 1.0f / splits) > 3.5f) p.splits = splits;
+        return p;
+    }
+    struct Way {
+        int nf, nw, kw, at_once;     // workgroups a CU
+        float a_step[2];             // us of a step of a workgroup, up to 32 and up to 64 rows, with all of a CU's
+    };
+    static constexpr Way ways[] = {{1, 2, 4, 1, {1.28f, 2.0f}}, {1, 4, 2, 1, {0.84f, 1.2f}}, {1, 8, 1, 2, {1.14f, 1.64f}}, {2, 8, 1, 1, {1.1f, 1.53f}}};
+    const int m_groups = (a.m - 1) / (4 * p.xu) + 1;
+    float best = 0.0f;
+    for (const Way& w : ways) {
+        const long long groups = (long long)((a.tiles - 1) / (w.nf * w.nw) + 1) * m_groups;
+        const int at_once = group == 32 ? 1 : w.at_once;
+        int kw = w.kw;
+        while (kw > a.steps) kw /= 2;
+        for (int splits = 1; splits <= (workspace ? kInt4Splits : 1) && splits * kw <= a.steps; splits++) {
+            const long long all = groups * splits, slots = (long long)at_once * cu_count;
+            // a workgroup alone on its CU is through sooner than two
+            const float a_step = w.a_step[p.xu == 16] * (w.at_once == 2 && (at_once == 1 || all <= cu_count) ? 0.6f : 1.0f);
+            const float rounds = (float)((all + slots - 1) / slots), turns = (float)((a.steps - 1) / (splits * kw) + 1);
+            const float parts = splits > 1 ? 2.5f + (float)splits * ((a.m - 1) / 16 + 1) * a.tiles * 1024 * 2 / 3.5e6f : 0.0f;
+            const float us = rounds * (turns * a_step + 1.5f) + parts;
+            if (best == 0.0f || us < best) best = us, p.nf = w.nf, p.nw = w.nw, p.kw = kw, p.splits = splits;
+        }
+    }
+    return p;
+}
+
+static int launch(Int4Args& a, int group, int flags, const Int4Plan& plan, hipStream_t stream) {
+    a.splits = plan.splits;
+    return group == 128 ? launch_int4_1(a, flags, plan, stream) : group == 64 ? launch_int4_2(a, flags, plan, stream) : launch_int4_4(a, flags, plan, stream);
+}
+
+// A K split adds its parts up in the stream's workspace by a second launch.  A recorded launch uses no memory of the library's, so that
+// graphs may replay side by side, and a call that can get no device memory does without too.
+static int launch_gemm(Int4Args& a, int group, int flags, int cu_count, hipStream_t stream) {
+    const Int4Plan plan = int4_plan(a, group, cu_count, true);
+    if (plan.splits == 1) return launch(a, group, flags, plan, stream);
+    if (!stream_is_capturing(stream)) {
+        std::lock_guard<std::recursive_mutex> turn(stream_turn(stream));
+        Workspace w;
+        const int rc = get_workspace(stream, (size_t)((a.m - 1) / 16 + 1) * a.tiles * plan.splits * 1024, 0, &w);
+        if (rc == SG_SUCCESS) {
+            a.ws = w.partials;
+            if (int failed = launch(a, group, flags, plan, stream)) return failed;
+            return launch_int4_sum(a, stream);
+        }
+        if (rc != SG_NO_DEVICE && rc != SG_WORKSPACE_TOO_SMALL) return rc;
+    }
+    return launch(a, group, flags, int4_plan(a, group, cu_count, false), stream);
+}
+
 }  // namespace sg
 
 using namespace sg;
@@ -99,8 +178,7 @@ int sg_int4_gemm(const void* A, const uint8_t* P, void* D, int m, int n, int k, 
     a.k = k;
     a.tiles = l.tiles;
     a.steps = l.steps;
-    auto* const launch = group == 128 ? launch_int4_1 : group == 64 ? launch_int4_2 : launch_int4_4;
-    return launch(a, flags, dev->cu_count, static_cast<hipStream_t>(stream));
+    return launch_gemm(a, group, flags, dev->cu_count, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

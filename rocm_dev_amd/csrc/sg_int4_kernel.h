@@ -111,25 +111,33 @@ __device__ __forceinline__ float int4_over_lanes(float v) {
 }
 
 // FLAGS: SG_INT4_ZEROS, SG_INT4_F16_SCALES.  The tile has 4 * XU activation rows.
-// LDS: [KW][NW > 1 ? 2 : 1][XU KB activations, NW > 1: [4 * XU][GPS] sums of groups], then in its place [KW][NW][NF * MF][64 lanes] f32x4.
-template <int GPS, int FLAGS, int NF, int XU, int NW, int DX>
-__global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
+// LDS: [KW][2][XU KB activations, NW > 1: [4 * XU][GPS] sums of groups], then in its place [KW][NW][NF * MF][64 lanes] f32x4.
+template <int GPS, int FLAGS, int NF, int XU, int NW, int DW, int DX, int MAXW, int MINB>
+__global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Args a) {
     constexpr bool ZEROS = FLAGS & SG_INT4_ZEROS, F16 = FLAGS & SG_INT4_F16_SCALES;
     constexpr int MF = XU < 4 ? 1 : XU / 4, LOADS = XU / NW, ROWS = 4 * XU < 16 ? 4 * XU : 16, PER = 4 / GPS;     // PER: instructions a group
     constexpr bool SHARED = NW > 1;
     constexpr int BUFFER = int4_buffer(GPS, XU, NW);
-    static_assert(XU % NW == 0 && (DX == 2 || DX == 4));
+    static_assert(XU % NW == 0 && (DX == 2 || DX == 4) && (DW == 2 || DW == 4));
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int wave = wave_id(), waves = (int)(blockDim.x >> 6), KW = waves / NW, kg = wave / NW, nw = wave % NW;
     const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    const int tn = at / a.m_groups, tm = at - tn * a.m_groups;       // neighbours share the weights
+    const int rest = at / a.m_groups, tm = at - rest * a.m_groups;       // neighbours share the weights, then the activations
+    const int split = a.splits > 1 ? rest / a.n_groups : 0, tn = a.splits > 1 ? rest - split * a.n_groups : rest;
+    const int begin = a.splits > 1 ? (int)((long long)a.steps * split / a.splits) : 0;
+    const int steps = a.splits > 1 ? (int)((long long)a.steps * (split + 1) / a.splits) : a.steps;      // the end of this part of K
     const int first_tile = (tn * NW + nw) * NF;
 
     // ---- operands: tiles beyond the last and rows beyond m take the last one again, and are not stored ----
-    size_t tile_at[NF];               // the tile's first step
+    const uint8_t *wb[NF], *sb[NF], *zb_[NF];
 #pragma unroll
-    for (int i = 0; i < NF; i++) tile_at[i] = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
+    for (int i = 0; i < NF; i++) {
+        const size_t tile = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
+        wb[i] = a.P + tile * 1024;
+        sb[i] = a.PS + tile * (GPS * 32);
+        zb_[i] = ZEROS ? a.PZ + tile * (GPS * 16) : nullptr;
+    }
     // Activations: load u of the tile has rows 4 u .. 4 u + 3, lane l piece l % 16 (8 columns) of row l / 16; in LDS the pieces of row i stand
     // permuted by i, so that the 16 lanes (r, g) of a fragment's read hit 16 bank groups.
     const uint8_t* const xb = reinterpret_cast<const uint8_t*>(a.A + (size_t)tm * 4 * XU * a.k);
@@ -144,75 +152,81 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
     const int xrow = r % ROWS;
 #pragma unroll
     for (int t = 0; t < 4; t++) xr[t] = (uint32_t)(xrow * 256 + ((4 * t + g) ^ xrow) * 16);
-    uint8_t* const xbuf = lds + kg * (SHARED ? 2 : 1) * BUFFER;
+    uint8_t* const xbuf = lds + kg * 2 * BUFFER;
 
     uint32_t ones = 0x3f803f80u;
     asm volatile("" : "+v"(ones));
-    u32x4 w[4][NF], x[DX][LOADS];
-    uint32_t s[4][NF][2 * GPS], z[4][NF][GPS];
+    u32x4 w[DW][NF], x[DX][LOADS];
+    uint32_t s[DW][NF][2 * GPS], z[DW][NF][GPS];
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
         for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // A step beyond the matrix loads the buffer's first bytes, which are not multiplied: a load that may not be issued would make every
-    // wait one for all loads.  A piece of a row beyond its end is the last piece again: its weights' scales are zero.
+    // A step beyond this part of K loads its first one again, which is not multiplied: a load that may not be issued would make every wait one
+    // for all loads.  A piece of a row beyond its end is the last piece again: its weights' scales are zero.  (32-bit offsets: k is below 2^24.)
+    auto inside = [&](int step) { return (uint32_t)(step < steps ? step : begin); };
     auto load_x = [&](auto dc, int step) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value % DX;
-        const int p = (step < a.steps ? 16 * step : 0) + piece;
+        const int p = (int)(16 * inside(step)) + piece;
         const uint32_t po = (uint32_t)(p < pieces ? p : pieces - 1) * 16;
 #pragma unroll
         for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xb + (xo[u] + po));
     };
     auto load_w = [&](auto dc, int step) __attribute__((always_inline)) {
-        constexpr int d = decltype(dc)::value;
+        constexpr int d = decltype(dc)::value % DW;
+        const uint32_t from = inside(step);
+        const uint32_t wo = from * 1024 + lane * 16, so = from * (GPS * 32) + g * (GPS * 8), zo = from * (GPS * 16) + g * (GPS * 4);
 #pragma unroll
         for (int i = 0; i < NF; i++) {
-            const size_t from = step < a.steps ? tile_at[i] + step : 0;
-            w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.P + from * 1024 + (uint32_t)(lane * 16)));
-            int4_take(s[d][i], a.PS + from * (GPS * 32) + (uint32_t)(g * GPS * 8));
-            if (ZEROS) int4_take(z[d][i], a.PZ + from * (GPS * 16) + (uint32_t)(g * GPS * 4));
+            w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wb[i] + wo));
+            int4_take(s[d][i], sb[i] + so);
+            if (ZEROS) int4_take(z[d][i], zb_[i] + zo);
         }
     };
-    // LDS operations of a wave are carried out in order: with one wave a group the next step's pieces may be written behind this step's reads.
+    // A step's activations are brought to LDS a step before they are read, in two places in turn.
     auto share_x = [&](auto dc) __attribute__((always_inline)) {
-        constexpr int d = decltype(dc)::value % DX;
-        uint8_t* const to = xbuf + (SHARED ? d % 2 * BUFFER : 0);
+        constexpr int d = decltype(dc)::value;
+        uint8_t* const to = xbuf + d % 2 * BUFFER;
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) *reinterpret_cast<u32x4*>(to + xw[u]) = x[d][u];
+        for (int u = 0; u < LOADS; u++) *reinterpret_cast<u32x4*>(to + xw[u]) = x[d % DX][u];
         if constexpr (SHARED) {
             // the sums of the groups: 4 * PER neighbouring lanes have a group's pieces
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
-                const float sum = int4_over_lanes<PER>(int4_sum8(x[d][u], ones));
+                const float sum = int4_over_lanes<PER>(int4_sum8(x[d % DX][u], ones));
                 if (piece % (4 * PER) == 0)
                     reinterpret_cast<float*>(to + XU * 1024)[piece / (4 * PER) * (4 * XU) + 4 * (nw * LOADS + u) + g] = sum;
             }
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     };
+    // behind a step: all waves have read its activations, and have brought the next one's
+    auto meet = [&]() __attribute__((always_inline)) {
+        if (SHARED) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
     auto multiply = [&](auto dc) __attribute__((always_inline)) {
-        constexpr int d = decltype(dc)::value;
+        constexpr int d = decltype(dc)::value % DW;
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const uint8_t* const from = xbuf + (SHARED ? d % 2 * BUFFER : 0);
+        const uint8_t* const from = xbuf + decltype(dc)::value % 2 * BUFFER;
         // A unit is a group of a tile; a unit's scales are applied behind the next one's products, whose results take their time.
-        u32x4 y[2][PER][MF];
+        constexpr int Y = MF < 4 ? 2 : 1;      // groups' activations at a time
+        u32x4 y[Y][PER][MF];
         float sum[2][MF];
         f32x4 part[2][MF];
         auto products = [&](int unit) __attribute__((always_inline)) {
-            const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2;
+            const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2, hy = q % Y;
             if (i == 0) {
 #pragma unroll
                 for (int j = 0; j < MF; j++) {
 #pragma unroll
-                    for (int t = 0; t < PER; t++) y[h][t][j] = *reinterpret_cast<const u32x4*>(from + j * 4096 + xr[q * PER + t]);
+                    for (int t = 0; t < PER; t++) y[hy][t][j] = *reinterpret_cast<const u32x4*>(from + j * 4096 + xr[q * PER + t]);
                     if constexpr (SHARED) {
                         sum[h][j] = reinterpret_cast<const float*>(from + XU * 1024)[q * (4 * XU) + 16 * j + r];
                     } else {
                         f32x4 of_all = zero;
 #pragma unroll
-                        for (int t = 0; t < PER; t++) of_all = mfma_bf16_16x16x32(u32x4{ones, ones, ones, ones}, y[h][t][j], of_all);
+                        for (int t = 0; t < PER; t++) of_all = mfma_bf16_16x16x32(u32x4{ones, ones, ones, ones}, y[hy][t][j], of_all);
                         sum[h][j] = of_all[0];
                     }
                 }
@@ -221,7 +235,7 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
             for (int t = 0; t < PER; t++) {
                 const u32x4 v = int4_widen(w[d][i][q * PER + t], ones);
 #pragma unroll
-                for (int j = 0; j < MF; j++) part[u][j] = mfma_bf16_16x16x32(v, y[h][t][j], t ? part[u][j] : zero);
+                for (int j = 0; j < MF; j++) part[u][j] = mfma_bf16_16x16x32(v, y[hy][t][j], t ? part[u][j] : zero);
             }
         };
         auto apply = [&](int unit) __attribute__((always_inline)) {
@@ -241,14 +255,16 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
         __builtin_amdgcn_sched_barrier(0);    // steps are not mixed: their temporaries would not fit
     };
     // Steps kg, kg + KW, ...  A group with one fewer than another goes through the other's barriers.
-    const int end = SHARED ? (a.steps - 1) / KW * KW + KW : a.steps;
-    int step = kg;
+    const int end = SHARED ? begin + (steps - begin - 1) / KW * KW + KW : steps;
+    int step = begin + kg;
     auto turn = [&](auto dc) __attribute__((always_inline)) {
-        share_x(dc);
-        if (!SHARED || step < a.steps) multiply(dc);
-        load_x(dc, step + DX * KW);
-        load_w(dc, step + 4 * KW);
+        using Next = std::integral_constant<int, (decltype(dc)::value + 1) % 4>;
+        share_x(Next{});                                     // (behind the last step what a step beyond the matrix loads)
+        load_x(Next{}, step + (DX + 1) * KW);
+        if (!SHARED || step < steps) multiply(dc);
+        load_w(dc, step + DW * KW);
         step += KW;
+        meet();
         return step < end;
     };
     using D0 = std::integral_constant<int, 0>;
@@ -261,14 +277,22 @@ __global__ void __launch_bounds__(512) int4_gemm_kernel(const Int4Args a) {
         load_x(D1{}, step + KW);
         load_w(D1{}, step + KW);
         if (DX > 2) load_x(D2{}, step + 2 * KW);
-        load_w(D2{}, step + 2 * KW);
+        if (DW > 2) load_w(D2{}, step + 2 * KW);
         if (DX > 2) load_x(D3{}, step + 3 * KW);
-        load_w(D3{}, step + 3 * KW);
+        if (DW > 2) load_w(D3{}, step + 3 * KW);
+        share_x(D0{});
+        load_x(D0{}, step + DX * KW);
+        meet();
         while (turn(D0{}) && turn(D1{}) && turn(D2{}) && turn(D3{})) {}
     }
 
     // ---- the groups' sums, in their order ----
     auto finish = [&](f32x4 v, int i, int j) __attribute__((always_inline)) {
+        if (a.splits > 1) {        // into the workspace, whole fragments
+            const int tile = first_tile + i, m_frag = tm * MF + j, m_frags = (a.m - 1) / 16 + 1;
+            if (tile < a.tiles && m_frag < m_frags) reinterpret_cast<f32x4*>(a.ws)[(((size_t)split * m_frags + m_frag) * a.tiles + tile) * 64 + lane] = v;
+            return;
+        }
         const int n_idx = (first_tile + i) * 16 + 4 * g, m_idx = tm * 4 * XU + 16 * j + r;
         if (r < ROWS && m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * 16.0f);
     };

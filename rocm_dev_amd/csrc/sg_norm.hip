@@ -6,7 +6,7 @@
 // to the bit: the sum of squares and the maximum come out of the same pass over the row and one reduction.  A row is held
 // in registers between the reduction and the codes: it is read from memory once.
 // fp32 throughout; roundings to fewer bits are the three outputs' own (v as bf16, since the next layer adds to what is
-// stored; the codes; Y).  y / s is a product with 1 / s: y itself carries the rounding of its sum of squares, so that a correctly rounded
+// stored; the codes; Y).  y / s is one product, v * w with rstd / s: y itself carries the rounding of its sum of squares, so that a correctly rounded
 // quotient (as the encoder's, whose input is exact) would mean nothing here.
 #include <cmath>
 
@@ -34,7 +34,7 @@ struct RowSums {
 };
 
 struct RowFactors {
-    float rstd, s, inv;
+    float rstd, s, code;         // code: rstd / s
     bool divide;                 // 1 / s does not stand for s
 };
 __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps) {
@@ -43,7 +43,7 @@ __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps
     float top = r.top * f.rstd;
     if (!(top > 0.0f)) top = 0.0f;                       // also NaN: an infinity times zero, or a row that holds a NaN
     f.s = top == 0.0f ? 1.0f : __fdiv_rn(top, 448.0f);
-    f.inv = __fdiv_rn(1.0f, f.s);
+    f.code = f.rstd * __fdiv_rn(1.0f, f.s);
     f.divide = !(f.s >= 0x1p-120f && f.s <= 0x1p120f);
     return f;
 }
@@ -64,79 +64,85 @@ __device__ __forceinline__ void see(RowSums& r, u32x4 v, u32x4 w) {
         r.top = fmaxf(r.top, fmaxf(fabsf(lo * bf16_lo(w[j])), fabsf(hi * bf16_hi(w[j]))));
     }
 }
+// codes and Y of eight columns, `at` chunks into the matrix
 template <bool DIVIDE>
-__device__ __forceinline__ u32x2 codes_of(const float (&y)[8], const RowFactors& f) {
-    float q[8];
+__device__ __forceinline__ void put_chunk(const NormArgs& a, size_t at, u32x4 v, u32x4 w, const RowFactors& f) {
+    float p[8], q[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = DIVIDE ? __fdiv_rn(y[j], f.s) : y[j] * f.inv;
+    for (int j = 0; j < 4; j++) {
+        p[2 * j] = bf16_lo(v[j]) * bf16_lo(w[j]);
+        p[2 * j + 1] = bf16_hi(v[j]) * bf16_hi(w[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = DIVIDE ? __fdiv_rn(p[j] * f.rstd, f.s) : p[j] * f.code;
     int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     w0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w0, true);
     int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
     w1 = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], w1, true);
-    return u32x2{canonical_nan_codes(w0), canonical_nan_codes(w1)};
-}
-// codes and Y of eight columns, `at` chunks into the matrix
-__device__ __forceinline__ void put(const NormArgs& a, size_t at, u32x4 v, u32x4 w, const RowFactors& f) {
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        y[2 * j] = bf16_lo(v[j]) * bf16_lo(w[j]) * f.rstd;
-        y[2 * j + 1] = bf16_hi(v[j]) * bf16_hi(w[j]) * f.rstd;
-    }
-    reinterpret_cast<u32x2*>(a.Q)[at] = f.divide ? codes_of<true>(y, f) : codes_of<false>(y, f);
+    __builtin_nontemporal_store(u32x2{canonical_nan_codes(w0), canonical_nan_codes(w1)}, reinterpret_cast<u32x2*>(a.Q) + at);
     if (a.Y) {
         u32x4 o;
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
-        reinterpret_cast<u32x4*>(a.Y)[at] = o;
+        for (int j = 0; j < 4; j++) o[j] = pack_bf16x2(p[2 * j] * f.rstd, p[2 * j + 1] * f.rstd);
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(a.Y) + at);
     }
+}
+__device__ __forceinline__ void put(const NormArgs& a, size_t at, u32x4 v, u32x4 w, const RowFactors& f) {
+    if (f.divide) put_chunk<true>(a, at, v, w, f);
+    else put_chunk<false>(a, at, v, w, f);
 }
 constexpr unsigned kOnes = 0x3f803f80u;      // two bf16 ones
 
-// A thread's chunks of its row: t, t + STEP, ...  One past the row's end takes the last chunk again, counts nothing and stores nothing.
+// A thread's chunks of a row: t, t + STEP, ...  One past the row's end is the last chunk again, counts nothing and is not stored.
 template <int STEP, int CH>
 struct RowChunks {
-    u32x4 v[CH], w[CH];
+    u32x4 x[CH], r[CH];
 
-    __device__ __forceinline__ RowSums load(const NormArgs& a, size_t row, int t, int nchunks) {
-        const u32x4* const x = reinterpret_cast<const u32x4*>(a.X) + row * nchunks;
+    static __device__ __forceinline__ int at(int c, int t, int nchunks) { return c * STEP + t < nchunks ? c * STEP + t : nchunks - 1; }
+    __device__ __forceinline__ void load(const NormArgs& a, size_t row, int t, int nchunks) {
+        const u32x4* const from = reinterpret_cast<const u32x4*>(a.X) + row * nchunks;
         const u32x4* const res = reinterpret_cast<const u32x4*>(a.residual) + row * nchunks;
-        const u32x4* const wt = reinterpret_cast<const u32x4*>(a.weight);
-        u32x4 r[CH];
 #pragma unroll
-        for (int c = 0; c < CH; c++) v[c] = __builtin_nontemporal_load(x + at(c, t, nchunks));
-        if (a.residual) {
+        for (int c = 0; c < CH; c++) x[c] = __builtin_nontemporal_load(from + at(c, t, nchunks));
+        if (a.residual)
 #pragma unroll
             for (int c = 0; c < CH; c++) r[c] = __builtin_nontemporal_load(res + at(c, t, nchunks));
-        }
-        if (a.weight) {
-#pragma unroll
-            for (int c = 0; c < CH; c++) w[c] = wt[at(c, t, nchunks)];
-        } else {
-#pragma unroll
-            for (int c = 0; c < CH; c++) w[c] = u32x4{kOnes, kOnes, kOnes, kOnes};
-        }
-        if (a.residual) {
-#pragma unroll
-            for (int c = 0; c < CH; c++) v[c] = add_bf16(v[c], r[c]);
-        }
-        RowSums sums = {0.0f, 0.0f};
-#pragma unroll
-        for (int c = 0; c < CH; c++)
-            if (c * STEP + t < nchunks) see(sums, v[c], w[c]);
-        return sums;
     }
-    __device__ __forceinline__ void store(const NormArgs& a, size_t row, int t, int nchunks, const RowFactors& f) {
+    // x becomes v
+    __device__ __forceinline__ void add(const NormArgs& a) {
+        if (a.residual)
 #pragma unroll
-        for (int c = 0; c < CH; c++)
-            if (c * STEP + t < nchunks) {
-                const size_t to = row * nchunks + c * STEP + t;
-                if (a.sum) reinterpret_cast<u32x4*>(a.sum)[to] = v[c];
-                put(a, to, v[c], w[c], f);
-            }
+            for (int c = 0; c < CH; c++) x[c] = add_bf16(x[c], r[c]);
     }
-    static __device__ __forceinline__ int at(int c, int t, int nchunks) { return c * STEP + t < nchunks ? c * STEP + t : nchunks - 1; }
 };
+__device__ __forceinline__ u32x4 weight_of(const NormArgs& a, int chunk) {
+    return a.weight ? reinterpret_cast<const u32x4*>(a.weight)[chunk] : u32x4{kOnes, kOnes, kOnes, kOnes};
+}
+template <int STEP, int CH, class Weight>
+__device__ __forceinline__ RowSums sums_of(const u32x4 (&v)[CH], int t, int nchunks, Weight&& weight) {
+    RowSums sums = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+        if (c * STEP + t < nchunks) see(sums, v[c], weight(c));
+    return sums;
+}
+template <int STEP, int CH, class Weight>
+__device__ __forceinline__ void put_row(const NormArgs& a, size_t row, const u32x4 (&v)[CH], int t, int nchunks, const RowFactors& f, Weight&& weight) {
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+        if (c * STEP + t < nchunks) {
+            const size_t to = row * nchunks + c * STEP + t;
+            if (a.sum) __builtin_nontemporal_store(v[c], reinterpret_cast<u32x4*>(a.sum) + to);
+            put(a, to, v[c], weight(c), f);
+        }
+}
+
+// Packed as they are, two values a register: the compiler would keep what it has unpacked.
+template <int CH>
+__device__ __forceinline__ void keep_packed(u32x4 (&v)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; c++) asm volatile("" : "+v"(v[c]));
+}
 
 template <int LANES>
 __device__ __forceinline__ RowSums over_lanes(RowSums r) {
@@ -164,15 +170,26 @@ __device__ __forceinline__ RowSums over_threads(RowSums r) {
     return r;
 }
 
-// One workgroup a row.
-template <int THREADS, int CH>
+// A workgroup a row.  KEEP: the weight is asked for with the row and stays in registers; otherwise it is read where it is used, twice, out of
+// the caches - later, but off the way of the first round of rows, and with fewer registers.
+template <int THREADS, int CH, bool KEEP>
 __global__ void __launch_bounds__(THREADS) rmsnorm_row_kernel(const NormArgs a) {
     const int t = threadIdx.x, nchunks = a.cols >> 3;
     RowChunks<THREADS, CH> row;
-    const RowSums sums = over_threads<THREADS>(row.load(a, blockIdx.x, t, nchunks));
+    u32x4 w[KEEP ? CH : 1];
+    auto weight = [&](int c) { return KEEP ? w[KEEP ? c : 0] : weight_of(a, row.at(c, t, nchunks)); };
+    row.load(a, blockIdx.x, t, nchunks);
+    if (KEEP)
+#pragma unroll
+        for (int c = 0; c < CH; c++) w[KEEP ? c : 0] = weight_of(a, row.at(c, t, nchunks));
+    row.add(a);
+    RowSums sums = sums_of<THREADS>(row.x, t, nchunks, weight);
+    keep_packed(row.x);
+    if (KEEP) keep_packed(w);
+    sums = over_threads<THREADS>(sums);
     const RowFactors f = row_factors(sums, a.cols, a.eps);
     if (t == 0) a.scales[blockIdx.x] = f.s;
-    row.store(a, blockIdx.x, t, nchunks, f);
+    put_row<THREADS>(a, blockIdx.x, row.x, t, nchunks, f, weight);
 }
 
 // Short rows: LANES lanes of a wave share one.
@@ -182,11 +199,17 @@ __global__ void __launch_bounds__(256) rmsnorm_short_rows_kernel(const NormArgs 
     const unsigned at = mine < (unsigned)a.rows ? mine : (unsigned)a.rows - 1;      // lanes past the last row store nothing
     const int t = (int)threadIdx.x % LANES, nchunks = a.cols >> 3;
     RowChunks<LANES, CH> row;
-    const RowSums sums = over_lanes<LANES>(row.load(a, at, t, nchunks));
+    u32x4 w[CH];
+    auto weight = [&](int c) { return w[c]; };
+    row.load(a, at, t, nchunks);
+#pragma unroll
+    for (int c = 0; c < CH; c++) w[c] = weight_of(a, row.at(c, t, nchunks));
+    row.add(a);
+    const RowSums sums = over_lanes<LANES>(sums_of<LANES>(row.x, t, nchunks, weight));
     if (mine >= (unsigned)a.rows) return;
     const RowFactors f = row_factors(sums, a.cols, a.eps);
     if (t == 0) a.scales[mine] = f.s;
-    row.store(a, mine, t, nchunks, f);
+    put_row<LANES>(a, mine, row.x, t, nchunks, f, weight);
 }
 
 // Rows beyond 65536 columns: two passes; v is read again where it is stored, and formed again where it is not.  (Its sum may
@@ -216,24 +239,36 @@ __global__ void __launch_bounds__(1024) rmsnorm_long_rows_kernel(const NormArgs 
     }
 }
 
-static int launch(const NormArgs& a, hipStream_t stream) {
+template <int THREADS, int CH>
+static void launch_row(const NormArgs& a, int cu_count, hipStream_t stream) {
+    // Where all rows but a CU's first run at once, the weight is read late: us, late against kept, 1021 x 10944 11.7 - 15.2, 2048 x 4096 with
+    // a residual 11.7 - 13.3, 1000 x 16384 20.6 - 23.7; a CU's first rows are waited for, and many rounds read it too often: 1 x 4096
+    // 3.3 - 2.8, 256 x 8192 5.5 - 5.1, 8192 x 8192 86.8 - 83.2.
+    const bool late = THREADS < 1024 && a.rows > cu_count && a.rows <= cu_count * (2048 / THREADS);
+    if (late) rmsnorm_row_kernel<THREADS, CH, false><<<(unsigned)a.rows, THREADS, 0, stream>>>(a);
+    else rmsnorm_row_kernel<THREADS, CH, true><<<(unsigned)a.rows, THREADS, 0, stream>>>(a);
+}
+
+static int launch(const NormArgs& a, int cu_count, hipStream_t stream) {
     const int nchunks = a.cols >> 3;
     const unsigned rows = (unsigned)a.rows;
+    // the smallest group of threads that holds the row in two chunks each, with more rows in four (as the encoder of rows)
 #define SG_SHORT(LANES, CH) rmsnorm_short_rows_kernel<LANES, CH><<<(rows - 1) / (256 / LANES) + 1, 256, 0, stream>>>(a)
-#define SG_ROW(THREADS, CH) rmsnorm_row_kernel<THREADS, CH><<<rows, THREADS, 0, stream>>>(a)
     if (nchunks <= 4) SG_SHORT(4, 1);
     else if (nchunks <= 16) SG_SHORT(16, 1);
     else if (nchunks <= 64) SG_SHORT(32, 2);
-    else if (nchunks <= 128) SG_ROW(64, 2);
-    else if (nchunks <= 256) SG_ROW(128, 2);
-    else if (nchunks <= 512) SG_ROW(256, 2);
-    else if (nchunks <= 1024) SG_ROW(512, 2);
-    else if (nchunks <= 2048) SG_ROW(1024, 2);
-    else if (nchunks <= 4096) SG_ROW(1024, 4);
-    else if (nchunks <= 8192) SG_ROW(1024, 8);
+    else if (nchunks <= 128) launch_row<64, 2>(a, cu_count, stream);
+    else if (nchunks <= 256) launch_row<128, 2>(a, cu_count, stream);
+    else if (nchunks <= 512) launch_row<256, 2>(a, cu_count, stream);
+    else if (nchunks <= 1024 && a.rows <= 1024) launch_row<512, 2>(a, cu_count, stream);
+    else if (nchunks <= 1024) launch_row<256, 4>(a, cu_count, stream);
+    else if (nchunks <= 2048 && a.rows <= 256) launch_row<1024, 2>(a, cu_count, stream);
+    else if (nchunks <= 2048) launch_row<512, 4>(a, cu_count, stream);
+    else if (nchunks <= 4096) launch_row<1024, 4>(a, cu_count, stream);
+    // (kept, the weight's registers would spill: 64 x 65536 19.0, 14.4 this way)
+    else if (nchunks <= 8192) rmsnorm_row_kernel<1024, 8, false><<<rows, 1024, 0, stream>>>(a);
     else rmsnorm_long_rows_kernel<<<rows, 1024, 0, stream>>>(a);
 #undef SG_SHORT
-#undef SG_ROW
     return report_hip("rmsnorm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
@@ -251,5 +286,5 @@ extern "C" int sg_rmsnorm_fp8_rows(const void* X, const void* residual, const vo
     if (int rc = get_device_info(&dev)) return rc;
     auto in = [](const void* p) { return static_cast<const uint8_t*>(p); };
     return launch(NormArgs{in(X), in(residual), in(weight), static_cast<uint8_t*>(sum), static_cast<uint8_t*>(Y), Q, scales, eps, rows, cols},
-                  static_cast<hipStream_t>(stream));
+                  dev->cu_count, static_cast<hipStream_t>(stream));
 }

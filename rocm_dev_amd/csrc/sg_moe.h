@@ -24,10 +24,10 @@ constexpr int kMoeFused = 8;        // tokens whose experts every workgroup choo
 struct MoePlanLayout {
     int parts_at, first_at, rows_at, weights_at, dwords, most;
 };
-__host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int top_k) {
+__host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int top_k, int cols) {
     const int pairs = m * top_k;
     MoePlanLayout l;
-    l.most = (experts < pairs ? experts : pairs) + pairs / 4;       // parts; COLS is at least 4
+    l.most = (experts < pairs ? experts : pairs) + pairs / cols;      // parts
     l.parts_at = 4;
     l.first_at = l.parts_at + l.most;
     l.rows_at = l.first_at + l.most;
@@ -36,18 +36,24 @@ __host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int
     return l;
 }
 
+// A tile's workgroups in the down projections: at most kMoeSplits of them, and kMoeSplitRows rows of partial sums in all.
+constexpr int kMoeSplits = 8, kMoeSplitRows = 16384;
+inline int moe_most_splits(int hidden) { return kMoeSplits * hidden <= kMoeSplitRows ? kMoeSplits : hidden < kMoeSplitRows ? kMoeSplitRows / hidden : 1; }
+
 struct MoeLayout {
-    size_t plan_at, h_at, bytes;     // logits first
+    size_t plan_at, h_at, sums_at, bytes;     // logits first
 };
 inline bool moe_takes(int m, int hidden, int inner, int experts, int top_k) {
     return m > 0 && m <= kMoeTokens && hidden > 0 && hidden % 16 == 0 && hidden <= kMoeSide && inner > 0 && inner % 16 == 0 &&
            inner <= kMoeSide && experts > 0 && experts <= kMoeExperts && top_k > 0 && top_k <= kMoeTopK && top_k <= experts;
 }
-inline MoeLayout moe_layout(int m, int inner, int experts, int top_k) {
+inline MoeLayout moe_layout(int m, int hidden, int inner, int experts, int top_k) {
     MoeLayout l;
     l.plan_at = ((size_t)m * experts * 4 + 255) / 256 * 256;
-    l.h_at = l.plan_at + ((size_t)moe_plan_layout(m, experts, top_k).dwords * 4 + 255) / 256 * 256;
-    l.bytes = l.h_at + (size_t)m * top_k * inner * 2;
+    l.h_at = l.plan_at + ((size_t)moe_plan_layout(m, experts, top_k, 4).dwords * 4 + 255) / 256 * 256;
+    l.sums_at = l.h_at + ((size_t)m * top_k * inner * 2 + 255) / 256 * 256;
+    const int splits = moe_most_splits(hidden);
+    l.bytes = l.sums_at + (splits > 1 ? (size_t)splits * m * hidden * 4 : 0);
     return l;
 }
 
@@ -65,6 +71,8 @@ struct MoeArgs {
     int32_t* plan;
     uint8_t* H;                      // [m * top_k][inner] bf16
     int m, hidden, inner, experts, top_k, renormalize;
+    float* sums;                     // [splits][m][hidden]
+    int splits;                      // down projections: workgroups that share a tile's steps
     int share;                       // gate and up: waves that share an item's columns (1, 2, 4)
 };
 

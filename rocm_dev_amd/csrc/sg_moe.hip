@@ -22,33 +22,72 @@ constexpr size_t kLdsBytes = 160 * 1024;      // a CU's
 
 template <int XU, int DEPTH>
 static size_t gate_up_lds(const MoeArgs& a) {
-    using Stages = MoeStages<2, XU>;
+    using Stages = MoeStages<2, XU, false>;
     const size_t ring = (size_t)4 * DEPTH * Stages::kBytes, room = moe_plan_room(a.m * a.top_k);
-    return (size_t)moe_plan_layout(a.m, a.experts, a.top_k).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) + (room > ring ? room : ring);
+    return (size_t)moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) +
+           (room > ring ? room : ring);
 }
-template <int XU, int DEPTH, bool CHOOSE>
-static int launch_gate_up(const MoeArgs& a, long long groups, int cu_count, hipStream_t stream) {
+template <int XU, int DEPTH, bool LINES>
+static int launch_gate_up(const MoeArgs& a, bool choose, long long groups, int cu_count, hipStream_t stream) {
     const size_t lds = gate_up_lds<XU, DEPTH>(a);
     const long long at_once = (long long)(kLdsBytes / lds) * cu_count;
     const unsigned grid = (unsigned)(groups < at_once ? groups : at_once);
-    static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_gate_up_kernel<XU, DEPTH, CHOOSE>), lds, granted)) return rc;
-    moe_gate_up_kernel<XU, DEPTH, CHOOSE><<<grid, 256, lds, stream>>>(a);
+    auto* const kernel = choose ? moe_gate_up_kernel<XU, DEPTH, LINES, true> : moe_gate_up_kernel<XU, DEPTH, LINES, false>;
+    static LdsGranted granted[2];
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, granted[choose])) return rc;
+    kernel<<<grid, 256, lds, stream>>>(a);
     return launched("moe_gate_up launch");
 }
 
 template <int XU, int DEPTH, int WAVES>
 static size_t down_lds(const MoeArgs& a) {
-    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
-    return (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64 + (size_t)WAVES * DEPTH * MoeStages<1, XU>::kBytes;
+    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, 4 * XU);
+    return (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64 + (size_t)WAVES * DEPTH * MoeStages<1, XU, false>::kBytes;
 }
-template <int XU, int DEPTH, int WAVES>
+template <int XU, int DEPTH, bool LINES, int WAVES>
 static int launch_down(const MoeArgs& a, hipStream_t stream) {
     const size_t lds = down_lds<XU, DEPTH, WAVES>(a);
     static LdsGranted granted;
-    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<XU, DEPTH, WAVES>), lds, granted)) return rc;
-    moe_down_kernel<XU, DEPTH, WAVES><<<a.hidden / 16, 64 * WAVES, lds, stream>>>(a);
+    if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<XU, DEPTH, LINES, WAVES>), lds, granted)) return rc;
+    moe_down_kernel<XU, DEPTH, LINES, WAVES><<<(unsigned)(a.hidden / 16 * a.splits), 64 * WAVES, lds, stream>>>(a);
     return launched("moe_down launch");
+}
+
+static bool off_lines(const uint8_t* weights, int columns) { return columns % 128 != 0 || (reinterpret_cast<uintptr_t>(weights) & 127u) != 0; }
+
+// waves: four, or eight where the rings fit.
+template <int XU, int N>
+static int launch_down_parts(const MoeArgs& a, int waves, hipStream_t stream) {
+    if (off_lines(a.W2, a.inner)) {
+        constexpr int L = N < 3 ? 3 : N;
+        if (waves == 8 && down_lds<XU, L, 8>(a) <= kLdsBytes) return launch_down<XU, L, true, 8>(a, stream);
+        if (waves == 8 && down_lds<XU, 3, 8>(a) <= kLdsBytes) return launch_down<XU, 3, true, 8>(a, stream);
+        if (down_lds<XU, 3, 4>(a) <= kLdsBytes) return launch_down<XU, 3, true, 4>(a, stream);
+    }
+    if (waves == 8 && down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, false, 8>(a, stream);
+    if (waves == 8 && down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, false, 8>(a, stream);
+    return launch_down<XU, 2, false, 4>(a, stream);
+}
+
+// How many workgroups share a tile of the down projections, and how many waves they have: eight, one workgroup a CU, or four, two.
+// Shared sums pay a launch that adds them up.  (2064 rows, 40 experts x 1376, 61 tokens: 129 tiles as they are 39.6 us, three workgroups each
+// 30.8 and 4.6 for the sums.  Sums joined by the last workgroup to arrive instead: 95 us, for the fences that write the L2s back.)
+static int down_splits(const MoeArgs& a, int cu_count, int* waves) {
+    const int tiles = a.hidden / 16, most = moe_most_splits(a.hidden);
+    const float bytes = a.experts * (1.0f - powf(1.0f - (float)a.top_k / a.experts, (float)a.m)) * a.hidden * (float)a.inner;
+    const long long steps = (long long)((a.inner + 127) / 128) * a.top_k;      // of one token: there are more
+    float best = 0.0f;
+    int splits = 1;
+    *waves = 8;
+    for (int w = 8; w >= 4; w -= 4)
+        for (int s = 1; s <= most && (s == 1 || steps >= 2ll * s * w); s++) {
+            const int slots = cu_count * (8 / w), all = tiles * s;
+            // of the memory's rate, 6 TB/s: a CU by itself takes in up to 1.4 times its part of it.  Sums are written and read at 4 TB/s.
+            const float used = (float)all / (float)((all + slots - 1) / slots * slots), rate = 1.4f * used < 1.0f ? 1.4f * used : 1.0f;
+            const float us = bytes / (6.0e6f * rate) + (s > 1 ? 4.0f + (float)s * a.m * a.hidden * 8 / 4e6f : 0.0f);
+            if (best == 0.0f || us < 0.97f * best) best = us, splits = s, *waves = w;
+        }
+    return splits;
 }
 
 // Parts of up to 4 * XU tokens; G and N stages in flight a wave.
@@ -56,28 +95,58 @@ template <int XU, int G, int N>
 static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
     const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
     const long long items = (long long)most * (a.inner / 16);
-    a.share = 1;
-    while (a.share < 4 && items * a.share < 16ll * cu_count && steps >= 4 * a.share) a.share *= 2;
-    const long long groups = (items * a.share + 3) / 4;
-    // A few workgroups more than fit at once would take as long again: shorter rings then, if all fit with them.
-    const bool shorter = groups > (long long)(kLdsBytes / gate_up_lds<XU, G>(a)) * cu_count && groups <= (long long)(kLdsBytes / gate_up_lds<XU, 2>(a)) * cu_count;
+    int waves;
+    a.splits = down_splits(a, cu_count, &waves);
+    // Waves that share an item, and stages in flight: what leaves the least to the last round.
+    const bool lines = off_lines(a.W1, a.hidden) && (a.share = 4, gate_up_lds<XU, 3>(a) <= kLdsBytes);
+    float best = 0.0f;
+    int share = 1;
+    bool shorter = false;
+    for (a.share = 1; a.share <= 4 && (a.share == 1 || steps >= 2 * a.share); a.share *= 2)
+        for (int s = 0; s < (lines ? 1 : 2); s++) {
+            const size_t lds = lines ? gate_up_lds<XU, 3>(a) : s ? gate_up_lds<XU, 2>(a) : gate_up_lds<XU, G>(a);
+            const long long slots = (long long)(kLdsBytes / lds) * cu_count * 4;
+            const float rounds = (float)((items * a.share + slots - 1) / slots) / a.share;
+            if (best == 0.0f || rounds < 0.97f * best) best = rounds, share = a.share, shorter = s;
+        }
+    a.share = share;
+    const long long groups = (items * share + 3) / 4;
     int rc;
-    if (choose) rc = shorter ? launch_gate_up<XU, 2, true>(a, groups, cu_count, stream) : launch_gate_up<XU, G, true>(a, groups, cu_count, stream);
-    else rc = shorter ? launch_gate_up<XU, 2, false>(a, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, groups, cu_count, stream);
-    if (rc) return rc;
-    if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, 8>(a, stream);
-    if (down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, 8>(a, stream);
-    return launch_down<XU, 2, 4>(a, stream);
+    if (lines) rc = launch_gate_up<XU, 3, true>(a, choose, groups, cu_count, stream);
+    else rc = shorter ? launch_gate_up<XU, 2, false>(a, choose, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, choose, groups, cu_count, stream);
+    if (!rc) rc = launch_down_parts<XU, N>(a, waves, stream);
+    if (rc || a.splits == 1) return rc;
+    moe_sum_kernel<<<(unsigned)((a.m * (long long)a.hidden + 1023) / 1024), 256, 0, stream>>>(a);
+    return (int)hipGetLastError();
 }
+
+// How many columns a part has.  An expert's tokens are as many as independent choices of top_k / experts give; each part reads the expert's
+// weights, 6 KB a stage of gate, up and down, beside XU KB of activations, which come out of the caches (0.2 of a KB by how it weighed: 32
+// tokens on 128 experts 330 us in parts of 4, 312 in parts of 8).
+static int part_columns(const MoeArgs& a) {
+    const float p = (float)a.top_k / a.experts;
+    float cost[4] = {};
+    float chance = 1.0f;                                     // of n tokens
+    for (int i = 0; i < a.m; i++) chance *= 1.0f - p;
+    if (chance < 1e-30f) return a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : 8;      // (nearly) every token
+    for (int n = 1; n <= a.m; n++) {
+        chance *= (float)(a.m - n + 1) / n * p / (1.0f - p);
+        for (int c = 0; c < 4; c++) cost[c] += chance * (float)((n - 1) / (4 << c) + 1) * (6.0f + 0.2f * (1 << c));
+    }
+    int best = 0;
+    for (int c = 1; c < 4; c++)
+        if (cost[c] < cost[best]) best = c;
+    return 1 << best;
+}
+
 // choose: by the logits, in the gate's launch
 static int launch_experts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
-    // Columns for an expert's tokens: as many as independent choices of m * top_k / experts on average rarely exceed.
-    const float mean = (float)a.m * a.top_k / a.experts, want = mean + 3.0f * sqrtf(mean);
-    const float columns = want < a.m ? want : a.m;
-    if (columns <= 4) return launch_parts<1, 3, 5>(a, choose, cu_count, stream);
-    if (columns <= 8) return launch_parts<2, 3, 4>(a, choose, cu_count, stream);
-    if (columns <= 16) return launch_parts<4, 2, 3>(a, choose, cu_count, stream);
-    return launch_parts<8, 2, 2>(a, choose, cu_count, stream);
+    switch (part_columns(a)) {
+        case 1: return launch_parts<1, 3, 5>(a, choose, cu_count, stream);
+        case 2: return launch_parts<2, 3, 4>(a, choose, cu_count, stream);
+        case 4: return launch_parts<4, 2, 3>(a, choose, cu_count, stream);
+        default: return launch_parts<8, 2, 2>(a, choose, cu_count, stream);
+    }
 }
 
 }  // namespace sg
@@ -94,7 +163,7 @@ int begin(MoeArgs& a, const void* X, const int32_t* ids, const float* weights, i
     if (off(X, 16) || off(ids, 4) || off(weights, 4)) return SG_BAD_ALIGNMENT;
     if (!workspace || workspace_bytes < need) return SG_WORKSPACE_TOO_SMALL;
     if (off(workspace, 256)) return SG_BAD_ALIGNMENT;
-    const MoeLayout l = moe_layout(m, inner, experts, top_k);
+    const MoeLayout l = moe_layout(m, hidden, inner, experts, top_k);
     uint8_t* const w = static_cast<uint8_t*>(workspace);
     a.X = static_cast<const uint8_t*>(X);
     a.ids = const_cast<int32_t*>(ids);
@@ -102,6 +171,7 @@ int begin(MoeArgs& a, const void* X, const int32_t* ids, const float* weights, i
     a.logits = reinterpret_cast<float*>(w);
     a.plan = reinterpret_cast<int32_t*>(w + l.plan_at);
     a.H = w + l.h_at;
+    a.sums = reinterpret_cast<float*>(w + l.sums_at);
     a.m = m;
     a.hidden = hidden;
     a.inner = inner;
@@ -131,7 +201,7 @@ int take_router(MoeArgs& a, const void* R, int renormalize) {
 extern "C" {
 
 size_t sg_moe_workspace_bytes(int m, int hidden, int inner, int experts, int top_k) {
-    return moe_takes(m, hidden, inner, experts, top_k) ? moe_layout(m, inner, experts, top_k).bytes : 0;
+    return moe_takes(m, hidden, inner, experts, top_k) ? moe_layout(m, hidden, inner, experts, top_k).bytes : 0;
 }
 
 int sg_moe_route(const void* X, const void* R, int32_t* ids, float* weights, int m, int hidden, int experts, int top_k, int renormalize,

@@ -44,7 +44,12 @@ __device__ __forceinline__ const uint8_t* moe_uniform(const uint8_t* p) {
 // Stages of 128 columns of RT 16-row tiles of weights and of 4 * XU rows of activations.
 // Columns: lane (r, g) takes the 16-byte pieces g and 4 + g of its weight row, codes 64 h + 16 g + 8 t .. + 7 for instruction (h, t), and
 // of its activations' row the same columns, piece 8 h + 2 g + t.
-template <int RT, int XU>
+//
+// LINES: rows that do not start on a 128-byte line (their pitch, a multiple of 16 bytes, is no multiple of 128).  128 bytes from anywhere lie on
+// two lines, and the next stage would ask for the second one again; so a stage's weights are the lines of each row, stage s its line s, and
+// a row that starts `shift` pieces into its first line has the columns of step s in stages s and s + 1: the shift is applied where
+// fragments are read, and a run of n steps takes n + 1 stages.  16 rows are a multiple of 256 bytes: a lane's shift is the same everywhere.
+template <int RT, int XU, bool LINES>
 struct MoeStages {
     static constexpr int kRows = 4 * XU, kBlocks = XU < 4 ? 1 : XU / 4;      // activation rows, blocks of 16 columns of the product
     static constexpr int kLoads = 2 * RT + XU, kBytes = kLoads * 1024;
@@ -52,32 +57,38 @@ struct MoeStages {
     uint32_t wo[2];                   // the lane's rows of a tile's loads, bytes from the first row
     int wp[2], xp[XU];                // ... and its pieces of stage 0
     int wr[2], xr[4];                 // where its fragments lie in a slot: pieces g and 4 + g; pieces (h, t) at 2 h + t
+    bool behind[2];                   // LINES: the piece is in the next stage
 
-    __device__ __forceinline__ void init(int columns) {
+    // weights: any tile's first row
+    __device__ __forceinline__ void init(const uint8_t* weights, int columns) {
         const int l = lane_id(), r = l & 15, g = l >> 4;
+        auto shift = [&](int row) { return LINES ? (int)((uint32_t)(reinterpret_cast<uintptr_t>(weights) + (uint32_t)(row * columns)) & 127u) >> 4 : 0; };
         pieces = columns / 16;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int row = 8 * u + (l >> 3);
             wo[u] = (uint32_t)(row * columns);
-            wp[u] = (l & 7) ^ (row >> 1);
+            wp[u] = ((l & 7) ^ (row >> 1)) - shift(row);
         }
 #pragma unroll
-        for (int u = 0; u < XU; u++) xp[u] = (l & 15) ^ (4 * u + (l >> 4) & 15);
+        for (int u = 0; u < XU; u++) xp[u] = (l & 15) ^ ((4 * u + (l >> 4)) & 15);
         const int at = r % (kRows < 16 ? kRows : 16);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            wr[h] = r * 128 + ((4 * h + g) ^ (r >> 1)) * 16;
+            const int place = 4 * h + g + shift(r);
+            behind[h] = place >= 8;
+            wr[h] = r * 128 + ((place & 7) ^ (r >> 1)) * 16;
 #pragma unroll
             for (int t = 0; t < 2; t++) xr[2 * h + t] = at * 256 + ((8 * h + 2 * g + t) ^ at) * 16;
         }
     }
-    // wb: the tiles' first rows; xb, xo: the activations and the lane's rows there, bytes.  A piece beyond a row's end is its last one again.
+    // wb: the tiles' first rows; xb, xo: the activations and the lane's rows there, bytes.  A piece beyond a row's ends is its first or last one.
     __device__ __forceinline__ void issue(unsigned slot, const uint8_t* const (&wb)[RT], const uint8_t* xb, const uint32_t (&xo)[XU], int step) const {
         uint32_t p[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int piece = 8 * step + wp[u];
+            int piece = 8 * step + wp[u];
+            if (LINES) piece = piece > 0 ? piece : 0;
             p[u] = wo[u] + (uint32_t)(piece < pieces ? piece : pieces - 1) * 16;
         }
 #pragma unroll
@@ -90,15 +101,15 @@ struct MoeStages {
             dma_1kb_at(xb, xo[u] + (uint32_t)(piece < 2 * pieces ? piece : 2 * pieces - 1) * 16, slot + (2 * RT + u) * 1024);
         }
     }
-    // Beyond the row's end the activations count as zeros.  (The weights there are the row's last ones again: a NaN among them is in the
-    // row's sum already, and there is no infinity in E4M3.)
-    __device__ __forceinline__ void multiply(const uint8_t* slot, f32x4 (&acc)[RT][kBlocks], int blocks, int step) const {
+    // next: the slot of the stage behind (LINES).  Beyond the row's end the activations count as zeros.  (The weights there are the row's
+    // first or last ones again: a NaN among them is in the row's sum already, and there is no infinity in E4M3.)
+    __device__ __forceinline__ void multiply(const uint8_t* slot, const uint8_t* next, f32x4 (&acc)[RT][kBlocks], int blocks, int step) const {
         const int g = lane_id() >> 4;
         u32x4 w[RT][2], x[kBlocks][4];
 #pragma unroll
         for (int i = 0; i < RT; i++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) w[i][h] = *reinterpret_cast<const u32x4*>(slot + 2048 * i + wr[h]);
+            for (int h = 0; h < 2; h++) w[i][h] = *reinterpret_cast<const u32x4*>((LINES && behind[h] ? next : slot) + 2048 * i + wr[h]);
 #pragma unroll
         for (int j = 0; j < kBlocks; j++)
 #pragma unroll
@@ -123,11 +134,13 @@ struct MoeStages {
     }
 };
 
-// Stage `at` of `total` has landed when at most the younger ones' loads are outstanding.
-template <int DEPTH, int LOADS>
+// Stage `at` of `total` has landed - LINES: and the one behind it - when at most the younger ones' loads are outstanding; DEPTH are issued
+// from `at` on.
+template <int DEPTH, int LOADS, bool LINES>
 __device__ __forceinline__ void moe_wait(int at, int total) {
-    if (at + DEPTH <= total) wait_vmcnt<(DEPTH - 1) * LOADS>();
-    else wait_vmcnt_upto((total - 1 - at) * LOADS);
+    static_assert(DEPTH >= (LINES ? 3 : 2));
+    if (at + DEPTH <= total) wait_vmcnt<(DEPTH - 1 - LINES) * LOADS>();
+    else wait_vmcnt_upto((total - 1 - LINES - at) * LOADS);
 }
 // All fragments are read: the slot may be filled again.
 __device__ __forceinline__ void moe_slot_read() {
@@ -171,15 +184,15 @@ __device__ __forceinline__ f32x4 moe_scales(const float* s, int g) {
 }
 
 // h = bf16( silu(S1 * (gate x)) * (S1 * (up x)) ).  An item is 16 gate rows and their 16 up rows of a part of the plan; `share` of a
-// workgroup's four waves share its columns, stage by stage in turn, and meet in LDS.  A wave's ring runs from one item into the next.
+// workgroup's four waves share its columns, a range each, and meet in LDS.  A wave's ring runs from one item into the next.
 // LDS: plan, [4 waves][2 * blocks][64 lanes] f32x4 where waves share, then the rings, and before them in their place the room for the plan.
-template <int XU, int DEPTH, bool CHOOSE>
+template <int XU, int DEPTH, bool LINES, bool CHOOSE>
 __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
-    using Stages = MoeStages<2, XU>;
+    using Stages = MoeStages<2, XU, LINES>;
     constexpr int BLOCKS = Stages::kBlocks;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
-    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
+    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows);
     const int share = a.share;
     f32x4* const part = reinterpret_cast<f32x4*>(lds + (size_t)l.dwords * 4);
     uint8_t* const rings = lds + (size_t)l.dwords * 4 + (share > 1 ? 4 * 2 * BLOCKS * 1024 : 0);
@@ -197,25 +210,25 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
     const int tiles = a.inner / 16, items = __builtin_amdgcn_readfirstlane(plan[0]) * tiles;
     const int steps = (a.hidden + 127) / 128, sharer = wave % share, stride = (int)gridDim.x * (4 / share);
     const int first = (int)blockIdx.x * (4 / share) + wave / share;
-    const int of_item = (steps - 1 - sharer) / share + 1;       // stages of an item (there are more steps than sharers)
-    const int total = first < items ? ((items - 1 - first) / stride + 1) * of_item : 0;
+    const int from = steps * sharer / share, of_item = steps * (sharer + 1) / share - from;       // (there are more steps than sharers)
+    const int total = first < items ? ((items - 1 - first) / stride + 1) * (of_item + LINES) : 0;
     Stages stages;
-    stages.init(a.hidden);
+    stages.init(a.W1, a.hidden);
     uint8_t* const ring = rings + wave * (DEPTH * Stages::kBytes);
     const unsigned ring_at = lds_addr(ring);
 
-    // An item's stages begin at another one in every item where rows are multiples of 512 bytes apart: waves that walk them in step meet in a
+    // An item's steps begin at another one in every item where rows are multiples of 512 bytes apart: waves that walk them in step meet in a
     // few memory channels then (hidden 4096: 229 -> 207 us).  Elsewhere waves in step share lines of the activations (2064: 60, 65 us).
-    const bool rotate = a.hidden % 512 == 0;
-    auto begin_of = [&](int item) { return rotate ? sharer + share * (int)((unsigned)item % (unsigned)of_item) : sharer; };
-    auto after = [&](int step) { return step + share < steps ? step + share : sharer; };
+    const bool rotate = !LINES && a.hidden % 512 == 0;
+    auto begin_of = [&](int item) { return rotate ? from + (int)((unsigned)item % (unsigned)of_item) : from; };
+    auto after = [&](int step) { return LINES || step + 1 < from + of_item ? step + 1 : from; };
     // ---- what to load next ----
     const uint8_t* wb[2] = {};
     uint32_t xo[XU] = {};
     int next_item = first, next_step = 0, next_left = 0, next_slot = 0, issued = 0;
     auto find = [&]() __attribute__((always_inline)) {
         next_step = begin_of(next_item);
-        next_left = of_item;
+        next_left = of_item + LINES;
         const int which = next_item / tiles, tile = next_item - which * tiles;
         const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]), e = packed & 0xffff, count = packed >> 16;
         const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
@@ -259,10 +272,17 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
                 for (int j = 0; j < BLOCKS; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             int step = begin_of(item);
             for (int left = of_item; left > 0; left--, at++, step = after(step)) {
-                moe_wait<DEPTH, Stages::kLoads>(at, total);
-                stages.multiply(ring + slot * Stages::kBytes, acc, blocks, step);
-                slot = slot + 1 == DEPTH ? 0 : slot + 1;
+                moe_wait<DEPTH, Stages::kLoads, LINES>(at, total);
+                const int next = slot + 1 == DEPTH ? 0 : slot + 1;
+                stages.multiply(ring + slot * Stages::kBytes, ring + next * Stages::kBytes, acc, blocks, step);
+                slot = next;
                 moe_slot_read();
+                if (issued < total) issue();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (LINES) {                 // the stage behind the last step is read
+                slot = slot + 1 == DEPTH ? 0 : slot + 1;
+                at++;
                 if (issued < total) issue();
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -304,20 +324,22 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
 // D = bf16( sum over experts of weight * S2 * (W2 h) ): a workgroup has 16 rows of hidden for all tokens, its waves share the stages of all
 // parts, in one range each.  A wave adds a part's product, scaled, to sums of its own - [tokens][16 rows] in LDS, where no other wave and
 // no second lane writes -, the waves' sums are added in wave order: no atomics, one order.
+// With fewer tiles than CUs, `splits` workgroups share a tile's steps, and moe_sum_kernel adds their sums up, in their order.
 // LDS: plan, S2 of the tile [parts][16], sums [waves][m][16], the rings.
-template <int XU, int DEPTH, int WAVES>
+template <int XU, int DEPTH, bool LINES, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
-    using Stages = MoeStages<1, XU>;
+    using Stages = MoeStages<1, XU, LINES>;
     constexpr int BLOCKS = Stages::kBlocks;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
-    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k);
+    const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows);
     float* const scales = reinterpret_cast<float*>(lds + (size_t)l.dwords * 4);
     float* const sums = scales + l.most * 16;
     const int tid = (int)threadIdx.x, lane = lane_id(), r = lane & 15, g = lane >> 4, wave = wave_id();
     uint8_t* const ring = reinterpret_cast<uint8_t*>(sums + WAVES * a.m * 16) + wave * (DEPTH * Stages::kBytes);
     const unsigned ring_at = lds_addr(ring);
-    const int tile = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int at_grid = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int tile = a.splits > 1 ? at_grid / a.splits : at_grid, split = a.splits > 1 ? at_grid - tile * a.splits : 0;
     for (int i = tid * 4; i < l.dwords; i += 64 * WAVES * 4) *reinterpret_cast<i32x4*>(plan + i) = *reinterpret_cast<const i32x4*>(a.plan + i);
     float* const own = sums + wave * a.m * 16;
     for (int i = lane; i < a.m * 16; i += 64) own[i] = 0.0f;
@@ -326,15 +348,19 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
     for (int i = tid; i < parts * 16; i += 64 * WAVES)      // row i % 16 for part i / 16
         scales[i] = a.S2 ? a.S2[(size_t)(plan[l.parts_at + (i >> 4)] & 0xffff) * a.hidden + tile * 16 + (i & 15)] : 1.0f;
 
-    const long long all = (long long)parts * steps, begin = all * wave / WAVES;
-    const int total = (int)(all * (wave + 1) / WAVES - begin);
+    const long long all = (long long)parts * steps;
+    const int sharer = split * WAVES + wave, sharers = a.splits * WAVES;
+    const long long begin = all * sharer / sharers, end = all * (sharer + 1) / sharers;
+    const int mine = (int)(end - begin);                     // steps; LINES: a stage more for each part that they touch
+    const int total = mine + (LINES && mine > 0 ? (int)((end - 1) / steps - begin / steps) + 1 : 0);
     Stages stages;
-    stages.init(a.inner);
+    stages.init(a.W2, a.inner);
     // ---- what to load next ----
     const uint8_t* wb[1] = {};
     uint32_t xo[XU] = {};
     int next_part = (int)(begin / steps), next_step = (int)(begin - (long long)next_part * steps), next_slot = 0, issued = 0;
     int part = next_part, step = next_step;                  // what to multiply next
+    int next_left = mine, next_of_part = 0;                  // steps to come, and stages of this part
     auto find = [&]() __attribute__((always_inline)) {
         const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + next_part]), e = packed & 0xffff, count = packed >> 16;
         const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + next_part]);
@@ -344,12 +370,16 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
             const int row = 4 * u + g;
             xo[u] = (uint32_t)rows[row < count ? row : count - 1] * (uint32_t)(a.inner * 2);
         }
+        const int here = steps - next_step < next_left ? steps - next_step : next_left;
+        next_left -= here;
+        next_of_part = here + LINES;
     };
     auto issue = [&]() __attribute__((always_inline)) {
         stages.issue(ring_at + next_slot * Stages::kBytes, wb, a.H, xo, next_step);
         next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
         issued++;
-        if (++next_step == steps) {
+        next_step++;
+        if (--next_of_part == 0) {
             next_step = 0;
             next_part++;
             if (issued < total) find();
@@ -360,17 +390,24 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
         for (int d = 0; d < DEPTH && d < total; d++) issue();
     }
     __syncthreads();                                         // the scales
-    for (int at = 0, slot = 0; at < total; part++, step = 0) {
+    for (int at = 0, slot = 0, left = mine; left > 0; part++, step = 0) {
         const int count = __builtin_amdgcn_readfirstlane(plan[l.parts_at + part]) >> 16, blocks = (count + 15) / 16;
         const int first = __builtin_amdgcn_readfirstlane(plan[l.first_at + part]);
         f32x4 acc[1][BLOCKS];
 #pragma unroll
         for (int j = 0; j < BLOCKS; j++) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (; step < steps && at < total; step++, at++) {
-            moe_wait<DEPTH, Stages::kLoads>(at, total);
-            stages.multiply(ring + slot * Stages::kBytes, acc, blocks, step);
-            slot = slot + 1 == DEPTH ? 0 : slot + 1;
+        for (; step < steps && left > 0; step++, at++, left--) {
+            moe_wait<DEPTH, Stages::kLoads, LINES>(at, total);
+            const int next = slot + 1 == DEPTH ? 0 : slot + 1;
+            stages.multiply(ring + slot * Stages::kBytes, ring + next * Stages::kBytes, acc, blocks, step);
+            slot = next;
             moe_slot_read();
+            if (issued < total) issue();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (LINES) {                     // the stage behind the last step is read
+            slot = slot + 1 == DEPTH ? 0 : slot + 1;
+            at++;
             if (issued < total) issue();
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -390,9 +427,24 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
         const int token = i >> 2, c = i & 3;
         f32x4 v = *reinterpret_cast<const f32x4*>(sums + token * 16 + 4 * c);
         for (int w = 1; w < WAVES; w++) v += *reinterpret_cast<const f32x4*>(sums + (w * a.m + token) * 16 + 4 * c);
-        const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-        *reinterpret_cast<u32x2*>(a.D + (size_t)token * a.hidden + tile * 16 + 4 * c) = o;
+        const size_t at = (size_t)token * a.hidden + tile * 16 + 4 * c;
+        if (a.splits > 1) {
+            *reinterpret_cast<f32x4*>(a.sums + (size_t)split * a.m * a.hidden + at) = v;
+        } else {
+            const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            *reinterpret_cast<u32x2*>(a.D + at) = o;
+        }
     }
+}
+
+// Four columns a thread.
+__global__ __launch_bounds__(256) void moe_sum_kernel(const MoeArgs a) {
+    const size_t n = (size_t)a.m * a.hidden, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= n) return;
+    f32x4 v = *reinterpret_cast<const f32x4*>(a.sums + at);
+    for (int s = 1; s < a.splits; s++) v += *reinterpret_cast<const f32x4*>(a.sums + s * n + at);
+    const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    *reinterpret_cast<u32x2*>(a.D + at) = o;
 }
 
 }  // namespace sg

@@ -109,6 +109,38 @@ def test_experts_larger(sg, m, experts, top_k, hidden, inner):
     check(experts_of(sg, X, ids, weights, E), *E.expected(X, ids, weights))
 
 
+@pytest.mark.parametrize("m,experts,top_k,hidden,inner", [(2, 6, 2, 512, 256), (20, 6, 3, 272, 400), (64, 4, 4, 1040, 144), (40, 64, 5, 640, 384)])
+@pytest.mark.parametrize("off", [16, 48, 112])
+def test_weights_off_their_lines(sg, m, experts, top_k, hidden, inner, off):
+    """Weights that start anywhere on a 128-byte line: the same values, to the order of the sums, as from its start."""
+    E = Experts(experts, hidden, inner, seed=31)
+    X = tokens(m, hidden, seed=32)
+    ids, weights = choices(m, experts, top_k, seed=33)
+
+    def moved(W, by):
+        out = torch.full((W.numel() + 256,), 0x7f, dtype=torch.uint8, device="cuda")      # NaNs around them
+        at = (by - out.data_ptr()) % 128
+        view = out[at:at + W.numel()].view(torch.float8_e4m3fn).view(W.shape)
+        view.copy_(W)
+        assert view.data_ptr() % 128 == by
+        return view
+    E.W1, E.W2 = moved(E.W1, off), moved(E.W2, (3 * off) % 128)
+    D = experts_of(sg, X, ids, weights, E)
+    check(D, *E.expected(X, ids, weights))
+    assert torch.equal(D, experts_of(sg, X, ids, weights, E))
+
+
+@pytest.mark.parametrize("m,experts,top_k,hidden,inner", [(1, 8, 4, 256, 16384), (16, 8, 4, 512, 4096), (61, 4, 3, 80, 16400), (33, 9, 9, 1040, 1936)])
+def test_few_rows_behind_long_ones(sg, m, experts, top_k, hidden, inner):
+    """Down projections of few rows and many columns: workgroups that share a tile, and their sums."""
+    E = Experts(experts, hidden, inner, seed=34)
+    X = tokens(m, hidden, seed=35)
+    ids, weights = choices(m, experts, top_k, seed=36)
+    D = experts_of(sg, X, ids, weights, E)
+    check(D, *E.expected(X, ids, weights))
+    assert torch.equal(D, experts_of(sg, X, ids, weights, E))
+
+
 @pytest.mark.parametrize("m", [3, 30, 64])
 def test_all_tokens_to_one_expert_and_no_scales(sg, m):
     E = Experts(9, 528, 400, seed=4, scales=False)

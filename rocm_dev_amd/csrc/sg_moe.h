@@ -18,9 +18,9 @@ constexpr int kMoeTopK = 16;
 constexpr int kMoeSide = 1 << 20;   // hidden, inner: rows of a tile, of all activations and of W1's count within 32 bits
 constexpr int kMoeFused = 8;        // tokens whose experts every workgroup chooses for itself
 
-// The plan: dwords [number of parts][part: expert | entries << 16][its first entry][entry: row of h = token * top_k + the choice that
-// names the expert first][its weight].  An entry is a token and an expert that it names; a part is up to COLS entries of one
-// expert, the columns of one product: an expert with more is read once for each part.
+// The plan: dwords [number of parts][part: expert | entries << 16][its first entry][entry: token << 16 | row of h = token * top_k + the
+// choice that names the expert first][its weight].  An entry is a token and an expert that it names; a part is up to COLS entries of one
+// expert, the columns of one product: an expert with more is read once for each part.  Gate and up keep it in LDS up to the weights.
 struct MoePlanLayout {
     int parts_at, first_at, rows_at, weights_at, dwords, most;
 };
@@ -32,6 +32,7 @@ __host__ __device__ inline MoePlanLayout moe_plan_layout(int m, int experts, int
     l.first_at = l.parts_at + l.most;
     l.rows_at = l.first_at + l.most;
     l.weights_at = l.rows_at + pairs;
+    l.weights_at = (l.weights_at + 3) / 4 * 4;
     l.dwords = (l.weights_at + pairs + 3) / 4 * 4;
     return l;
 }
@@ -73,7 +74,10 @@ struct MoeArgs {
     int m, hidden, inner, experts, top_k, renormalize;
     float* sums;                     // [splits][m][hidden]
     int splits;                      // down projections: workgroups that share a tile's steps
-    int share;                       // gate and up: waves that share an item's columns (1, 2, 4)
+    int share_log;                   // gate and up: 1 << this of four waves share an item's columns
+    int stride_parts, stride_tiles;  // ... and from a wave's item to its next one, as parts and tiles
+    uint32_t turn;                   // ... 2^32 / steps of a wave: the next tile begins a step later
+    uint32_t inv_tiles, inv_steps, inv_sharers;      // div_reciprocal: gate and up's tiles, the down projections' steps and sharers
 };
 
 }  // namespace sg

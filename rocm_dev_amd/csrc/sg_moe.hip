@@ -18,20 +18,26 @@ static int launch_choose(const MoeArgs& a, hipStream_t stream) {
     return launched("moe_choose launch");
 }
 
-constexpr size_t kLdsBytes = 160 * 1024;      // a CU's
+constexpr size_t kLdsBytes = 160 * 1024;      // a CU's, given out in pieces of 1280
+static int lds_workgroups(size_t lds) { return (int)(128 / ((lds + 1279) / 1280)); }
 
 template <int XU, int DEPTH>
 static size_t gate_up_lds(const MoeArgs& a) {
     using Stages = MoeStages<2, XU, false>;
     const size_t ring = (size_t)4 * DEPTH * Stages::kBytes, room = moe_plan_room(a.m * a.top_k);
-    return (size_t)moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows).dwords * 4 + (a.share > 1 ? 4 * 2 * Stages::kBlocks * 1024 : 0) +
-           (room > ring ? room : ring);
+    return (size_t)moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows).weights_at * 4 + 4 * (DEPTH + 2) * 128 +
+           (a.share_log > 0 ? 4 * 2 * Stages::kBlocks * 1024 : 0) + (room > ring ? room : ring);
 }
 template <int XU, int DEPTH, bool LINES>
-static int launch_gate_up(const MoeArgs& a, bool choose, long long groups, int cu_count, hipStream_t stream) {
+static int launch_gate_up(MoeArgs& a, bool choose, long long groups, int cu_count, hipStream_t stream) {
     const size_t lds = gate_up_lds<XU, DEPTH>(a);
-    const long long at_once = (long long)(kLdsBytes / lds) * cu_count;
+    const long long at_once = (long long)lds_workgroups(lds) * cu_count;
     const unsigned grid = (unsigned)(groups < at_once ? groups : at_once);
+    const long long stride = (long long)grid * 4 >> a.share_log;
+    a.stride_parts = (int)(stride / (a.inner / 16));
+    a.stride_tiles = (int)(stride % (a.inner / 16));
+    a.turn = (uint32_t)(0x100000000ull * (1u << a.share_log) / (unsigned)((a.hidden + 127) / 128) + 1);
+    a.inv_tiles = div_reciprocal((unsigned)a.inner / 16);
     auto* const kernel = choose ? moe_gate_up_kernel<XU, DEPTH, LINES, true> : moe_gate_up_kernel<XU, DEPTH, LINES, false>;
     static LdsGranted granted[2];
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, granted[choose])) return rc;
@@ -42,10 +48,12 @@ static int launch_gate_up(const MoeArgs& a, bool choose, long long groups, int c
 template <int XU, int DEPTH, int WAVES>
 static size_t down_lds(const MoeArgs& a) {
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, 4 * XU);
-    return (size_t)l.dwords * 4 + (size_t)l.most * 64 + (size_t)WAVES * a.m * 64 + (size_t)WAVES * DEPTH * MoeStages<1, XU, false>::kBytes;
+    return (size_t)l.dwords * 4 + WAVES * (DEPTH + 2) * 64 + (size_t)WAVES * a.m * 64 + (size_t)WAVES * DEPTH * MoeStages<1, XU, false>::kBytes;
 }
 template <int XU, int DEPTH, bool LINES, int WAVES>
-static int launch_down(const MoeArgs& a, hipStream_t stream) {
+static int launch_down(MoeArgs& a, hipStream_t stream) {
+    a.inv_steps = div_reciprocal((unsigned)(a.inner + 127) / 128);
+    a.inv_sharers = div_reciprocal((unsigned)(a.splits * WAVES));
     const size_t lds = down_lds<XU, DEPTH, WAVES>(a);
     static LdsGranted granted;
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(moe_down_kernel<XU, DEPTH, LINES, WAVES>), lds, granted)) return rc;
@@ -57,7 +65,7 @@ static bool off_lines(const uint8_t* weights, int columns) { return columns % 12
 
 // waves: four, or eight where the rings fit.
 template <int XU, int N>
-static int launch_down_parts(const MoeArgs& a, int waves, hipStream_t stream) {
+static int launch_down_parts(MoeArgs& a, int waves, hipStream_t stream) {
     if (off_lines(a.W2, a.inner)) {
         constexpr int L = N < 3 ? 3 : N;
         if (waves == 8 && down_lds<XU, L, 8>(a) <= kLdsBytes) return launch_down<XU, L, true, 8>(a, stream);
@@ -98,19 +106,19 @@ static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t strea
     int waves;
     a.splits = down_splits(a, cu_count, &waves);
     // Waves that share an item, and stages in flight: what leaves the least to the last round.
-    const bool lines = off_lines(a.W1, a.hidden) && (a.share = 4, gate_up_lds<XU, 3>(a) <= kLdsBytes);
+    const bool lines = off_lines(a.W1, a.hidden) && (a.share_log = 2, gate_up_lds<XU, 3>(a) <= kLdsBytes);
     float best = 0.0f;
-    int share = 1;
+    int share_log = 0;
     bool shorter = false;
-    for (a.share = 1; a.share <= 4 && (a.share == 1 || steps >= 2 * a.share); a.share *= 2)
+    for (a.share_log = 0; a.share_log <= 2 && (a.share_log == 0 || steps >= 2 << a.share_log); a.share_log++)
         for (int s = 0; s < (lines ? 1 : 2); s++) {
             const size_t lds = lines ? gate_up_lds<XU, 3>(a) : s ? gate_up_lds<XU, 2>(a) : gate_up_lds<XU, G>(a);
-            const long long slots = (long long)(kLdsBytes / lds) * cu_count * 4;
-            const float rounds = (float)((items * a.share + slots - 1) / slots) / a.share;
-            if (best == 0.0f || rounds < 0.97f * best) best = rounds, share = a.share, shorter = s;
+            const long long slots = (long long)lds_workgroups(lds) * cu_count * 4;
+            const float rounds = (float)(((items << a.share_log) + slots - 1) / slots) / (1 << a.share_log);
+            if (best == 0.0f || rounds < 0.97f * best) best = rounds, share_log = a.share_log, shorter = s;
         }
-    a.share = share;
-    const long long groups = (items * share + 3) / 4;
+    a.share_log = share_log;
+    const long long groups = ((items << share_log) + 3) / 4;
     int rc;
     if (lines) rc = launch_gate_up<XU, 3, true>(a, choose, groups, cu_count, stream);
     else rc = shorter ? launch_gate_up<XU, 2, false>(a, choose, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, choose, groups, cu_count, stream);

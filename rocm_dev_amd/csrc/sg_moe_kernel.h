@@ -134,13 +134,16 @@ struct MoeStages {
     }
 };
 
-// Stage `at` of `total` has landed - LINES: and the one behind it - when at most the younger ones' loads are outstanding; DEPTH are issued
-// from `at` on.
+// Of `flying` stages, DEPTH at most, the oldest - LINES: and the one behind it - has landed when at most the younger ones' loads are
+// outstanding.  `here` steps are left of its item, this one counted: with stages of the next item in flight, whose `scales` were asked for in
+// front of them, there is a load more: without it the last step of an item would wait for a load issued just before.
 template <int DEPTH, int LOADS, bool LINES>
-__device__ __forceinline__ void moe_wait(int at, int total) {
+__device__ __forceinline__ void moe_wait(int flying, int here, bool scales) {
     static_assert(DEPTH >= (LINES ? 3 : 2));
-    if (at + DEPTH <= total) wait_vmcnt<(DEPTH - 1 - LINES) * LOADS>();
-    else wait_vmcnt_upto((total - 1 - LINES - at) * LOADS);
+    const bool more = scales && flying > here + LINES;
+    if (flying != DEPTH) wait_vmcnt_upto((flying - 1 - LINES) * LOADS + more);
+    else if (more) wait_vmcnt<(DEPTH - 1 - LINES) * LOADS + 1>();
+    else wait_vmcnt<(DEPTH - 1 - LINES) * LOADS>();
 }
 // All fragments are read: the slot may be filled again.
 __device__ __forceinline__ void moe_slot_read() {
@@ -169,23 +172,21 @@ __device__ __forceinline__ float moe_silu(float v) {
     return v * ((v < 0.0f ? t : 1.0f) / (1.0f + t));
 }
 
-// 16 floats of a row scale: what lane (r, g) multiplies its rows 4 g .. 4 g + 3 with.  Scalar loads: a vector load here would be waited for
-// behind every stage in flight.
-__device__ __forceinline__ f32x4 moe_scales(const float* s, int g) {
-    if (!s) return f32x4{1.f, 1.f, 1.f, 1.f};
-    const __attribute__((address_space(4))) float* const c = (const __attribute__((address_space(4))) float*)s;
-    f32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float a = c[i], b = c[4 + i], d = c[8 + i], e = c[12 + i];
-        v[i] = g & 2 ? (g & 1 ? e : d) : (g & 1 ? b : a);
-    }
-    return v;
+// Row scales reach LDS as a product's operands do, by a load in front of its first stage: a vector load to registers would be waited for behind
+// every stage in flight, scalar loads 0.8 us at the head of an item.
+// A wave's ring has DEPTH stages in flight, each of an item of its own at the least, and one found that has none: DEPTH + 2 slots.
+// first, second: 16 floats each, by lanes 0 to 15 and 16 to 31 (second: or NULL)
+__device__ __forceinline__ void moe_issue_scales(const float* first, const float* second, unsigned slot) {
+    const int lane = lane_id();
+    const float* const from = (lane < 16 ? first : second) + (lane & 15);
+    slot = __builtin_amdgcn_readfirstlane(slot);
+    if (lane < (second ? 32 : 16)) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(slot) : "memory", "m0");
 }
 
 // h = bf16( silu(S1 * (gate x)) * (S1 * (up x)) ).  An item is 16 gate rows and their 16 up rows of a part of the plan; `share` of a
 // workgroup's four waves share its columns, a range each, and meet in LDS.  A wave's ring runs from one item into the next.
-// LDS: plan, [4 waves][2 * blocks][64 lanes] f32x4 where waves share, then the rings, and before them in their place the room for the plan.
+// LDS: plan, the waves' scales, [4 waves][2 * blocks][64 lanes] f32x4 where waves share, then the rings, and before them in their place
+// the room for the plan.
 template <int XU, int DEPTH, bool LINES, bool CHOOSE>
 __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
     using Stages = MoeStages<2, XU, LINES>;
@@ -193,107 +194,126 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows);
-    const int share = a.share;
-    f32x4* const part = reinterpret_cast<f32x4*>(lds + (size_t)l.dwords * 4);
-    uint8_t* const rings = lds + (size_t)l.dwords * 4 + (share > 1 ? 4 * 2 * BLOCKS * 1024 : 0);
+    const int share_log = a.share_log, share = 1 << share_log;
+    constexpr int SCALES = DEPTH + 2;
     const int lane = lane_id(), r = lane & 15, g = lane >> 4, wave = wave_id();
-    {
-        const MoePlanRoom room = moe_room(rings, a.m * a.top_k);
-        moe_make_plan<Stages::kRows, CHOOSE>(a, l, room, plan);
-        if (blockIdx.x == 0) {       // for the second launch, and the caller
-            for (int i = (int)threadIdx.x; i < l.dwords; i += 256) a.plan[i] = plan[i];
-            if (CHOOSE)
-                for (int i = (int)threadIdx.x; i < a.m * a.top_k; i += 256) a.ids[i] = room.ids[i], a.weights[i] = room.weights[i];
-        }
-        __syncthreads();
-    }
-    const int tiles = a.inner / 16, items = __builtin_amdgcn_readfirstlane(plan[0]) * tiles;
-    const int steps = (a.hidden + 127) / 128, sharer = wave % share, stride = (int)gridDim.x * (4 / share);
-    const int first = (int)blockIdx.x * (4 / share) + wave / share;
-    const int from = steps * sharer / share, of_item = steps * (sharer + 1) / share - from;       // (there are more steps than sharers)
-    const int total = first < items ? ((items - 1 - first) / stride + 1) * (of_item + LINES) : 0;
+    float* const scales = reinterpret_cast<float*>(lds + (size_t)l.weights_at * 4) + wave * SCALES * 32;
+    f32x4* const part = reinterpret_cast<f32x4*>(lds + (size_t)l.weights_at * 4 + 4 * SCALES * 128);
+    uint8_t* const rings = lds + (size_t)l.weights_at * 4 + 4 * SCALES * 128 + (share > 1 ? 4 * 2 * BLOCKS * 1024 : 0);
+    const int tiles = a.inner / 16, steps = (a.hidden + 127) / 128, sharer = wave & (share - 1), stride = (int)gridDim.x * 4 >> share_log;
+    const int first = ((int)blockIdx.x * 4 + wave) >> share_log;
+    const int from = steps * sharer >> share_log, of_item = (steps * (sharer + 1) >> share_log) - from;       // (there are more steps than sharers)
+    const int first_part = (int)fast_div((unsigned)first, (unsigned)tiles, a.inv_tiles);
     Stages stages;
     stages.init(a.W1, a.hidden);
+    if (CHOOSE && a.m == 1) {
+        if (wave == 0) moe_plan_token(a, l, blockIdx.x == 0, plan);
+        __syncthreads();
+    } else {
+        const MoePlanRoom room = moe_room(rings, a.m * a.top_k);
+        moe_make_plan<Stages::kRows, CHOOSE>(a, l, room, plan);
+        if (CHOOSE && blockIdx.x == 0)
+            for (int i = (int)threadIdx.x; i < a.m * a.top_k; i += 256) a.ids[i] = room.ids[i], a.weights[i] = room.weights[i];
+        __syncthreads();
+    }
+    if (blockIdx.x == 0)             // for the second launch
+        for (int i = (int)threadIdx.x; i < l.weights_at; i += 256) a.plan[i] = plan[i];
+    const int items = __builtin_amdgcn_readfirstlane(plan[0]) * tiles;
     uint8_t* const ring = rings + wave * (DEPTH * Stages::kBytes);
     const unsigned ring_at = lds_addr(ring);
 
-    // An item's steps begin at another one in every item where rows are multiples of 512 bytes apart: waves that walk them in step meet in a
-    // few memory channels then (hidden 4096: 229 -> 207 us).  Elsewhere waves in step share lines of the activations (2064: 60, 65 us).
+    // A tile's steps begin a step behind the one before where rows are multiples of 512 bytes apart: waves that walk them in step meet in a
+    // few memory channels then (hidden 4096: 229 -> 207 us).  Elsewhere waves in step share lines of the activations (2064: 60, with it 65 us).
     const bool rotate = !LINES && a.hidden % 512 == 0;
-    auto begin_of = [&](int item) { return rotate ? from + (int)((unsigned)item % (unsigned)of_item) : from; };
+    auto begin_of = [&](int tile) { return rotate ? from + (int)((uint64_t)((uint32_t)tile * a.turn) * (uint32_t)of_item >> 32) : from; };
     auto after = [&](int step) { return LINES || step + 1 < from + of_item ? step + 1 : from; };
     // ---- what to load next ----
     const uint8_t* wb[2] = {};
     uint32_t xo[XU] = {};
-    int next_item = first, next_step = 0, next_left = 0, next_slot = 0, issued = 0;
+    struct Item {
+        int part, tile;
+    };
+    auto advance = [&](Item& i) __attribute__((always_inline)) {
+        i.part += a.stride_parts;
+        i.tile += a.stride_tiles;
+        if (i.tile >= tiles) i.tile -= tiles, i.part++;
+    };
+    Item next = {first_part, first - first_part * tiles};
+    int next_item = first, next_step = 0, next_left = 0, next_slot = 0, next_scales = 0, flying = 0;
     auto find = [&]() __attribute__((always_inline)) {
-        next_step = begin_of(next_item);
+        next_step = begin_of(next.tile);
         next_left = of_item + LINES;
-        const int which = next_item / tiles, tile = next_item - which * tiles;
-        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]), e = packed & 0xffff, count = packed >> 16;
-        const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
-        wb[0] = a.W1 + ((size_t)e * 2 * a.inner + tile * 16) * a.hidden;
+        const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + next.part]), e = packed & 0xffff, count = packed >> 16;
+        const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + next.part]);
+        wb[0] = a.W1 + ((size_t)e * 2 * a.inner + next.tile * 16) * a.hidden;
         wb[1] = wb[0] + (size_t)a.inner * a.hidden;
 #pragma unroll
         for (int u = 0; u < XU; u++) {
             const int row = 4 * u + g;
-            xo[u] = (uint32_t)rows[row < count ? row : count - 1] / (uint32_t)a.top_k * (uint32_t)(a.hidden * 2);
+            xo[u] = (uint32_t)(rows[row < count ? row : count - 1] >> 16) * (uint32_t)(a.hidden * 2);
+        }
+        if (a.S1) {
+            const float* const s = a.S1 + (e * 2 * a.inner + next.tile * 16);      // below 2^31
+            moe_issue_scales(s, s + a.inner, lds_addr(scales + next_scales * 32));
+            next_scales = next_scales + 1 == SCALES ? 0 : next_scales + 1;
         }
     };
     auto issue = [&]() __attribute__((always_inline)) {
         stages.issue(ring_at + next_slot * Stages::kBytes, wb, a.X, xo, next_step);
         next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
-        issued++;
+        flying++;
         next_step = after(next_step);
         if (--next_left == 0) {
+            advance(next);
             next_item += stride;
-            if (issued < total) find();
+            if (next_item < items) find();
         }
     };
-    if (total > 0) {
+    if (first < items) {
         find();
-        for (int d = 0; d < DEPTH && d < total; d++) issue();
+        for (int d = 0; d < DEPTH && next_item < items; d++) issue();
     }
-    int at = 0, slot = 0, item = first;
-    for (int round = (int)blockIdx.x * (4 / share); round < items; round += stride, item += stride) {
+    int slot = 0, item = first, scales_at = 0;
+    Item now = {first_part, first - first_part * tiles};
+    for (int round = (int)blockIdx.x * 4 >> share_log; round < items; round += stride, item += stride, advance(now)) {
         f32x4 acc[2][BLOCKS];
-        int count = 0, blocks = 0, entry = 0, tile = 0, row = 0;       // row of W1's rows of all experts: below 2^31
+        int count = 0, blocks = 0, entry = 0;
         if (item < items) {
-            const int which = item / tiles;
-            tile = item - which * tiles;
-            const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + which]);
+            const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + now.part]);
             count = packed >> 16;
             blocks = (count + 15) / 16;
-            entry = l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + which]);
-            row = (packed & 0xffff) * 2 * a.inner + tile * 16;
+            entry = l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + now.part]);
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < BLOCKS; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            int step = begin_of(item);
-            for (int left = of_item; left > 0; left--, at++, step = after(step)) {
-                moe_wait<DEPTH, Stages::kLoads, LINES>(at, total);
+            int step = begin_of(now.tile);
+            for (int left = of_item; left > 0; left--, step = after(step)) {
+                moe_wait<DEPTH, Stages::kLoads, LINES>(flying, left, a.S1 != nullptr);
                 const int next = slot + 1 == DEPTH ? 0 : slot + 1;
                 stages.multiply(ring + slot * Stages::kBytes, ring + next * Stages::kBytes, acc, blocks, step);
                 slot = next;
                 moe_slot_read();
-                if (issued < total) issue();
+                flying--;
+                if (next_item < items) issue();
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (LINES) {                 // the stage behind the last step is read
                 slot = slot + 1 == DEPTH ? 0 : slot + 1;
-                at++;
-                if (issued < total) issue();
+                flying--;
+                if (next_item < items) issue();
                 __builtin_amdgcn_sched_barrier(0);
             }
             moe_settle(acc);
         }
         auto finish = [&](f32x4 gate, f32x4 up, int j) __attribute__((always_inline)) {
-            gate *= moe_scales(a.S1 ? a.S1 + row : nullptr, g);
-            up *= moe_scales(a.S1 ? a.S1 + row + a.inner : nullptr, g);
+            if (a.S1) {
+                gate *= *reinterpret_cast<const f32x4*>(scales + scales_at * 32 + 4 * g);
+                up *= *reinterpret_cast<const f32x4*>(scales + scales_at * 32 + 16 + 4 * g);
+            }
             const u32x2 o = {pack_bf16x2(moe_silu(gate[0]) * up[0], moe_silu(gate[1]) * up[1]),
                              pack_bf16x2(moe_silu(gate[2]) * up[2], moe_silu(gate[3]) * up[3])};
-            if (16 * j + r < count) *reinterpret_cast<u32x2*>(a.H + ((size_t)plan[entry + 16 * j + r] * a.inner + tile * 16 + 4 * g) * 2) = o;
+            if (16 * j + r < count) *reinterpret_cast<u32x2*>(a.H + ((size_t)(plan[entry + 16 * j + r] & 0xffff) * a.inner + now.tile * 16 + 4 * g) * 2) = o;
         };
         if (share == 1) {
 #pragma unroll
@@ -318,6 +338,7 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
             }
             __syncthreads();
         }
+        scales_at = scales_at + 1 == SCALES ? 0 : scales_at + 1;
     }
 }
 
@@ -325,7 +346,7 @@ __global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeArgs a) {
 // parts, in one range each.  A wave adds a part's product, scaled, to sums of its own - [tokens][16 rows] in LDS, where no other wave and
 // no second lane writes -, the waves' sums are added in wave order: no atomics, one order.
 // With fewer tiles than CUs, `splits` workgroups share a tile's steps, and moe_sum_kernel adds their sums up, in their order.
-// LDS: plan, S2 of the tile [parts][16], sums [waves][m][16], the rings.
+// LDS: plan, the waves' scales, sums [waves][m][16], the rings.
 template <int XU, int DEPTH, bool LINES, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
     using Stages = MoeStages<1, XU, LINES>;
@@ -333,11 +354,12 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     int32_t* const plan = reinterpret_cast<int32_t*>(lds);
     const MoePlanLayout l = moe_plan_layout(a.m, a.experts, a.top_k, Stages::kRows);
-    float* const scales = reinterpret_cast<float*>(lds + (size_t)l.dwords * 4);
-    float* const sums = scales + l.most * 16;
+    constexpr int SCALES = DEPTH + 2;
+    float* const sums = reinterpret_cast<float*>(lds + (size_t)l.dwords * 4) + WAVES * SCALES * 16;
     const int tid = (int)threadIdx.x, lane = lane_id(), r = lane & 15, g = lane >> 4, wave = wave_id();
     uint8_t* const ring = reinterpret_cast<uint8_t*>(sums + WAVES * a.m * 16) + wave * (DEPTH * Stages::kBytes);
     const unsigned ring_at = lds_addr(ring);
+    float* const scales = reinterpret_cast<float*>(lds + (size_t)l.dwords * 4) + wave * SCALES * 16;
     const int at_grid = xcd_order((int)blockIdx.x, (int)gridDim.x);
     const int tile = a.splits > 1 ? at_grid / a.splits : at_grid, split = a.splits > 1 ? at_grid - tile * a.splits : 0;
     for (int i = tid * 4; i < l.dwords; i += 64 * WAVES * 4) *reinterpret_cast<i32x4*>(plan + i) = *reinterpret_cast<const i32x4*>(a.plan + i);
@@ -345,22 +367,17 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
     for (int i = lane; i < a.m * 16; i += 64) own[i] = 0.0f;
     __syncthreads();
     const int parts = __builtin_amdgcn_readfirstlane(plan[0]), steps = (a.inner + 127) / 128;
-    for (int i = tid; i < parts * 16; i += 64 * WAVES)      // row i % 16 for part i / 16
-        scales[i] = a.S2 ? a.S2[(size_t)(plan[l.parts_at + (i >> 4)] & 0xffff) * a.hidden + tile * 16 + (i & 15)] : 1.0f;
-
-    const long long all = (long long)parts * steps;
-    const int sharer = split * WAVES + wave, sharers = a.splits * WAVES;
-    const long long begin = all * sharer / sharers, end = all * (sharer + 1) / sharers;
-    const int mine = (int)(end - begin);                     // steps; LINES: a stage more for each part that they touch
-    const int total = mine + (LINES && mine > 0 ? (int)((end - 1) / steps - begin / steps) + 1 : 0);
+    const uint32_t all = (uint32_t)(parts * steps);          // up to 768 parts of 8192 steps, and 64 sharers
+    const uint32_t sharer = (uint32_t)(split * WAVES + wave), sharers = (uint32_t)(a.splits * WAVES);
+    const int begin = (int)fast_div(all * sharer, sharers, a.inv_sharers), mine = (int)fast_div(all * (sharer + 1), sharers, a.inv_sharers) - begin;
     Stages stages;
     stages.init(a.W2, a.inner);
     // ---- what to load next ----
     const uint8_t* wb[1] = {};
     uint32_t xo[XU] = {};
-    int next_part = (int)(begin / steps), next_step = (int)(begin - (long long)next_part * steps), next_slot = 0, issued = 0;
+    int next_part = (int)fast_div((unsigned)begin, (unsigned)steps, a.inv_steps), next_step = begin - next_part * steps, next_slot = 0, next_scales = 0, flying = 0;
     int part = next_part, step = next_step;                  // what to multiply next
-    int next_left = mine, next_of_part = 0;                  // steps to come, and stages of this part
+    int next_left = mine, next_of_part = 0;                  // steps of parts to come, and stages of this one (LINES: one more than steps)
     auto find = [&]() __attribute__((always_inline)) {
         const int packed = __builtin_amdgcn_readfirstlane(plan[l.parts_at + next_part]), e = packed & 0xffff, count = packed >> 16;
         const int32_t* const rows = plan + l.rows_at + __builtin_amdgcn_readfirstlane(plan[l.first_at + next_part]);
@@ -368,55 +385,62 @@ __global__ void __launch_bounds__(64 * WAVES) moe_down_kernel(const MoeArgs a) {
 #pragma unroll
         for (int u = 0; u < XU; u++) {
             const int row = 4 * u + g;
-            xo[u] = (uint32_t)rows[row < count ? row : count - 1] * (uint32_t)(a.inner * 2);
+            xo[u] = (uint32_t)(rows[row < count ? row : count - 1] & 0xffff) * (uint32_t)(a.inner * 2);
         }
         const int here = steps - next_step < next_left ? steps - next_step : next_left;
         next_left -= here;
         next_of_part = here + LINES;
+        if (a.S2) {
+            moe_issue_scales(a.S2 + ((size_t)e * a.hidden + tile * 16), nullptr, lds_addr(scales + next_scales * 16));
+            next_scales = next_scales + 1 == SCALES ? 0 : next_scales + 1;
+        }
     };
     auto issue = [&]() __attribute__((always_inline)) {
         stages.issue(ring_at + next_slot * Stages::kBytes, wb, a.H, xo, next_step);
         next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
-        issued++;
+        flying++;
         next_step++;
         if (--next_of_part == 0) {
             next_step = 0;
             next_part++;
-            if (issued < total) find();
+            if (next_left > 0) find();
         }
     };
-    if (total > 0) {
+    if (mine > 0) {
         find();
-        for (int d = 0; d < DEPTH && d < total; d++) issue();
+        for (int d = 0; d < DEPTH && next_of_part > 0; d++) issue();
     }
-    __syncthreads();                                         // the scales
-    for (int at = 0, slot = 0, left = mine; left > 0; part++, step = 0) {
+    int scales_at = 0;
+    for (int slot = 0, left = mine; left > 0; part++, step = 0) {
         const int count = __builtin_amdgcn_readfirstlane(plan[l.parts_at + part]) >> 16, blocks = (count + 15) / 16;
         const int first = __builtin_amdgcn_readfirstlane(plan[l.first_at + part]);
         f32x4 acc[1][BLOCKS];
 #pragma unroll
         for (int j = 0; j < BLOCKS; j++) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (; step < steps && left > 0; step++, at++, left--) {
-            moe_wait<DEPTH, Stages::kLoads, LINES>(at, total);
+        for (; step < steps && left > 0; step++, left--) {
+            moe_wait<DEPTH, Stages::kLoads, LINES>(flying, steps - step < left ? steps - step : left, a.S2 != nullptr);
             const int next = slot + 1 == DEPTH ? 0 : slot + 1;
             stages.multiply(ring + slot * Stages::kBytes, ring + next * Stages::kBytes, acc, blocks, step);
             slot = next;
             moe_slot_read();
-            if (issued < total) issue();
+            flying--;
+            if (next_of_part > 0) issue();
             __builtin_amdgcn_sched_barrier(0);
         }
         if (LINES) {                     // the stage behind the last step is read
             slot = slot + 1 == DEPTH ? 0 : slot + 1;
-            at++;
-            if (issued < total) issue();
+            flying--;
+            if (next_of_part > 0) issue();
             __builtin_amdgcn_sched_barrier(0);
         }
         moe_settle(acc);
-        const f32x4 scale = *reinterpret_cast<const f32x4*>(scales + part * 16 + 4 * g);
+        f32x4 scale = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (a.S2) scale = *reinterpret_cast<const f32x4*>(scales + scales_at * 16 + 4 * g);
+        scales_at = scales_at + 1 == SCALES ? 0 : scales_at + 1;
 #pragma unroll
         for (int j = 0; j < BLOCKS; j++)
             if (16 * j + r < count) {
-                const int entry = first + 16 * j + r, token = (int)((uint32_t)plan[l.rows_at + entry] / (uint32_t)a.top_k);
+                const int entry = first + 16 * j + r, token = plan[l.rows_at + entry] >> 16;
                 const float weight = __uint_as_float((uint32_t)plan[l.weights_at + entry]);
                 f32x4* const sum = reinterpret_cast<f32x4*>(own + token * 16 + 4 * g);
                 *sum += acc[0][j] * scale * weight;

@@ -99,9 +99,9 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 }
 
 // One wave: the top_k experts of a token and their weights, by top_k rounds of a maximum over the lanes' own logits.
-// PER: experts a lane, lane l has l, l + 64, ...  ids, weights: of the token.
+// PER: experts a lane, lane l has l, l + 64, ...  Lane c returns the c-th choice and, asked for it, its weight.
 template <int PER>
-__device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, int32_t* ids, float* weights) {
+__device__ __forceinline__ int moe_choose(const MoeArgs& a, int t, bool weighed, float& weight) {
     const int lane = lane_id();
     float v[PER];
     uint32_t key[PER];
@@ -138,7 +138,9 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, int32_t* ids
         if (c == 0) first = at;
         if (lane == c) mine = at, id = e;
     }
-    float p = expf(mine - first), all = 0.0f;
+    if (!weighed) return id;
+    const float p = expf(mine - first);
+    float all = 0.0f;
     if (a.renormalize) {
         all = lane < a.top_k ? p : 0.0f;
     } else {
@@ -147,23 +149,48 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, int32_t* ids
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-    if (lane < a.top_k) {
-        ids[lane] = id;
-        weights[lane] = p / all;
-    }
+    weight = p / all;
+    return id;
 }
 
-__device__ __forceinline__ void moe_choose_any(const MoeArgs& a, int t, int32_t* ids, float* weights) {
-    if (a.experts <= 64) moe_choose<1>(a, t, ids, weights);
-    else if (a.experts <= 128) moe_choose<2>(a, t, ids, weights);
-    else if (a.experts <= 256) moe_choose<4>(a, t, ids, weights);
-    else moe_choose<8>(a, t, ids, weights);
+__device__ __forceinline__ int moe_choose_any(const MoeArgs& a, int t, bool weighed, float& weight) {
+    if (a.experts <= 64) return moe_choose<1>(a, t, weighed, weight);
+    if (a.experts <= 128) return moe_choose<2>(a, t, weighed, weight);
+    if (a.experts <= 256) return moe_choose<4>(a, t, weighed, weight);
+    return moe_choose<8>(a, t, weighed, weight);
+}
+__device__ __forceinline__ void moe_choose_into(const MoeArgs& a, int t, int32_t* ids, float* weights) {
+    float weight = 0.0f;
+    const int id = moe_choose_any(a, t, true, weight);
+    if (lane_id() < a.top_k) {
+        ids[lane_id()] = id;
+        weights[lane_id()] = weight;
+    }
 }
 
 // A wave a token.
 __global__ void __launch_bounds__(64) moe_choose_kernel(const MoeArgs a) {
     const size_t at = (size_t)blockIdx.x * a.top_k;
-    moe_choose_any(a, (int)blockIdx.x, a.ids + at, a.weights + at);
+    moe_choose_into(a, (int)blockIdx.x, a.ids + at, a.weights + at);
+}
+
+// The plan of one token, by one wave: its choices in the order of their experts.  What the products wait for is this: the weights
+// are left to the workgroup that hands the plan on.
+__device__ __forceinline__ void moe_plan_token(const MoeArgs& a, const MoePlanLayout& l, bool hands_on, int32_t* plan) {
+    float weight = 0.0f;
+    const int lane = lane_id(), id = moe_choose_any(a, 0, hands_on, weight);
+    int at = 0;
+    for (int c = 0; c < a.top_k; c++) at += __builtin_amdgcn_readlane(id, c) < id;
+    if (lane >= a.top_k) return;
+    plan[0] = a.top_k;
+    plan[l.parts_at + at] = id | 1 << 16;
+    plan[l.first_at + at] = at;
+    plan[l.rows_at + at] = lane;
+    if (hands_on) {
+        a.plan[l.weights_at + at] = (int32_t)__float_as_uint(weight);
+        a.ids[lane] = id;
+        a.weights[lane] = weight;
+    }
 }
 
 // LDS that a workgroup makes the plan in.
@@ -185,12 +212,13 @@ __device__ __forceinline__ MoePlanRoom moe_room(uint8_t* at, int pairs) {
     return r;
 }
 
-// Who goes where, by a workgroup of 256 threads: the choices (made here, or the caller's) into the room, the plan into `plan`, both LDS.
+// Who goes where, by a workgroup of 256 threads: the choices (made here, or the caller's) into the room, the plan into `plan`, both LDS, but
+// for the weights: the workgroup that hands the plan on writes them to its place.
 template <int COLS, bool CHOOSE>
 __device__ __forceinline__ void moe_make_plan(const MoeArgs& a, const MoePlanLayout& l, const MoePlanRoom& room, int32_t* plan) {
     const int tid = (int)threadIdx.x, pairs = a.m * a.top_k;
     if (CHOOSE) {
-        for (int t = wave_id(); t < a.m; t += 4) moe_choose_any(a, t, room.ids + t * a.top_k, room.weights + t * a.top_k);
+        for (int t = wave_id(); t < a.m; t += 4) moe_choose_into(a, t, room.ids + t * a.top_k, room.weights + t * a.top_k);
     } else {
         for (int i = tid; i < pairs; i += 256) {
             room.ids[i] = a.ids[i];
@@ -251,8 +279,8 @@ __device__ __forceinline__ void moe_make_plan(const MoeArgs& a, const MoePlanLay
         const uint32_t lo = room.tokens[2 * e], hi = room.tokens[2 * e + 1];
         const int before = t < 32 ? __popc(lo & ((1u << t) - 1u)) : __popc(lo) + __popc(hi & ((1u << (t - 32)) - 1u));
         const int at = room.place[e] + before;
-        plan[l.rows_at + at] = i;
-        plan[l.weights_at + at] = (int32_t)__float_as_uint(weight);
+        plan[l.rows_at + at] = t << 16 | i;
+        if (blockIdx.x == 0) a.plan[l.weights_at + at] = (int32_t)__float_as_uint(weight);
     }
     __syncthreads();
 }

@@ -392,7 +392,7 @@ int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const
  *     scales[r] = absmax(y[r,:]) / 448 (1 if that is zero; NaNs do not count);   Q = e4m3_rne_sat(y / scales[r]), a NaN 0x7f
  * and, each if its pointer is not NULL, sum = v (the next residual) and Y = bf16(y) (a router's input).  residual and weight
  * ([cols]) may be NULL: nothing added, factors of 1.  sum may be X's or the residual's own memory; Q and Y overlap no input.
- * A row whose squares' sum is no finite fp32 has y = 0, or NaN where v is not finite.  cols must be a multiple of 16, all
+ * A row whose squares' sum is no finite fp32 has y = 0, or NaN where v * weight is not finite.  cols must be a multiple of 16, all
  * matrices and weight 16-byte aligned, scales 4-byte, eps finite and not negative. */
 int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const void* weight_bf16, void* sum_bf16, void* Y_bf16,
                         uint8_t* Q, float* scales, float eps, int rows, int cols, void* stream);
@@ -402,11 +402,13 @@ int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const voi
  *     D[i][j] = bf16( sum_k A[i][k] * (B[j][k] - zeros[j][g]) * scales[j][g] ),  g = k / group
  * Codes are 0..15, two a byte, the even column in the low nibble ([n][k / 2], row stride b_stride bytes); scales [n][k / group] are
  * bf16, or fp16 with SG_INT4_F16_SCALES; zeros [n][k / group] are bytes, used as they are, with SG_INT4_ZEROS, and 8 without.  k must be a
- * multiple of group.  sg_int4_pack lays the weights out as the matrix instruction takes them: once, when a program loads them, into
+ * multiple of group and at most 2^24.  sg_int4_pack lays the weights out as the matrix instruction takes them: once, when a program loads them, into
  * sg_int4_packed_bytes(n, k, group, flags) bytes (0 for what sg_int4_pack refuses), all of which are written.  sg_int4_gemm takes
  * that P with the same n, k, group and flags.  Any m >= 1; it is made for few rows, and beyond 64 reads the weights again for every 64.
  * Sums are fp32, in an order fixed by the shape: results are bit-reproducible.  Within a group the sum of A * (1 + B / 16) is corrected by the sum of A,
- * so a row of A with an infinity or a NaN has NaN outputs.
+ * so a row of A with an infinity or a NaN has NaN outputs.  Few weight rows with a long k share K among workgroups, in the stream's
+ * workspace (above), except under capture, where a launch uses none - its sums may then be added up in another order than an eager
+ * call's - as a call does that can get no device memory.
  * B, A and P 16-byte aligned (A's rows are k values apart), b_stride a multiple of 16 and at least k / 2, D 8-byte, scales 2-byte aligned. */
 #define SG_INT4_ZEROS 1
 #define SG_INT4_F16_SCALES 2
@@ -427,7 +429,7 @@ int    sg_int4_gemm(const void* A_bf16, const uint8_t* P, void* D_bf16, int m, i
  *   sg_moe_layer    both;  ids and weights are outputs
  * workspace: sg_moe_workspace_bytes(...) bytes of device memory (0 for sizes that are refused), 256-byte aligned, no content needed; calls in
  * stream order may share it, calls that overlap - recorded graphs that replay side by side too - need one each.  Nothing else is
- * allocated or kept.  1 <= m <= 64, hidden and inner multiples of 16, experts <= 512, top_k <= 16 and <= experts; X, R, W1, W2 and D
+ * allocated or kept.  1 <= m <= 64, hidden and inner multiples of 16 up to 2^20, experts <= 512, top_k <= 16 and <= experts; X, R, W1, W2 and D
  * 16-byte aligned, floats and ids 4-byte.  D must not overlap an input. */
 size_t sg_moe_workspace_bytes(int m, int hidden, int inner, int experts, int top_k);
 int sg_moe_route(const void* X_bf16, const void* R_bf16, int32_t* ids, float* weights, int m, int hidden, int experts, int top_k,

@@ -64,12 +64,6 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
 // 32.5 (the same, six splits; unsplit 91, 39 on four waves), 8192 x 28672 60 (eight splits; 97 on two waves).
 Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
     Int4Plan p{1, a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : a.m <= 32 ? 8 : 16, 1, 1, 1};
-#ifdef SG_SWEEP
-    {
-        p.nf = atoi(getenv("SW_NF")), p.nw = atoi(getenv("SW_NW")), p.kw = atoi(getenv("SW_KW")), p.splits = atoi(getenv("SW_SPLITS"));
-        return p;
-    }
-#endif
     if (p.xu <= 4) {
         p.nf = a.tiles > cu_count ? 2 : 1;
         const int groups = (a.tiles - 1) / p.nf + 1;

@@ -1,4 +1,7 @@
 """sg_int4_pack and sg_int4_gemm against the formula in 64 bits."""
+import random
+import threading
+
 import pytest
 import torch
 
@@ -175,3 +178,80 @@ def test_registered_operators(sg):
     assert torch.equal(P, w.P)
     assert torch.equal(torch.ops.sgemm.int4_gemm(A.t().contiguous().t(), P, 100, 64, True, True), run(sg, A, w))
     torch.library.opcheck(torch.ops.sgemm.int4_gemm.default, (A, P, 100, 64, True, True), test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("m,n,k,group", [(1, 1024, 32768, 128), (8, 512, 16384, 128), (30, 1040, 16384, 32), (64, 512, 16384, 64)])
+def test_k_shared_by_workgroups(sg, m, n, k, group):
+    """Few weight rows with a long k: parts of K are added up in the stream's workspace, or, recorded, not shared."""
+    w = Weights(sg, n, k, group, True, False, seed=13)
+    A = activations(m, k, seed=13)
+    want = check(sg, A, w)
+    ref, tol = w.expected(A)
+    outs, streams = [torch.empty_like(want) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for out, stream in zip(outs, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            sg.int4_gemm(A, w.P, out, **w.kw(), check=True)
+        graphs.append(graph)
+    recorded = None
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):      # side by side, beside an eager call
+            with torch.cuda.stream(stream):
+                graph.replay()
+        assert torch.equal(run(sg, A, w), want)
+        torch.cuda.synchronize()
+        recorded = outs[0].clone() if recorded is None else recorded
+        assert torch.equal(outs[0], recorded) and torch.equal(outs[1], recorded)
+    assert ((recorded.double() - ref).abs() <= tol).all()
+
+
+def test_threads_on_one_stream(sg):
+    """Calls that hand each other the stream's workspace, enqueued by two threads at once."""
+    ws = [Weights(sg, 512, 16384, 128, False, False, seed=s) for s in range(2)]
+    A = activations(8, 16384, seed=14)
+    want = [run(sg, A, w) for w in ws]
+    outs = [[torch.empty_like(t) for _ in range(20)] for t in want]
+    stream, codes = torch.cuda.Stream(), []
+
+    def work(w, out):
+        with torch.cuda.stream(stream):
+            for d in out:
+                codes.append(sg.int4_gemm(A, w.P, d, **w.kw()))
+    threads = [threading.Thread(target=work, args=args) for args in zip(ws, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [0] * 40
+    assert all(torch.equal(d, t) for out, t in zip(outs, want) for d in out)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_sizes(sg, seed):
+    rng = random.Random(seed)
+    group = rng.choice((32, 64, 128))
+    m, n, k = rng.randint(1, rng.choice((4, 16, 70))), rng.randint(1, rng.choice((300, 9000))), group * rng.randint(1, rng.choice((3000, 12000)) // group)
+    check(sg, activations(m, k, seed), Weights(sg, n, k, group, rng.random() < 0.5, rng.random() < 0.5, seed))
+
+
+def test_weights_beyond_4_gigabytes(sg):
+    n, k, group = 139264, 65536, 128
+    B = torch.randint(0, 256, (n, k // 2), device="cuda", dtype=torch.uint8)
+    S = (torch.rand((n, k // group), device="cuda") + 0.1).bfloat16()
+    P = torch.empty(sg.int4_packed_bytes(n, k, group), dtype=torch.uint8, device="cuda")
+    assert P.numel() > 2 ** 32
+    sg.int4_pack(B, S, P, check=True)
+    for m in (2, 40):
+        A = activations(m, k, seed=m)
+        D = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        sg.int4_gemm(A, P, D, group=group, check=True)
+        for rows in (slice(0, 64), slice(n - 64, n)):
+            w = Weights(sg, 64, k, group, False, False, seed=0)
+            w.B, w.S = B[rows], S[rows]
+            ref, tol = w.expected(A)
+            assert ((D[:, rows].double() - ref).abs() <= tol).all()

@@ -1,4 +1,6 @@
 """sg_moe_route, sg_moe_experts and sg_moe_layer against their formulas in 64 bits."""
+import random
+
 import pytest
 import torch
 
@@ -382,3 +384,61 @@ def test_a_block_of_a_decoder(sg):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((stream, O, Y, Q.view(torch.uint8), rows, shared, D, ids, weights), want))
         sg.int4_gemm(A, P, empty(m, hidden), group=64, check=True)
+
+
+def test_layers_on_two_streams_at_once(sg):
+    """Eager calls that overlap, each on its stream, without a workspace of the caller's."""
+    E = Experts(16, 512, 272, seed=40)
+    R = tokens(16, 512, seed=41)
+    for m in (1, 12):
+        Xs = [tokens(m, 512, seed=42 + s) for s in range(2)]
+
+        def layer(X):
+            D = torch.empty_like(X)
+            ids, weights = torch.empty((m, 3), dtype=torch.int32, device="cuda"), torch.empty((m, 3), device="cuda")
+            sg.moe_layer(X, R, E.W1, E.W2, D, ids, weights, E.S1, E.S2, check=True)
+            return D, ids, weights
+        want = [layer(X) for X in Xs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in Xs]
+        got = [[], []]
+        for _ in range(10):
+            for s, X in enumerate(Xs):
+                with torch.cuda.stream(streams[s]):
+                    got[s].append(layer(X))
+        torch.cuda.synchronize()
+        for s in range(2):
+            assert all(torch.equal(a, b) for g in got[s] for a, b in zip(g, want[s]))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_sizes(sg, seed):
+    rng = random.Random(seed)
+    m, experts = rng.randint(1, rng.choice((8, 64))), rng.randint(1, rng.choice((12, 130)))
+    top_k, hidden, inner = rng.randint(1, min(8, experts)), 16 * rng.randint(1, 160), 16 * rng.randint(1, 120)
+    E = Experts(experts, hidden, inner, seed, scales=rng.random() < 0.8)
+    X, R = tokens(m, hidden, seed + 100), tokens(experts, hidden, seed + 200)
+    D, ids, weights = torch.empty_like(X), torch.empty((m, top_k), dtype=torch.int32, device="cuda"), torch.empty((m, top_k), device="cuda")
+    assert sg.moe_layer(X, R, E.W1, E.W2, D, ids, weights, E.S1, E.S2) == 0
+    if E.S1 is None:                                        # few codes of E4M3 hold weights this small: a norm would say little
+        ref, tol = E.expected(X, ids, weights)
+        assert ((D.double() - ref).abs() <= tol).all()
+    else:
+        check(D, *E.expected(X, ids, weights))
+
+
+def test_weights_beyond_4_gigabytes(sg):
+    """The first and the last expert of 9.4 GB of W1 and 4.7 GB of W2, by rows on and off their 128-byte lines."""
+    for experts, hidden, inner in ((80, 4096, 14336), (80, 4112, 14352)):
+        E = Experts.__new__(Experts)
+        E.experts, E.hidden, E.inner = experts, hidden, inner
+        E.W1 = torch.randint(0, 0x70, (experts, 2 * inner, hidden), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        E.W2 = torch.randint(0, 0x70, (experts, hidden, inner), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        assert E.W2.numel() > 2 ** 32
+        E.S1 = (torch.rand((experts, 2 * inner), device="cuda") + 0.5) / (50 * hidden ** 0.5)
+        E.S2 = (torch.rand((experts, hidden), device="cuda") + 0.5) / (50 * inner ** 0.5)
+        ids = torch.tensor([[0, experts - 1], [experts - 1, 1]], dtype=torch.int32, device="cuda")
+        weights = torch.tensor([[0.5, 0.25], [0.75, 1.0]], device="cuda")
+        X = tokens(2, hidden, seed=50)
+        check(experts_of(sg, X, ids, weights, E), *E.expected(X, ids, weights))
+        del E

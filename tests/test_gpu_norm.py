@@ -1,4 +1,6 @@
 """sg_rmsnorm_fp8_rows against its formula in 64 bits."""
+import random
+
 import pytest
 import torch
 
@@ -157,3 +159,34 @@ def test_registered_operator(sg):
     Q, s, total, _ = torch.ops.sgemm.rmsnorm_fp8_rows(X)
     assert torch.equal(total, X) and torch.equal(Q, run(sg, X, eps=1e-6)[0])
     torch.library.opcheck(torch.ops.sgemm.rmsnorm_fp8_rows.default, (X, w, res), test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_drawn_sizes(sg, seed):
+    rng = random.Random(seed)
+    rows, cols = rng.randint(1, rng.choice((8, 700))), 16 * rng.randint(1, rng.choice((64, 1100)))
+    X, weight, residual = operands(rows, cols, seed, residual=rng.random() < 0.6)
+    weight = weight if rng.random() < 0.8 else None
+    Q, s, S, Y = run(sg, X, weight, residual)
+    v, y = expected(X, weight, residual, 1e-5)
+    assert torch.equal(S, v)
+    check(Q, s, Y, y)
+
+
+@pytest.mark.parametrize("cols", [512, 8192, 98304])
+def test_matrices_beyond_4_gigabytes(sg, cols):
+    rows = 2 ** 32 // cols + 5
+    X = torch.empty((rows, cols), dtype=torch.bfloat16, device="cuda")
+    part, weight, _ = operands(64, cols, seed=5)
+    X[:64] = part
+    X[64:] = 1
+    X[-64:] = part
+    Q, s = torch.empty((rows, cols), dtype=torch.uint8, device="cuda"), torch.empty(rows, device="cuda")
+    total = torch.empty_like(X)
+    assert sg.rmsnorm_fp8_rows(X, Q, s, weight, None, total, None, 1e-5) == 0
+    # (64 rows by themselves may add their squares up in another order than as many of these)
+    _, y = expected(part, weight, None, 1e-5)
+    for rows_at in (slice(0, 64), slice(rows - 64, rows)):
+        check(Q[rows_at], s[rows_at], None, y)
+        assert torch.equal(Q[rows_at], Q[:64]) and torch.equal(s[rows_at], s[:64]) and torch.equal(total[rows_at], part)
+    assert torch.equal(Q[64:80], Q[-80:-64]) and (s[64:-64] == s[64]).all()

@@ -54,8 +54,12 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
 
 // The build, its waves and its K splits by the shape; us below are of one MI355X, medians of graph replays on cold weights.
 //
-// Up to 16 rows: one tile a wave where there are at most as many tiles as CUs (4096 x 4096 at one row 4.9, two tiles 5.6), two elsewhere
-// (28672 x 4096 14.2, 15.5), on as many waves as leave each a few steps.  K splits where idle CUs can take them and the steps that a
+// Up to 16 rows: one tile a wave where there are at most as many tiles as CUs (13 rows of 3712 x 10944, groups of 32, 11.4; two tiles 14.7), or up to
+// three times as many and at most eight rows (1 x 11008 x 4096 7.5, two 8.0; 13 rows 11.4, 9.9), two elsewhere (5 x 28672 x 4096 15.1,
+// one 15.6), on as many waves as leave each a few steps: 1 x 3712 x 10944, groups of 64, sixteen 8.1, eight 9.8; 1 x 6144 x 4096 eight
+// 5.8, four 6.6, two 9.5; 1 x 28672 x 4096 two 13.9, four 14.8, eight 15.7, in groups of 32 19.2, 17.9, 19.5.  With more than eight rows and
+// many tiles the activations are what goes to a CU most: four waves share them (13 x 28672 x 4096 14.6, each its own 16.3; in groups
+// of 32 19.3 and 19.8, 57344 x 8192 67.5 and 63.1).  K splits where idle CUs can take them and the steps that a
 // wave has left outweigh the second launch: 1 x 1024 x 32768 14.3 -> 9.8, 8 x 512 x 16384 10.9 -> 7.3.
 //
 // Beyond, the waves' vector units bound what a workgroup does, so that its time is its steps times that of one, and a product's that of
@@ -65,10 +69,12 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
 Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
     Int4Plan p{1, a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : a.m <= 32 ? 8 : 16, 1, 1, 1};
     if (p.xu <= 4) {
-        p.nf = a.tiles > cu_count ? 2 : 1;
+        p.nf = a.tiles <= cu_count || (p.xu < 4 && a.tiles > 2 * cu_count && a.tiles <= 3 * cu_count) ? 1 : 2;
         const int groups = (a.tiles - 1) / p.nf + 1;
-        if (p.nf == 1) p.kw = p.xu == 1 && (a.steps >= 96 || (a.steps >= 48 && a.tiles <= cu_count / 2)) ? 16 : 8;
-        else p.kw = groups <= cu_count ? 8 : groups <= 2 * cu_count || a.steps >= 48 ? 4 : 2;
+        if (groups <= cu_count) p.kw = p.nf == 1 && p.xu == 1 && a.steps >= 32 ? 16 : 8;
+        else if (p.nf == 1 || groups <= 2 * cu_count) p.kw = 4;
+        else if (p.xu == 4 && group >= 64) p.nw = 4, p.kw = 2;
+        else p.kw = a.steps >= 48 || (group == 32 && p.xu < 4) ? 4 : 2;
         while (p.kw > a.steps) p.kw /= 2;
         if (!workspace || 2 * groups > cu_count) return p;
         const int splits = cu_count / groups < kInt4Splits ? cu_count / groups : kInt4Splits;
@@ -85,7 +91,7 @@ Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
     float best = 0.0f;
     for (const Way& w : ways) {
         const long long groups = (long long)((a.tiles - 1) / (w.nf * w.nw) + 1) * m_groups;
-        const int at_once = group == 32 ? 1 : w.at_once;
+        const int at_once = group == 32 && p.xu == 16 ? 1 : w.at_once;
         int kw = w.kw;
         while (kw > a.steps) kw /= 2;
         for (int splits = 1; splits <= (workspace ? kInt4Splits : 1) && splits * kw <= a.steps; splits++) {

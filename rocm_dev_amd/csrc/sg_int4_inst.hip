@@ -14,7 +14,7 @@ static int launch_build(Int4Args& a, const Int4Plan& plan, hipStream_t stream) {
     const long long grid = (long long)a.n_groups * a.m_groups * a.splits;
     if (grid > INT_MAX) return SG_BAD_ARGUMENT;
     constexpr int MF = XU < 4 ? 1 : XU / 4, DX = XU / NW <= 2 && DW == 4 ? 4 : 2;      // activations: DX steps in flight
-    const size_t acts = (size_t)kw * 2 * int4_buffer(SG_GPS, XU, NW), sums = kw > 1 ? (size_t)kw * NW * NF * MF * 1024 : 0;
+    const size_t acts = (size_t)kw * (2 * int4_buffer(SG_GPS, XU, NW) + NW * NF * 256), sums = kw > 1 ? (size_t)kw * NW * NF * MF * 1024 : 0;
     const size_t lds = acts > sums ? acts : sums;
     auto* const kernel = int4_gemm_kernel<SG_GPS, FLAGS, NF, XU, NW, DW, DX, MAXW, MINB>;
     static LdsGranted granted;
@@ -23,8 +23,9 @@ static int launch_build(Int4Args& a, const Int4Plan& plan, hipStream_t stream) {
     return report_hip("int4_gemm launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
 }
 
-// Up to 16 rows a wave has the activations to itself: one tile on up to eight waves (sixteen with four rows), or two on up to eight.  Beyond, waves share
-// them: two or four waves of a tile each, eight of one (two such workgroups a CU, but for groups of 32, whose scales take the registers) or two.
+// Up to 16 rows a wave has the activations to itself: one tile on up to eight waves (sixteen with four rows), or two on up to eight; four waves of
+// two tiles share them where there are many tiles.  Beyond, waves share them: two or four waves of a tile each, eight of one (two such
+// workgroups a CU, but for 64 rows in groups of 32, which take too many registers) or two.
 template <int FLAGS>
 static int launch_flags(Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     switch (p.xu * 100 + p.nw * 10 + p.nf) {
@@ -33,11 +34,12 @@ static int launch_flags(Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     case XU * 100 + 12: return launch_build<FLAGS, 2, XU, 1, 2, 8, 1>(a, p, stream);
         SG_ROWS(1) SG_ROWS(2) SG_ROWS(4)
 #undef SG_ROWS
+        case 442: return launch_build<FLAGS, 2, 4, 4, 4, 8, 1>(a, p, stream);
 #define SG_ROWS(XU)                                                                    \
     case XU * 100 + 21: return launch_build<FLAGS, 1, XU, 2, 4, 8, 1>(a, p, stream);   \
     case XU * 100 + 41: return launch_build<FLAGS, 1, XU, 4, 4, 8, 1>(a, p, stream);   \
-    case XU * 100 + 81: return launch_build<FLAGS, 1, XU, 8, 2, 8, SG_GPS < 4 ? 4 : 1>(a, p, stream); \
-    case XU * 100 + 82: return launch_build<FLAGS, 2, XU, 8, SG_GPS < 4 ? 4 : 2, 8, 1>(a, p, stream);
+    case XU * 100 + 81: return launch_build<FLAGS, 1, XU, 8, 2, 8, SG_GPS == 4 && XU == 16 ? 1 : 4>(a, p, stream); \
+    case XU * 100 + 82: return launch_build<FLAGS, 2, XU, 8, 4, 8, 1>(a, p, stream);
         SG_ROWS(8) SG_ROWS(16)
 #undef SG_ROWS
         default: return SG_INVALID_CONFIG;

@@ -4,13 +4,15 @@
 // codes are widened on the way: 1 + q / 16 by a rotation and a mask a pair (sg_int4.h), and the product of a group is set right behind it,
 //     sum A * (q - z) = 16 * ( sum A * (1 + q / 16)  -  (1 + z / 16) * sum A ),
 // the activations' own sum by the same instruction on a matrix of ones, once for all tiles of a wave - or, where waves share the activations,
-// by those that bring them.  Seven vector operations a dword of eight codes: a third of the clocks at the rate at which the memory
-// delivers, up to 16 rows.  Beyond, the two fp32 multiply-adds an output and group are what the vector units are busy with.
+// by those that bring them.  Up to 16 rows what is left beside that stream is the way of everything into a CU, 64 bytes a clock: the
+// activations, read again for every tile or two, are four times a tile's codes.  Beyond, vector units and matrix units are busy in turn:
+// the two fp32 multiply-adds an output and group, the widening, then the products, none beside the others (64 rows of 57344 x 8192 in
+// groups of 64, of 131 us: without the products 94, without the scales' multiply-adds 112, without the activations' reads from LDS 119).
 // The correction cancels: both of its terms are up to 16 * sum|A| / |sum A (q - z)| times the result, about 50 at
 // groups of 128 of noise, so that 2^-24 of fp32 becomes 2^-18 of a group's sum, against 2^-9 of the output's rounding.
 //
 // A wave takes NF 16-row weight tiles and all rows of an activation tile, and walks a part of K in steps of 128 columns.  Weights go from
-// memory to registers as they lie, four steps in flight.  Activations come by 4 rows x 256 bytes a load, whole lines, and go through
+// memory to registers as they lie, DW steps in flight, two where a wave has few.  Activations come by 4 rows x 256 bytes a load, whole lines, and go through
 // LDS: NW waves with weight tiles of their own share them (and a barrier a step), KW such groups share K by steps and meet in LDS,
 // partial sums added in their order: the result does not depend on which wave is first.
 #pragma once
@@ -46,7 +48,7 @@ __device__ __forceinline__ float int4_sum8(u32x4 v, uint32_t ones) {
     }
     return sum;
 }
-// four scales of two dwords, four zeros of one
+// four scales of two dwords
 template <bool F16>
 __device__ __forceinline__ f32x4 int4_scales(uint32_t lo, uint32_t hi) {
     if (F16) {
@@ -55,11 +57,10 @@ __device__ __forceinline__ f32x4 int4_scales(uint32_t lo, uint32_t hi) {
     }
     return f32x4{bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi)};
 }
-__device__ __forceinline__ f32x4 int4_zeros(uint32_t z) {      // 1 + z / 16
-    f32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = fmaf((float)((z >> (8 * i)) & 0xffu), 0.0625f, 1.0f);
-    return v;
+// 1 + z / 16 in fp16, exactly, two a register as the multiply-add takes them: bytes under 1024's exponent, 1024 + z, times 1 / 16, less 63
+__device__ __forceinline__ f16x2_t int4_zeros(uint32_t z, uint32_t bytes) {
+    const f16x2_t v = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, z, bytes));
+    return __builtin_elementwise_fma(v, f16x2_t{(_Float16)0.0625f, (_Float16)0.0625f}, f16x2_t{(_Float16)-63.0f, (_Float16)-63.0f});
 }
 
 // N dwords by as few loads as their alignment (N dwords, at most four) allows
@@ -111,7 +112,7 @@ __device__ __forceinline__ float int4_over_lanes(float v) {
 }
 
 // FLAGS: SG_INT4_ZEROS, SG_INT4_F16_SCALES.  The tile has 4 * XU activation rows.
-// LDS: [KW][2][XU KB activations, NW > 1: [4 * XU][GPS] sums of groups], then in its place [KW][NW][NF * MF][64 lanes] f32x4.
+// LDS: [KW][2][XU KB activations, NW > 1: [4 * XU][GPS] sums of groups], [KW][NW][NF][256 bytes of scales and zeros], then in its place [KW][NW][NF * MF][64 lanes] f32x4.
 template <int GPS, int FLAGS, int NF, int XU, int NW, int DW, int DX, int MAXW, int MINB>
 __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Args a) {
     constexpr bool ZEROS = FLAGS & SG_INT4_ZEROS, F16 = FLAGS & SG_INT4_F16_SCALES;
@@ -130,13 +131,16 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
     const int first_tile = (tn * NW + nw) * NF;
 
     // ---- operands: tiles beyond the last and rows beyond m take the last one again, and are not stored ----
-    const uint8_t *wb[NF], *sb[NF], *zb_[NF];
+    // Scales and zeros: a dword a lane, 8 * GPS of scales and behind them 4 * GPS of zeros, by way of LDS to the lanes that use them.  (Each lane
+    // loading what it uses itself loads everything 16 times: 4 KB a tile and step in groups of 32, by a path of 64 bytes a clock.)
+    const bool of_zeros = ZEROS && lane >= 8 * GPS && lane < 12 * GPS;
+    const uint32_t s_step = of_zeros ? GPS * 16 : GPS * 32, s_lane = (of_zeros ? lane - 8 * GPS : lane < 8 * GPS ? lane : 0) * 4;
+    const uint8_t *wb[NF], *sb[NF];
 #pragma unroll
     for (int i = 0; i < NF; i++) {
         const size_t tile = (size_t)(first_tile + i < a.tiles ? first_tile + i : a.tiles - 1) * a.steps;
         wb[i] = a.P + tile * 1024;
-        sb[i] = a.PS + tile * (GPS * 32);
-        zb_[i] = ZEROS ? a.PZ + tile * (GPS * 16) : nullptr;
+        sb[i] = (of_zeros ? a.PZ : a.PS) + (tile * s_step + s_lane);
     }
     // Activations: load u of the tile has rows 4 u .. 4 u + 3, lane l piece l % 16 (8 columns) of row l / 16; in LDS the pieces of row i stand
     // permuted by i, so that the 16 lanes (r, g) of a fragment's read hit 16 bank groups.
@@ -152,37 +156,36 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
     const int xrow = r % ROWS;
 #pragma unroll
     for (int t = 0; t < 4; t++) xr[t] = (uint32_t)(xrow * 256 + ((4 * t + g) ^ xrow) * 16);
-    uint8_t* const xbuf = lds + kg * 2 * BUFFER;
+    uint8_t *const xbuf = lds + kg * 2 * BUFFER, *const sbuf = lds + KW * 2 * BUFFER + wave * (NF * 256);
 
     uint32_t ones = 0x3f803f80u;
     asm volatile("" : "+v"(ones));
     u32x4 w[DW][NF], x[DX][LOADS];
-    uint32_t s[DW][NF][2 * GPS], z[DW][NF][GPS];
+    uint32_t s[DW][NF];
     f32x4 acc[NF][MF];
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
         for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // A step beyond this part of K loads its first one again, which is not multiplied: a load that may not be issued would make every wait one
+    // A step beyond this part of K loads one piece for all lanes, which is not multiplied: a load that may not be issued would make every wait one
     // for all loads.  A piece of a row beyond its end is the last piece again: its weights' scales are zero.  (32-bit offsets: k is below 2^24.)
-    auto inside = [&](int step) { return (uint32_t)(step < steps ? step : begin); };
     auto load_x = [&](auto dc, int step) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value % DX;
-        const int p = (int)(16 * inside(step)) + piece;
+        const uint32_t live = step < steps ? ~0u : 0u;
+        const int p = 16 * step + piece;
         const uint32_t po = (uint32_t)(p < pieces ? p : pieces - 1) * 16;
 #pragma unroll
-        for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xb + (xo[u] + po));
+        for (int u = 0; u < LOADS; u++) x[d][u] = *reinterpret_cast<const u32x4*>(xb + ((xo[u] + po) & live));
     };
     auto load_w = [&](auto dc, int step) __attribute__((always_inline)) {
         constexpr int d = decltype(dc)::value % DW;
-        const uint32_t from = inside(step);
-        const uint32_t wo = from * 1024 + lane * 16, so = from * (GPS * 32) + g * (GPS * 8), zo = from * (GPS * 16) + g * (GPS * 4);
+        const uint32_t live = step < steps ? ~0u : 0u, from = (uint32_t)step;
+        const uint32_t wo = (from * 1024 + lane * 16) & live, so = (from * s_step) & live;
 #pragma unroll
         for (int i = 0; i < NF; i++) {
             w[d][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wb[i] + wo));
-            int4_take(s[d][i], sb[i] + so);
-            if (ZEROS) int4_take(z[d][i], zb_[i] + zo);
+            s[d][i] = *reinterpret_cast<const uint32_t*>(sb[i] + so);
         }
     };
     // A step's activations are brought to LDS a step before they are read, in two places in turn.
@@ -214,8 +217,15 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
         u32x4 y[Y][PER][MF];
         float sum[2][MF];
         f32x4 part[2][MF];
+        uint32_t scales[NF][2 * GPS], zeros[NF][GPS];
+#pragma unroll
+        for (int i = 0; i < NF; i++) *reinterpret_cast<uint32_t*>(sbuf + i * 256 + lane * 4) = s[d][i];
         auto products = [&](int unit) __attribute__((always_inline)) {
             const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2, hy = q % Y;
+            if (q == 0) {
+                int4_take(scales[i], sbuf + i * 256 + g * (GPS * 8));
+                if (ZEROS) int4_take(zeros[i], sbuf + i * 256 + GPS * 32 + g * (GPS * 4));
+            }
             if (i == 0) {
 #pragma unroll
                 for (int j = 0; j < MF; j++) {
@@ -240,12 +250,16 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
         };
         auto apply = [&](int unit) __attribute__((always_inline)) {
             const int q = unit / NF, i = unit % NF, h = q % 2, u = unit % 2;
-            const f32x4 scale = int4_scales<F16>(s[d][i][2 * q], s[d][i][2 * q + 1]);
-            const f32x4 zb = ZEROS ? int4_zeros(z[d][i][q]) : f32x4{1.5f, 1.5f, 1.5f, 1.5f};
+            const f32x4 scale = int4_scales<F16>(scales[i][2 * q], scales[i][2 * q + 1]);
+            f16x2_t zb[2];
+            if (ZEROS) zb[0] = int4_zeros(zeros[i][q], 0x04010400u), zb[1] = int4_zeros(zeros[i][q], 0x04030402u);
 #pragma unroll
             for (int j = 0; j < MF; j++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[i][j][c] = fmaf(scale[c], fmaf(-zb[c], sum[h][j], part[u][j][c]), acc[i][j][c]);
+                for (int c = 0; c < 4; c++) {
+                    const float by = ZEROS ? (float)(c % 2 ? zb[c / 2].y : zb[c / 2].x) : 1.5f;
+                    acc[i][j][c] = fmaf(scale[c], fmaf(-by, sum[h][j], part[u][j][c]), acc[i][j][c]);
+                }
         };
 #pragma unroll
         for (int unit = 0; unit <= GPS * NF; unit++) {
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
     };
     // Steps kg, kg + KW, ...  A group with one fewer than another goes through the other's barriers.
     const int end = SHARED ? begin + (steps - begin - 1) / KW * KW + KW : steps;
-    int step = begin + kg;
+    int step = begin + kg, left = step < end ? (end - 1 - step) / KW + 1 : 0;
     auto turn = [&](auto dc) __attribute__((always_inline)) {
         using Next = std::integral_constant<int, (decltype(dc)::value + 1) % 4>;
         share_x(Next{});                                     // (behind the last step what a step beyond the matrix loads)
@@ -264,14 +278,14 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
         if (!SHARED || step < steps) multiply(dc);
         load_w(dc, step + DW * KW);
         step += KW;
+        left--;
         meet();
-        return step < end;
     };
     using D0 = std::integral_constant<int, 0>;
     using D1 = std::integral_constant<int, 1>;
     using D2 = std::integral_constant<int, 2>;
     using D3 = std::integral_constant<int, 3>;
-    if (step < end) {
+    if (left > 0) {
         load_x(D0{}, step);
         load_w(D0{}, step);
         load_x(D1{}, step + KW);
@@ -283,7 +297,22 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
         share_x(D0{});
         load_x(D0{}, step + DX * KW);
         meet();
-        while (turn(D0{}) && turn(D1{}) && turn(D2{}) && turn(D3{})) {}
+        // As many turns as there are places by turn, and what is left behind them: a loop with an exit in its midst has its head waiting for all
+        // loads in flight.
+        constexpr int TURNS = DW > DX ? DW : DX;
+        while (left >= TURNS) {
+            turn(D0{});
+            turn(D1{});
+            if constexpr (TURNS > 2) {
+                turn(D2{});
+                turn(D3{});
+            }
+        }
+        if (left > 0) turn(D0{});
+        if constexpr (TURNS > 2) {
+            if (left > 0) turn(D1{});
+            if (left > 0) turn(D2{});
+        }
     }
 
     // ---- the groups' sums, in their order ----

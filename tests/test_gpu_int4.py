@@ -231,6 +231,11 @@ def test_threads_on_one_stream(sg):
     assert all(torch.equal(d, t) for out, t in zip(outs, want) for d in out)
 
 
+@pytest.mark.parametrize("m,n,k,group", [(13, 40000, 640, 128), (16, 20017, 2048, 64), (9, 17000, 416, 32), (4, 11008, 1024, 128), (8, 12003, 1344, 64)])
+def test_many_tiles(sg, m, n, k, group):
+    check(sg, activations(m, k, seed=15), Weights(sg, n, k, group, True, True, seed=15))
+
+
 @pytest.mark.parametrize("seed", range(24))
 def test_drawn_sizes(sg, seed):
     rng = random.Random(seed)

@@ -392,7 +392,7 @@ int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const
  *     scales[r] = absmax(y[r,:]) / 448 (1 if that is zero; NaNs do not count);   Q = e4m3_rne_sat(y / scales[r]), a NaN 0x7f
  * and, each if its pointer is not NULL, sum = v (the next residual) and Y = bf16(y) (a router's input).  residual and weight
  * ([cols]) may be NULL: nothing added, factors of 1.  sum may be X's or the residual's own memory; Q and Y overlap no input.
- * A row whose squares' sum is no finite fp32 has y = 0, or NaN where v * weight is not finite.  cols must be a multiple of 16, all
+ * The squares' sum is fp32, in an order fixed by rows and cols.  A row where it is not finite has y = 0, or NaN where v * weight is not finite.  cols must be a multiple of 16, all
  * matrices and weight 16-byte aligned, scales 4-byte, eps finite and not negative. */
 int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const void* weight_bf16, void* sum_bf16, void* Y_bf16,
                         uint8_t* Q, float* scales, float eps, int rows, int cols, void* stream);

@@ -755,7 +755,7 @@ def moe_workspace_bytes(m, hidden, inner, experts, top_k):
     """Bytes of workspace that moe_layer and moe_experts take for these sizes."""
     need = lib.sg_moe_workspace_bytes(m, hidden, inner, experts, top_k)
     if need == 0:
-        raise ValueError("1 <= m <= 64 tokens, hidden and inner multiples of 16, up to 512 experts and top_k <= 16 of them are taken, got m = %d, "
+        raise ValueError("1 <= m <= 64 tokens, hidden and inner multiples of 16 up to 2^20, up to 512 experts and top_k <= 16 of them are taken, got m = %d, "
                          "hidden = %d, inner = %d, experts = %d, top_k = %d" % (m, hidden, inner, experts, top_k))
     return need
 

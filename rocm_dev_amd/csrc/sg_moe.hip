@@ -125,7 +125,7 @@ static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t strea
     if (!rc) rc = launch_down_parts<XU, N>(a, waves, stream);
     if (rc || a.splits == 1) return rc;
     moe_sum_kernel<<<(unsigned)((a.m * (long long)a.hidden + 1023) / 1024), 256, 0, stream>>>(a);
-    return (int)hipGetLastError();
+    return launched("moe_sum launch");
 }
 
 // How many columns a part has.  An expert's tokens are as many as independent choices of top_k / experts give; each part reads the expert's

@@ -62,10 +62,11 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
 // of 32 19.3 and 19.8, 57344 x 8192 67.5 and 63.1).  K splits where idle CUs can take them and the steps that a
 // wave has left outweigh the second launch: 1 x 1024 x 32768 14.3 -> 9.8, 8 x 512 x 16384 10.9 -> 7.3.
 //
-// Beyond, the waves' vector units bound what a workgroup does, so that its time is its steps times that of one, and a product's that of
-// its rounds of workgroups.  The four ways - two or four waves of one tile and groups of them that share K, eight of one tile, eight of two -
-// and their K splits are compared by that: 64 rows of 57344 x 8192 98 (two tiles on eight waves; 203 on two waves of one), 10240 x 8192
-// 32.5 (the same, six splits; unsplit 91, 39 on four waves), 8192 x 28672 60 (eight splits; 97 on two waves).
+// Beyond, the waves' vector and matrix units bound what a workgroup does, so that its time is its steps times that of one, and a product's
+// that of its rounds of workgroups.  The four ways - two or four waves of one tile and groups of them that share K, eight of one tile, eight
+// of two - and their K splits are compared by that.  64 rows, groups of 64, without the splits' second launch (5): 57344 x 8192 110 (two tiles on
+// eight waves; 211 on two waves of one), 10240 x 8192 24.4 (the same, six splits; unsplit 91, 39 on four waves), 8192 x 28672 54.6 (eight
+// splits; 98 on two waves).
 Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
     Int4Plan p{1, a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : a.m <= 32 ? 8 : 16, 1, 1, 1};
     if (p.xu <= 4) {

@@ -63,18 +63,21 @@ static int launch_down(MoeArgs& a, hipStream_t stream) {
 
 static bool off_lines(const uint8_t* weights, int columns) { return columns % 128 != 0 || (reinterpret_cast<uintptr_t>(weights) & 127u) != 0; }
 
-// waves: four, or eight where the rings fit.
+// waves: four, or eight where the rings fit (not with 32 rows of activations a stage).
 template <int XU, int N>
 static int launch_down_parts(MoeArgs& a, int waves, hipStream_t stream) {
-    if (off_lines(a.W2, a.inner)) {
-        constexpr int L = N < 3 ? 3 : N;
-        if (waves == 8 && down_lds<XU, L, 8>(a) <= kLdsBytes) return launch_down<XU, L, true, 8>(a, stream);
-        if (waves == 8 && down_lds<XU, 3, 8>(a) <= kLdsBytes) return launch_down<XU, 3, true, 8>(a, stream);
-        if (down_lds<XU, 3, 4>(a) <= kLdsBytes) return launch_down<XU, 3, true, 4>(a, stream);
+    const bool lines = off_lines(a.W2, a.inner);
+    if constexpr (8 * 2 * MoeStages<1, XU, false>::kBytes < kLdsBytes) {
+        if (waves == 8 && lines) {
+            if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, true, 8>(a, stream);
+            if (down_lds<XU, 3, 8>(a) <= kLdsBytes) return launch_down<XU, 3, true, 8>(a, stream);
+        }
+        if (waves == 8 && !lines) {
+            if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, false, 8>(a, stream);
+            if (down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, false, 8>(a, stream);
+        }
     }
-    if (waves == 8 && down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, false, 8>(a, stream);
-    if (waves == 8 && down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, false, 8>(a, stream);
-    return launch_down<XU, 2, false, 4>(a, stream);
+    return lines ? launch_down<XU, 3, true, 4>(a, stream) : launch_down<XU, 2, false, 4>(a, stream);
 }
 
 // How many workgroups share a tile of the down projections, and how many waves they have: eight, one workgroup a CU, or four, two.
@@ -106,7 +109,9 @@ static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t strea
     int waves;
     a.splits = down_splits(a, cu_count, &waves);
     // Waves that share an item, and stages in flight: what leaves the least to the last round.
-    const bool lines = off_lines(a.W1, a.hidden) && (a.share_log = 2, gate_up_lds<XU, 3>(a) <= kLdsBytes);
+    // (32 rows of activations a stage leave no room for a third one)
+    constexpr bool kLines = 4 * 3 * MoeStages<2, XU, true>::kBytes + 4 * 2 * MoeStages<2, XU, true>::kBlocks * 1024 < kLdsBytes;
+    const bool lines = kLines && off_lines(a.W1, a.hidden) && (a.share_log = 2, gate_up_lds<XU, 3>(a) <= kLdsBytes);
     float best = 0.0f;
     int share_log = 0;
     bool shorter = false;
@@ -120,7 +125,7 @@ static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t strea
     a.share_log = share_log;
     const long long groups = ((items << share_log) + 3) / 4;
     int rc;
-    if (lines) rc = launch_gate_up<XU, 3, true>(a, choose, groups, cu_count, stream);
+    if (lines) rc = launch_gate_up<XU, kLines ? 3 : 2, kLines>(a, choose, groups, cu_count, stream);
     else rc = shorter ? launch_gate_up<XU, 2, false>(a, choose, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, choose, groups, cu_count, stream);
     if (!rc) rc = launch_down_parts<XU, N>(a, waves, stream);
     if (rc || a.splits == 1) return rc;

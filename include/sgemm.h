@@ -55,7 +55,7 @@ const char* sg_strerror(int code);
  * device and stream: calls on one stream run in order and share a workspace, calls on different
  * streams may overlap and never share one.  Host threads may call on one stream at the same time: a call whose
  * launches hand each other memory (a GEMM and the sum of its K split's partials, the row encoder and the GEMM on
- * its codes) enqueues them with no other such call of the library's in between.  (hipStreamPerThread is one handle
+ * its codes, a router's or a mixture-of-experts layer's, in the caller's workspace) enqueues them with no other such call of the library's in between.  (hipStreamPerThread is one handle
  * for a stream of every thread's own: pass it from one thread only.)  A workspace is created, or grown, by the first launch on its
  * stream that needs it (split_k > 1, also when the library chooses the split itself); at most 512 MB of
  * partials per launch, beyond that SG_WORKSPACE_TOO_SMALL.  An outgrown buffer is kept until it is released

@@ -211,6 +211,8 @@ int take_router(MoeArgs& a, const void* R, int renormalize) {
 }
 }  // namespace
 
+// Every entry point below holds its stream's turn from its first launch to its last: they hand each other logits, the plan, h and sums
+// through the caller's workspace, and another thread's call on the stream, whose plan may be of other sizes, must not come in between.
 extern "C" {
 
 size_t sg_moe_workspace_bytes(int m, int hidden, int inner, int experts, int top_k) {
@@ -225,6 +227,7 @@ int sg_moe_route(const void* X, const void* R, int32_t* ids, float* weights, int
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::recursive_mutex> turn(stream_turn(st));
     if (int rc = launch_logits(a, st)) return rc;
     return launch_choose(a, st);
 }
@@ -239,7 +242,9 @@ int sg_moe_experts(const void* X, const int32_t* ids, const float* weights, cons
     if (int rc = take_experts(a, W1, S1, W2, S2, D)) return rc;
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
-    return launch_experts(a, false, dev->cu_count, static_cast<hipStream_t>(stream));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::recursive_mutex> turn(stream_turn(st));
+    return launch_experts(a, false, dev->cu_count, st);
 }
 
 int sg_moe_layer(const void* X, const void* R, const uint8_t* W1, const float* S1, const uint8_t* W2, const float* S2, void* D, int32_t* ids,
@@ -254,6 +259,7 @@ int sg_moe_layer(const void* X, const void* R, const uint8_t* W1, const float* S
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    std::lock_guard<std::recursive_mutex> turn(stream_turn(st));
     if (int rc = launch_logits(a, st)) return rc;
     const bool fused = m <= kMoeFused;
     if (!fused)

@@ -39,7 +39,9 @@ struct RowFactors {
 };
 __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps) {
     RowFactors f;
-    f.rstd = 1.0f / sqrtf(r.squares / (float)cols + eps);
+    const float mean = r.squares / (float)cols + eps;
+    // (with an eps as small, few values in a long row have a mean below fp32's normal range, though their squares are not: 2^64 times it)
+    f.rstd = mean < 0x1p-100f ? 0x1p32f / sqrtf(r.squares * 0x1p64f / (float)cols + eps * 0x1p64f) : 1.0f / sqrtf(mean);
     float top = r.top * f.rstd;
     if (!(top > 0.0f)) top = 0.0f;                       // also NaN: an infinity times zero, or a row that holds a NaN
     f.s = top == 0.0f ? 1.0f : __fdiv_rn(top, 448.0f);

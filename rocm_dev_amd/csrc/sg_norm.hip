@@ -35,7 +35,7 @@ struct RowSums {
 
 struct RowFactors {
     float rstd, s, code;         // code: rstd / s
-    bool divide;                 // 1 / s does not stand for s
+    bool divide;                 // `code` does not stand for a quotient by s
 };
 __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps) {
     RowFactors f;
@@ -46,7 +46,8 @@ __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps
     if (!(top > 0.0f)) top = 0.0f;                       // also NaN: an infinity times zero, or a row that holds a NaN
     f.s = top == 0.0f ? 1.0f : __fdiv_rn(top, 448.0f);
     f.code = f.rstd * __fdiv_rn(1.0f, f.s);
-    f.divide = !(f.s >= 0x1p-120f && f.s <= 0x1p120f);
+    // code is about 448 / max|v * w|: a large rstd can lift s into the range whose reciprocals are normal while code itself overflows
+    f.divide = !(f.s >= 0x1p-120f && f.s <= 0x1p120f && f.code <= 0x1p120f);
     return f;
 }
 

@@ -25,3 +25,21 @@ def test_means_below_the_normal_range(sg, cols, v):
     rows = [0, 1, 3]                                # (a row of zeros is 0 / 0)
     Q, s, _, Y = run(sg, X, eps=0.0)
     check(Q[rows], s[rows], Y[rows], y[rows])
+
+
+# 448 / max|v * w| is beyond fp32's largest value below 2^-119.2, wherever rstd leaves the scale itself
+@pytest.mark.parametrize("cols", [64, 1040, 8192, 65552])
+@pytest.mark.parametrize("v,w,eps", [(-120, 0, 1e-6), (-120, None, 1e-8), (-119, 0, 1e-5), (-126, 0, 1e-12), (-60, -60, 0.0), (-50, -73, 0.0), (-62, -48, 0.0)])
+def test_small_products_with_a_scale_in_range(sg, cols, v, w, eps):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(cols)
+    X = ((torch.rand((5, cols), generator=gen, device="cuda") * 2 - 1) * 2.0 ** v).bfloat16()
+    X[:, ::5] = 0
+    X[2] = 0
+    X[2, 7], X[2, 8] = 2.0 ** v, -2.0 ** v
+    weight = None if w is None else torch.full((cols,), 2.0 ** w, device="cuda").bfloat16()
+    _, y = expected(X, weight, None, eps)
+    Q, s, _, Y = run(sg, X, weight, eps=eps)
+    check(Q, s, Y, y)
+    assert not Q[:, ::5].view(torch.float8_e4m3fn).float().any()
+    assert Q[2, 7] == 0x7e and Q[2, 8] == 0xfe

@@ -44,7 +44,8 @@ __device__ __forceinline__ RowFactors row_factors(RowSums r, int cols, float eps
     f.rstd = mean < 0x1p-100f ? 0x1p32f / sqrtf(r.squares * 0x1p64f / (float)cols + eps * 0x1p64f) : 1.0f / sqrtf(mean);
     float top = r.top * f.rstd;
     if (!(top > 0.0f)) top = 0.0f;                       // also NaN: an infinity times zero, or a row that holds a NaN
-    f.s = top == 0.0f ? 1.0f : __fdiv_rn(top, 448.0f);
+    f.s = __fdiv_rn(top, 448.0f);
+    if (f.s == 0.0f) f.s = 1.0f;                         // also a top whose 448th part is nearer to zero than to 2^-149
     f.code = f.rstd * __fdiv_rn(1.0f, f.s);
     // code is about 448 / max|v * w|: a large rstd can lift s into the range whose reciprocals are normal while code itself overflows
     f.divide = !(f.s >= 0x1p-120f && f.s <= 0x1p120f && f.code <= 0x1p120f);
@@ -77,7 +78,11 @@ __device__ __forceinline__ void put_chunk(const NormArgs& a, size_t at, u32x4 v,
         p[2 * j + 1] = bf16_hi(v[j]) * bf16_hi(w[j]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = DIVIDE ? __fdiv_rn(p[j] * f.rstd, f.s) : p[j] * f.code;
+    for (int j = 0; j < 8; j++) {
+        q[j] = DIVIDE ? __fdiv_rn(p[j] * f.rstd, f.s) : p[j] * f.code;
+        // a scale of few steps of 2^-149 may be a third below the 448th part that it stands for
+        if (DIVIDE) q[j] = q[j] > 448.0f ? 448.0f : q[j] < -448.0f ? -448.0f : q[j];
+    }
     int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     w0 = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w0, true);
     int w1 = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);

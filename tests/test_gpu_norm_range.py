@@ -43,3 +43,19 @@ def test_small_products_with_a_scale_in_range(sg, cols, v, w, eps):
     check(Q, s, Y, y)
     assert not Q[:, ::5].view(torch.float8_e4m3fn).float().any()
     assert Q[2, 7] == 0x7e and Q[2, 8] == 0xfe
+
+
+@pytest.mark.parametrize("cols", [64, 1040, 65552])
+@pytest.mark.parametrize("w", range(-80, -64))
+def test_scales_at_the_end_of_the_range(sg, cols, w):
+    """eps = 1 makes the root 1 to fp32's last bit: y is v * w, at most 2^(w - 70).  The scale is a multiple of 2^-149, or, where
+    448ths of the largest are nearer to zero, 1; codes are of y over that scale, cut off at 448."""
+    X = torch.tensor([0, 1, -1, 0.5, -0.75, 0.125, 2.0 ** -6, 0], device="cuda").mul(2.0 ** -70).bfloat16().repeat(3, cols // 8)
+    weight = torch.full((cols,), 2.0 ** w, device="cuda").bfloat16()
+    Q, s, _, _ = run(sg, X, weight, eps=1.0)
+    y = X.double() * 2.0 ** w
+    want = 2.0 ** (w - 70) / 448
+    steps = round(want * 2.0 ** 149)                # (no 448th of a power of two lies between two multiples)
+    assert (s.double() == (steps * 2.0 ** -149 if steps else 1.0)).all()
+    codes = (y / s.double()[:, None]).clamp(-448, 448).float().to(torch.float8_e4m3fn)
+    assert torch.equal(Q.view(torch.float8_e4m3fn).float(), codes.float())

@@ -8,7 +8,7 @@
 //     zeros   [n / 16][k / 128][4][groups][4 rows]   8 bits  (with SG_INT4_ZEROS)
 // with n, k rounded up; what is beyond the matrix holds code 0 and scale 0.  Within a dword, code 2 p (the pair's low half) lies at
 // bit 3 + 4 p and code 2 p + 1 at bit 19 + 4 p (mod 32): rotated right by 4 p and masked with 0x00780078 the pair lies in the
-// mantissas of two bf16, and with 0x3f80 in each half it is 1 + q / 16, exactly.
+// mantissas of two bf16, and with a power of two in each half it is that times 1 + q / 16, exactly.
 #pragma once
 
 #include "sg_device.h"

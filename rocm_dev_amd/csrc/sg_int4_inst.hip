@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) int4_sum_kernel(const Int4Args a) {
         if (s < a.splits) v += t[s];
     const int m_frag = (int)(f / a.tiles), tile = (int)(f - (size_t)m_frag * a.tiles);
     const int m_idx = m_frag * 16 + (lane & 15), n_idx = tile * 16 + 4 * (lane >> 4);
-    if (m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * 16.0f);
+    if (m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * kInt4OutOfUnits);
 }
 
 int launch_int4_sum(const Int4Args& a, hipStream_t stream) {

@@ -1,13 +1,16 @@
 // Products of bf16 activations with 4-bit integer weights:  D[m,n] = bf16( sum_g s[n,g] * sum_{k in g} A[m,k] * (q[n,k] - z[n,g]) ).
 //
 // What bounds it is the stream of weights, half a byte a value and the groups' scales.  The matrix instruction takes bf16, so the
-// codes are widened on the way: 1 + q / 16 by a rotation and a mask a pair (sg_int4.h), and the product of a group is set right behind it,
-//     sum A * (q - z) = 16 * ( sum A * (1 + q / 16)  -  (1 + z / 16) * sum A ),
-// the activations' own sum by the same instruction on a matrix of ones, once for all tiles of a wave - or, where waves share the activations,
+// codes are widened on the way: u (1 + q / 16) by a rotation and a mask a pair (sg_int4.h), u = 2^-13, and the product of a group is set
+// right behind it,
+//     sum A * (q - z) = 16 / u * ( sum A * u (1 + q / 16)  -  (1 + z / 16) * sum A * u ),
+// the activations' own sum by the same instruction on a matrix of u, once for all tiles of a wave - or, where waves share the activations,
 // by those that bring them.  Up to 16 rows what is left beside that stream is the way of everything into a CU, 64 bytes a clock: the
 // activations, read again for every tile or two, are four times a tile's codes.  Beyond, vector units and matrix units are busy in turn:
 // the two fp32 multiply-adds an output and group, the widening, then the products, none beside the others (64 rows of 57344 x 8192 in
 // groups of 64, of 131 us: without the products 94, without the scales' multiply-adds 112, without the activations' reads from LDS 119).
+// u keeps the sums of finite activations finite: 128 columns below 2^128 times 1 + 255 / 16 are below 2^140, and fp32 ends at 2^128.  What it costs
+// lies at the other end: products of activations below 2^-113 reach into fp32's subnormals, steps of 2^-149, 2^-132 * |s| of a result.
 // The correction cancels: both of its terms are up to 16 * sum|A| / |sum A (q - z)| times the result, about 50 at
 // groups of 128 of noise, so that 2^-24 of fp32 becomes 2^-18 of a group's sum, against 2^-9 of the output's rounding.
 //
@@ -31,20 +34,22 @@ __device__ __forceinline__ f32x4 mfma_bf16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// eight codes of a dword as 1 + q / 16; `ones` are two bf16 ones in a vector register, so that mask and ones are one instruction
+constexpr uint32_t kInt4Units = 0x39003900u;      // u = 2^-13 in two bf16
+constexpr float kInt4OutOfUnits = 131072.0f;      // 16 / u
+// eight codes of a dword as u (1 + q / 16); `units` in a vector register, so that mask and units are one instruction
 // (it takes one constant from elsewhere)
-__device__ __forceinline__ u32x4 int4_widen(uint32_t d, uint32_t ones) {
-    return u32x4{(d & 0x00780078u) | ones, (d >> 4 & 0x00780078u) | ones, (d >> 8 & 0x00780078u) | ones,
-                 (__builtin_amdgcn_alignbit(d, d, 12) & 0x00780078u) | ones};
+__device__ __forceinline__ u32x4 int4_widen(uint32_t d, uint32_t units) {
+    return u32x4{(d & 0x00780078u) | units, (d >> 4 & 0x00780078u) | units, (d >> 8 & 0x00780078u) | units,
+                 (__builtin_amdgcn_alignbit(d, d, 12) & 0x00780078u) | units};
 }
-// the sum of eight bf16
-__device__ __forceinline__ float int4_sum8(u32x4 v, uint32_t ones) {
-    const bf16x2_vec one = __builtin_bit_cast(bf16x2_vec, ones);
+// u times the sum of eight bf16
+__device__ __forceinline__ float int4_sum8(u32x4 v, uint32_t units) {
+    const bf16x2_vec unit = __builtin_bit_cast(bf16x2_vec, units);
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const uint32_t two = v[c];          // (a bit cast of v[c] itself takes element 0)
-        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_vec, two), one, sum, false);
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_vec, two), unit, sum, false);
     }
     return sum;
 }
@@ -158,8 +163,8 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
     for (int t = 0; t < 4; t++) xr[t] = (uint32_t)(xrow * 256 + ((4 * t + g) ^ xrow) * 16);
     uint8_t *const xbuf = lds + kg * 2 * BUFFER, *const sbuf = lds + KW * 2 * BUFFER + wave * (NF * 256);
 
-    uint32_t ones = 0x3f803f80u;
-    asm volatile("" : "+v"(ones));
+    uint32_t units = kInt4Units;
+    asm volatile("" : "+v"(units));
     u32x4 w[DW][NF], x[DX][LOADS];
     uint32_t s[DW][NF];
     f32x4 acc[NF][MF];
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
             // the sums of the groups: 4 * PER neighbouring lanes have a group's pieces
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
-                const float sum = int4_over_lanes<PER>(int4_sum8(x[d % DX][u], ones));
+                const float sum = int4_over_lanes<PER>(int4_sum8(x[d % DX][u], units));
                 if (piece % (4 * PER) == 0)
                     reinterpret_cast<float*>(to + XU * 1024)[piece / (4 * PER) * (4 * XU) + 4 * (nw * LOADS + u) + g] = sum;
             }
@@ -236,14 +241,14 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
                     } else {
                         f32x4 of_all = zero;
 #pragma unroll
-                        for (int t = 0; t < PER; t++) of_all = mfma_bf16_16x16x32(u32x4{ones, ones, ones, ones}, y[hy][t][j], of_all);
+                        for (int t = 0; t < PER; t++) of_all = mfma_bf16_16x16x32(u32x4{units, units, units, units}, y[hy][t][j], of_all);
                         sum[h][j] = of_all[0];
                     }
                 }
             }
 #pragma unroll
             for (int t = 0; t < PER; t++) {
-                const u32x4 v = int4_widen(w[d][i][q * PER + t], ones);
+                const u32x4 v = int4_widen(w[d][i][q * PER + t], units);
 #pragma unroll
                 for (int j = 0; j < MF; j++) part[u][j] = mfma_bf16_16x16x32(v, y[hy][t][j], t ? part[u][j] : zero);
             }
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(64 * MAXW, MINB) int4_gemm_kernel(const Int4Ar
             return;
         }
         const int n_idx = (first_tile + i) * 16 + 4 * g, m_idx = tm * 4 * XU + 16 * j + r;
-        if (r < ROWS && m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * 16.0f);
+        if (r < ROWS && m_idx < a.m && n_idx < a.n) int4_store4(a, m_idx, n_idx, v * kInt4OutOfUnits);
     };
     if (KW == 1) {
 #pragma unroll

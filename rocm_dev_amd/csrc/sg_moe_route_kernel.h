@@ -17,9 +17,9 @@ __device__ __forceinline__ void halve(double (&v)[N], int o) {
 }
 
 // logits[t][e] = sum_k X[t][k] * R[e][k].  A workgroup of four waves an expert and up to TOKENS (1, 8) tokens: it reads the expert's row once.
-// Which experts are chosen is decided by these sums, so they are held in 64 bits - products of bf16 are exact in fp32, eight of
-// them are added in fp32, those sums in fp64 - and rounded to fp32 once: which expert comes first does not depend on an
-// order of summation but where two logits are equal to fp32's last bit.
+// Which experts are chosen is decided by these sums, so they are held in 64 bits - a product of bf16 is exact there, whatever its size - and
+// rounded to fp32 once: an order of summation could only show where a sum lies within 2^-53 of its terms' size of a border between two
+// fp32 values.
 template <int TOKENS>
 __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
     __shared__ double of_wave[4][TOKENS];
@@ -44,14 +44,13 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const MoeArgs a) {
         for (int h = 0; h < 2; h++) {
             if (h && second == p) break;
 #pragma unroll
-            for (int t = 0; t < TOKENS; t++) {
-                float s = 0.0f;
+            for (int j = 0; j < 4; j++) {
+                const double lo = bf16_lo(w[h][j]), hi = bf16_hi(w[h][j]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    s = fmaf(bf16_lo(w[h][j]), bf16_lo(v[h][t][j]), s);
-                    s = fmaf(bf16_hi(w[h][j]), bf16_hi(v[h][t][j]), s);
+                for (int t = 0; t < TOKENS; t++) {
+                    sum[t] = fma(lo, (double)bf16_lo(v[h][t][j]), sum[t]);
+                    sum[t] = fma(hi, (double)bf16_hi(v[h][t][j]), sum[t]);
                 }
-                sum[t] += (double)s;
             }
         }
     }

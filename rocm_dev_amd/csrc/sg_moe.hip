@@ -63,42 +63,56 @@ static int launch_down(MoeArgs& a, hipStream_t stream) {
 
 static bool off_lines(const uint8_t* weights, int columns) { return columns % 128 != 0 || (reinterpret_cast<uintptr_t>(weights) & 127u) != 0; }
 
-// waves: four, or eight where the rings fit (not with 32 rows of activations a stage).
-template <int XU, int N>
-static int launch_down_parts(MoeArgs& a, int waves, hipStream_t stream) {
-    const bool lines = off_lines(a.W2, a.inner);
-    if constexpr (8 * 2 * MoeStages<1, XU, false>::kBytes < kLdsBytes) {
-        if (waves == 8 && lines) {
-            if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, true, 8>(a, stream);
-            if (down_lds<XU, 3, 8>(a) <= kLdsBytes) return launch_down<XU, 3, true, 8>(a, stream);
-        }
-        if (waves == 8 && !lines) {
-            if (down_lds<XU, N, 8>(a) <= kLdsBytes) return launch_down<XU, N, false, 8>(a, stream);
-            if (down_lds<XU, 2, 8>(a) <= kLdsBytes) return launch_down<XU, 2, false, 8>(a, stream);
-        }
+// Builds of the down projections: four waves, or eight where the rings fit (not with 32 rows of activations a stage), on N stages in flight
+// if the LDS holds them.
+template <int XU, int N, bool LINES>
+struct DownBuilds {
+    static constexpr int kFew = LINES ? 3 : 2;
+    static constexpr bool kEight = 8 * 2 * MoeStages<1, XU, false>::kBytes < kLdsBytes;
+    // LDS of the build on that many waves; more than there is: none
+    static size_t lds(const MoeArgs& a, int waves) {
+        if (waves == 4) return down_lds<XU, kFew, 4>(a);
+        if (!kEight) return kLdsBytes + 1;
+        const size_t all = down_lds<XU, N, 8>(a);
+        return all <= kLdsBytes ? all : down_lds<XU, kFew, 8>(a);
     }
-    return lines ? launch_down<XU, 3, true, 4>(a, stream) : launch_down<XU, 2, false, 4>(a, stream);
-}
+    static int launch(MoeArgs& a, int waves, hipStream_t stream) {
+        if constexpr (kEight)
+            if (waves == 8) return down_lds<XU, N, 8>(a) <= kLdsBytes ? launch_down<XU, N, LINES, 8>(a, stream) : launch_down<XU, kFew, LINES, 8>(a, stream);
+        return launch_down<XU, kFew, LINES, 4>(a, stream);
+    }
+};
 
-// How many workgroups share a tile of the down projections, and how many waves they have: eight, one workgroup a CU, or four, two.
-// Shared sums pay a launch that adds them up.  (2064 rows, 40 experts x 1376, 61 tokens: 129 tiles as they are 39.6 us, three workgroups each
+// How many workgroups share a tile of the down projections, and how many waves they have: eight, one workgroup a CU, or four, two where they
+// fit.  Shared sums pay a launch that adds them up.  (2064 rows, 40 experts x 1376, 61 tokens: 129 tiles as they are 39.6 us, three workgroups each
 // 30.8 and 4.6 for the sums.  Sums joined by the last workgroup to arrive instead: 95 us, for the fences that write the L2s back.)
+template <class Builds>
 static int down_splits(const MoeArgs& a, int cu_count, int* waves) {
     const int tiles = a.hidden / 16, most = moe_most_splits(a.hidden);
     const float bytes = a.experts * (1.0f - powf(1.0f - (float)a.top_k / a.experts, (float)a.m)) * a.hidden * (float)a.inner;
     const long long steps = (long long)((a.inner + 127) / 128) * a.top_k;      // of one token: there are more
     float best = 0.0f;
     int splits = 1;
-    *waves = 8;
-    for (int w = 8; w >= 4; w -= 4)
+    *waves = 4;
+    for (int w = 8; w >= 4; w -= 4) {
+        const size_t lds = Builds::lds(a, w);
+        if (lds > kLdsBytes) continue;
+        const int at_once = w == 4 && lds_workgroups(lds) > 1 ? 2 : 1;
         for (int s = 1; s <= most && (s == 1 || steps >= 2ll * s * w); s++) {
-            const int slots = cu_count * (8 / w), all = tiles * s;
+            const int slots = cu_count * at_once, all = tiles * s;
             // of the memory's rate, 6 TB/s: a CU by itself takes in up to 1.4 times its part of it.  Sums are written and read at 4 TB/s.
             const float used = (float)all / (float)((all + slots - 1) / slots * slots), rate = 1.4f * used < 1.0f ? 1.4f * used : 1.0f;
             const float us = bytes / (6.0e6f * rate) + (s > 1 ? 4.0f + (float)s * a.m * a.hidden * 8 / 4e6f : 0.0f);
             if (best == 0.0f || us < 0.97f * best) best = us, splits = s, *waves = w;
         }
+    }
     return splits;
+}
+template <class Builds>
+static int launch_down_of(MoeArgs& a, int cu_count, hipStream_t stream) {
+    int waves;
+    a.splits = down_splits<Builds>(a, cu_count, &waves);
+    return Builds::launch(a, waves, stream);
 }
 
 // Parts of up to 4 * XU tokens; G and N stages in flight a wave.
@@ -106,8 +120,6 @@ template <int XU, int G, int N>
 static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t stream) {
     const int pairs = a.m * a.top_k, most = a.experts < pairs ? a.experts : pairs, steps = (a.hidden + 127) / 128;
     const long long items = (long long)most * (a.inner / 16);
-    int waves;
-    a.splits = down_splits(a, cu_count, &waves);
     // Waves that share an item, and stages in flight: what leaves the least to the last round.
     // (32 rows of activations a stage leave no room for a third one)
     constexpr bool kLines = 4 * 3 * MoeStages<2, XU, true>::kBytes + 4 * 2 * MoeStages<2, XU, true>::kBlocks * 1024 < kLdsBytes;
@@ -127,7 +139,7 @@ static int launch_parts(MoeArgs& a, bool choose, int cu_count, hipStream_t strea
     int rc;
     if (lines) rc = launch_gate_up<XU, kLines ? 3 : 2, kLines>(a, choose, groups, cu_count, stream);
     else rc = shorter ? launch_gate_up<XU, 2, false>(a, choose, groups, cu_count, stream) : launch_gate_up<XU, G, false>(a, choose, groups, cu_count, stream);
-    if (!rc) rc = launch_down_parts<XU, N>(a, waves, stream);
+    if (!rc) rc = off_lines(a.W2, a.inner) ? launch_down_of<DownBuilds<XU, N, true>>(a, cu_count, stream) : launch_down_of<DownBuilds<XU, N, false>>(a, cu_count, stream);
     if (rc || a.splits == 1) return rc;
     moe_sum_kernel<<<(unsigned)((a.m * (long long)a.hidden + 1023) / 1024), 256, 0, stream>>>(a);
     return launched("moe_sum launch");

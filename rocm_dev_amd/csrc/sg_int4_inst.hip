@@ -24,7 +24,7 @@ static int launch_build(Int4Args& a, const Int4Plan& plan, hipStream_t stream) {
 }
 
 // Up to 16 rows a wave has the activations to itself: one tile on up to eight waves (sixteen with four rows), or two on up to eight; four waves of
-// two tiles share them where there are many tiles.  Beyond, waves share them: two or four waves of a tile each, eight of one (two such
+// two tiles share them where there are many tiles, in groups of 64 and 128.  Beyond, waves share them: two or four waves of a tile each, eight of one (two such
 // workgroups a CU, but for 64 rows in groups of 32, which take too many registers) or two.
 template <int FLAGS>
 static int launch_flags(Int4Args& a, const Int4Plan& p, hipStream_t stream) {
@@ -34,7 +34,9 @@ static int launch_flags(Int4Args& a, const Int4Plan& p, hipStream_t stream) {
     case XU * 100 + 12: return launch_build<FLAGS, 2, XU, 1, 2, 8, 1>(a, p, stream);
         SG_ROWS(1) SG_ROWS(2) SG_ROWS(4)
 #undef SG_ROWS
+#if SG_GPS < 4
         case 442: return launch_build<FLAGS, 2, 4, 4, 4, 8, 1>(a, p, stream);
+#endif
 #define SG_ROWS(XU)                                                                    \
     case XU * 100 + 21: return launch_build<FLAGS, 1, XU, 2, 4, 8, 1>(a, p, stream);   \
     case XU * 100 + 41: return launch_build<FLAGS, 1, XU, 4, 4, 8, 1>(a, p, stream);   \

@@ -30,6 +30,7 @@ static size_t gate_up_lds(const MoeArgs& a) {
 }
 template <int XU, int DEPTH, bool LINES>
 static int launch_gate_up(MoeArgs& a, bool choose, long long groups, int cu_count, hipStream_t stream) {
+    using Stages = MoeStages<2, XU, LINES>;
     const size_t lds = gate_up_lds<XU, DEPTH>(a);
     const long long at_once = (long long)lds_workgroups(lds) * cu_count;
     const unsigned grid = (unsigned)(groups < at_once ? groups : at_once);
@@ -38,7 +39,12 @@ static int launch_gate_up(MoeArgs& a, bool choose, long long groups, int cu_coun
     a.stride_tiles = (int)(stride % (a.inner / 16));
     a.turn = (uint32_t)(0x100000000ull * (1u << a.share_log) / (unsigned)((a.hidden + 127) / 128) + 1);
     a.inv_tiles = div_reciprocal((unsigned)a.inner / 16);
-    auto* const kernel = choose ? moe_gate_up_kernel<XU, DEPTH, LINES, true> : moe_gate_up_kernel<XU, DEPTH, LINES, false>;
+    auto* kernel = moe_gate_up_kernel<XU, DEPTH, LINES, false>;
+    if constexpr (Stages::kRows <= kMoeFused) {      // (wider parts are for more tokens: part_columns)
+        if (choose) kernel = moe_gate_up_kernel<XU, DEPTH, LINES, true>;
+    } else if (choose) {
+        return SG_INVALID_CONFIG;
+    }
     static LdsGranted granted[2];
     if (int rc = request_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, granted[choose])) return rc;
     kernel<<<grid, 256, lds, stream>>>(a);
@@ -159,7 +165,7 @@ static int part_columns(const MoeArgs& a) {
         for (int c = 0; c < 4; c++) cost[c] += chance * (float)((n - 1) / (4 << c) + 1) * (6.0f + 0.2f * (1 << c));
     }
     int best = 0;
-    for (int c = 1; c < 4; c++)
+    for (int c = 1; c < 4 && 2 << c < a.m; c++)              // (twice the columns of a part that holds all tokens cost more)
         if (cost[c] < cost[best]) best = c;
     return 1 << best;
 }

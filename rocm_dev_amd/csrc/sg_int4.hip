@@ -1,6 +1,4 @@
 // 4-bit integer weights with group scales: packing, launches and C entry points (include/sgemm.h).
-#include <limits.h>
-
 #include "sg_int4.h"
 
 namespace sg {
@@ -117,6 +115,18 @@ static int launch(Int4Args& a, int group, int flags, const Int4Plan& plan, hipSt
 // graphs may replay side by side, and a call that can get no device memory does without too.
 static int launch_gemm(Int4Args& a, int group, int flags, int cu_count, hipStream_t stream) {
     const Int4Plan plan = int4_plan(a, group, cu_count, true);
+    // A launch has fewer than 2^32 threads: beyond, half of the rows at a time.
+    const long long groups = (long long)((a.tiles - 1) / (plan.nf * plan.nw) + 1) * ((a.m - 1) / (4 * plan.xu) + 1) * plan.splits;
+    if (groups * 64 * plan.kw * plan.nw >= 1ll << 32 && a.m > 64) {
+        const int half = (a.m / 2 + 63) / 64 * 64;
+        Int4Args first = a;
+        first.m = half;
+        if (int rc = launch_gemm(first, group, flags, cu_count, stream)) return rc;
+        a.A += (size_t)half * a.k;
+        a.D += (size_t)half * a.n;
+        a.m -= half;
+        return launch_gemm(a, group, flags, cu_count, stream);
+    }
     if (plan.splits == 1) return launch(a, group, flags, plan, stream);
     if (!stream_is_capturing(stream)) {
         std::lock_guard<std::recursive_mutex> turn(stream_turn(stream));
@@ -154,12 +164,24 @@ int sg_int4_pack(const uint8_t* B, const void* scales, const uint8_t* zeros, uin
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
     const Int4Layout l = int4_layout(n, k, group, flags);
-    const size_t grid = ((size_t)l.tiles * l.steps + 3) / 4;
-    if (grid > INT_MAX) return SG_BAD_ARGUMENT;
-    const Int4PackArgs a{B, static_cast<const uint16_t*>(scales), zeros, P, reinterpret_cast<uint16_t*>(P + l.scales_at), P + l.zeros_at,
-                         n, k, group, b_stride, l.tiles, l.steps, l.gps};
-    int4_pack_kernel<<<(unsigned)grid, 256, 0, static_cast<hipStream_t>(stream)>>>(a);
-    return report_hip("int4_pack launch", hipGetLastError()) == hipSuccess ? SG_SUCCESS : SG_LAUNCH_FAILED;
+    Int4PackArgs a{B, static_cast<const uint16_t*>(scales), zeros, P, reinterpret_cast<uint16_t*>(P + l.scales_at), P + l.zeros_at,
+                   n, k, group, b_stride, l.tiles, l.steps, l.gps};
+    const int most = ((1 << 26) - 4) / l.steps;      // tiles: a launch has fewer than 2^32 threads
+    for (int left = l.tiles;; left -= most) {
+        a.tiles = left < most ? left : most;
+        const size_t grid = ((size_t)a.tiles * l.steps + 3) / 4;
+        int4_pack_kernel<<<(unsigned)grid, 256, 0, static_cast<hipStream_t>(stream)>>>(a);
+        if (report_hip("int4_pack launch", hipGetLastError()) != hipSuccess) return SG_LAUNCH_FAILED;
+        if (left <= most) return SG_SUCCESS;
+        const size_t rows = (size_t)most * 16, at = (size_t)most * l.steps, groups = k / group;
+        a.B += rows * b_stride;
+        a.scales += rows * groups;
+        if (a.zeros) a.zeros += rows * groups;
+        a.n -= (int)rows;
+        a.P += at * 1024;
+        a.PS += at * l.gps * 16;
+        a.PZ += at * l.gps * 16;
+    }
 }
 
 int sg_int4_gemm(const void* A, const uint8_t* P, void* D, int m, int n, int k, int group, int flags, void* stream) {

@@ -293,6 +293,18 @@ extern "C" int sg_rmsnorm_fp8_rows(const void* X, const void* residual, const vo
     DeviceInfo* dev;
     if (int rc = get_device_info(&dev)) return rc;
     auto in = [](const void* p) { return static_cast<const uint8_t*>(p); };
-    return launch(NormArgs{in(X), in(residual), in(weight), static_cast<uint8_t*>(sum), static_cast<uint8_t*>(Y), Q, scales, eps, rows, cols},
-                  dev->cu_count, static_cast<hipStream_t>(stream));
+    NormArgs a{in(X), in(residual), in(weight), static_cast<uint8_t*>(sum), static_cast<uint8_t*>(Y), Q, scales, eps, rows, cols};
+    constexpr int kMost = 1 << 21;      // a launch has fewer than 2^32 threads, a row up to 1024 of them
+    for (int left = rows;; left -= kMost) {
+        a.rows = left < kMost ? left : kMost;
+        if (int rc = launch(a, dev->cu_count, static_cast<hipStream_t>(stream))) return rc;
+        if (left <= kMost) return SG_SUCCESS;
+        const size_t values = (size_t)kMost * cols;
+        a.X += 2 * values;
+        if (a.residual) a.residual += 2 * values;
+        if (a.sum) a.sum += 2 * values;
+        if (a.Y) a.Y += 2 * values;
+        a.Q += values;
+        a.scales += kMost;
+    }
 }

@@ -389,10 +389,11 @@ int sg_mxfp4_gemm_fp8act(const uint8_t* A, const uint8_t* P, void* D_bf16, const
  * activations are E4M3 (sg_skinny_gemm_rowcol, sg_mxfp4_gemm_fp8act), the residual's addition before it.  No counterpart in
  * the reference.
  *     v = X, or bf16(X + residual);   y = v * weight / sqrt(mean over the row of v^2 + eps)   (fp32)
- *     scales[r] = absmax(y[r,:]) / 448 (1 if that is zero; NaNs do not count);   Q = e4m3_rne_sat(y / scales[r]), a NaN 0x7f
+ *     scales[r] = absmax(y[r,:]) / 448 (1 if that quotient is zero or the row holds a NaN);   Q = e4m3_rne_sat(y / scales[r]), a NaN 0x7f
  * and, each if its pointer is not NULL, sum = v (the next residual) and Y = bf16(y) (a router's input).  residual and weight
  * ([cols]) may be NULL: nothing added, factors of 1.  sum may be X's or the residual's own memory; Q and Y overlap no input.
- * The squares' sum is fp32, in an order fixed by rows and cols.  A row where it is not finite has y = 0, or NaN where v * weight is not finite.  cols must be a multiple of 16, all
+ * The squares' sum is fp32, in an order fixed by rows and cols (squares below 2^-126 as its subnormals hold them).  A row where it overflows has
+ * y = 0, or NaN where v * weight is not finite; a row with a NaN is NaN throughout.  cols must be a multiple of 16, all
  * matrices and weight 16-byte aligned, scales 4-byte, eps finite and not negative. */
 int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const void* weight_bf16, void* sum_bf16, void* Y_bf16,
                         uint8_t* Q, float* scales, float eps, int rows, int cols, void* stream);
@@ -406,9 +407,12 @@ int sg_rmsnorm_fp8_rows(const void* X_bf16, const void* residual_bf16, const voi
  * sg_int4_packed_bytes(n, k, group, flags) bytes (0 for what sg_int4_pack refuses), all of which are written.  sg_int4_gemm takes
  * that P with the same n, k, group and flags.  Any m >= 1; it is made for few rows, and beyond 64 reads the weights again for every 64.
  * Sums are fp32, in an order fixed by the shape: results are bit-reproducible.  Within a group the sum of A * (1 + B / 16) is corrected by the sum of A,
- * so a row of A with an infinity or a NaN has NaN outputs.  Few weight rows with a long k share K among workgroups, in the stream's
- * workspace (above), except under capture, where a launch uses none - its sums may then be added up in another order than an eager
- * call's - as a call does that can get no device memory.
+ * so a row of A with an infinity or a NaN has NaN outputs; of finite activations no sum overflows within a group.  P does not record what it was packed
+ * with: another k, group or flag of the same size - scales of the other type have the same size always - gives wrong results, and no error.
+ * Shapes whose tiles alone leave CUs idle (few weight rows with a long k; above 16 rows most that do not come out in whole rounds of
+ * workgroups, 64 x 10240 x 8192 for one) share K among workgroups, in the stream's workspace (above), except under capture, where a launch
+ * uses none - its sums may then be added up in another order than an eager call's, and it may take longer - as a call does that can get no
+ * device memory.
  * B, A and P 16-byte aligned (A's rows are k values apart), b_stride a multiple of 16 and at least k / 2, D 8-byte, scales 2-byte aligned. */
 #define SG_INT4_ZEROS 1
 #define SG_INT4_F16_SCALES 2

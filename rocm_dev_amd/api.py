@@ -733,7 +733,8 @@ def int4_pack(B, scales, P, zeros=None, check=False):
 
 def int4_gemm(A, P, D, group=128, zeros=False, scale_dtype=torch.bfloat16, check=False):
     """D[m,n] = bf16(A @ B^T), A [m, k] bfloat16, B packed into P (int4_pack) in groups of `group` columns, with zeros or without, its
-    scales in scale_dtype."""
+    scales in scale_dtype.  P does not record these: its size is checked, but that is the same for both types of scales, and with the
+    other one the results are wrong."""
     flags = _int4_flags(zeros, scale_dtype)
     rc = host.int4_gemm(A, P, D, group, flags)
     if rc is not None:

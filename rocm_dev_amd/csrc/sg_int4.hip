@@ -56,15 +56,15 @@ __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4PackArgs a) {
 // three times as many and at most eight rows (1 x 11008 x 4096 7.5, two 8.0; 13 rows 11.4, 9.9), two elsewhere (5 x 28672 x 4096 15.1,
 // one 15.6), on as many waves as leave each a few steps: 1 x 3712 x 10944, groups of 64, sixteen 8.1, eight 9.8; 1 x 6144 x 4096 eight
 // 5.8, four 6.6, two 9.5; 1 x 28672 x 4096 two 13.9, four 14.8, eight 15.7, in groups of 32 19.2, 17.9, 19.5.  With more than eight rows and
-// many tiles the activations are what goes to a CU most: four waves share them (13 x 28672 x 4096 14.6, each its own 16.3; in groups
-// of 32 19.3 and 19.8, 57344 x 8192 67.5 and 63.1).  K splits where idle CUs can take them and the steps that a
+// many tiles the activations are what goes to a CU most: four waves share them (13 x 28672 x 4096 14.6, each its own 16.3), but not
+// in groups of 32 (19.3 and 19.8, 57344 x 8192 67.5 and 63.1).  K splits where idle CUs can take them and the steps that a
 // wave has left outweigh the second launch: 1 x 1024 x 32768 14.3 -> 9.8, 8 x 512 x 16384 10.9 -> 7.3.
 //
 // Beyond, the waves' vector and matrix units bound what a workgroup does, so that its time is its steps times that of one, and a product's
 // that of its rounds of workgroups.  The four ways - two or four waves of one tile and groups of them that share K, eight of one tile, eight
-// of two - and their K splits are compared by that.  64 rows, groups of 64, without the splits' second launch (5): 57344 x 8192 110 (two tiles on
-// eight waves; 211 on two waves of one), 10240 x 8192 24.4 (the same, six splits; unsplit 91, 39 on four waves), 8192 x 28672 54.6 (eight
-// splits; 98 on two waves).
+// of two - and their K splits are compared by that.  64 rows, groups of 64: 57344 x 8192 101 (two tiles on eight waves; twice that on two waves of one),
+// 10240 x 8192 32 with the splits' second launch (the same, six splits; unsplit 38 on four waves), 8192 x 8192 26 (30), 8192 x 28672 54
+// (eight splits; unsplit 91).
 Int4Plan int4_plan(const Int4Args& a, int group, int cu_count, bool workspace) {
     Int4Plan p{1, a.m <= 4 ? 1 : a.m <= 8 ? 2 : a.m <= 16 ? 4 : a.m <= 32 ? 8 : 16, 1, 1, 1};
     if (p.xu <= 4) {

@@ -183,7 +183,11 @@ __device__ __forceinline__ void moe_issue_scales(const float* first, const float
     if (lane < (second ? 32 : 16)) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(slot) : "memory", "m0");
 }
 
-// h = bf16( silu(S1 * (gate x)) * (S1 * (up x)) ).  An item is 16 gate rows and their 16 up rows of a part of the plan; `share` of a
+// h = bf16( silu(S1 * (gate x)) * (S1 * (up x)) ): rounded to bf16, since the second product's instruction takes nothing wider at its rate.  It
+// shows as one more rounding of an output's size, 2.3e-3 in the norm against 1.65e-3.  Two bf16 parts would undo that but double the activations of the down
+// projections, which cost as much of the way into a CU as the weights: by the next wider builds 112.9 -> 126.1 us for 32 tokens on 128 experts and
+// 29.7 -> 44.2 for 61 on 40 off their lines (8 tokens or one: the same within 1 %, but then a token's result would hang on how many come with it).
+// An item is 16 gate rows and their 16 up rows of a part of the plan; `share` of a
 // workgroup's four waves share its columns, a range each, and meet in LDS.  A wave's ring runs from one item into the next.
 // LDS: plan, the waves' scales, [4 waves][2 * blocks][64 lanes] f32x4 where waves share, then the rings, and before them in their place
 // the room for the plan.

@@ -2,9 +2,9 @@
 //
 //   v = bf16(X + residual);   y = v * w * rstd,  rstd = 1 / sqrt(sum(v^2) / cols + eps);   s = absmax(y) / 448;   Q = e4m3(y / s)
 //
-// v * w is a product of two bf16 values, exact in fp32, and rstd is one factor of the whole row, so absmax(y) is rstd * max|v * w|
-// to the bit: the sum of squares and the maximum come out of the same pass over the row and one reduction.  A row is held
-// in registers between the reduction and the codes: it is read from memory once.
+// v * w is a product of two bf16 values, exact in fp32 (above 2^-133, or wherever |w| >= 2^-9), and rstd is one factor of the whole
+// row, so absmax(y) is rstd * max|v * w| to the bit: the sum of squares and the maximum come out of the same pass over the row
+// and one reduction.  A row is held in registers between the reduction and the codes: it is read from memory once.
 // fp32 throughout; roundings to fewer bits are the three outputs' own (v as bf16, since the next layer adds to what is
 // stored; the codes; Y).  y / s is one product, v * w with rstd / s: y itself carries the rounding of its sum of squares, so that a correctly rounded
 // quotient (as the encoder's, whose input is exact) would mean nothing here.
